@@ -1,0 +1,182 @@
+"""Activation checkpoints in 8 bits: what a layer's backward pass needs of its input, kept as int8 codes with one float32 scale per 64 neighbouring values (1.06 bytes per value
+instead of 4), as HIP kernels (include/ur5learn.h, csrc/ur5_act8.h).
+
+``pack`` / ``PackedActivation.unpack`` are the checkpoint itself; ``PackedActivation.weight_grad`` is a pointwise convolution's weight gradient that reads the codes as they are;
+``pointwise_conv`` is such a layer; ``saved_activations`` keeps every activation that a network saves for its backward pass this way (``agent.Learner(activations="int8")``). The
+forward pass is unchanged; gradients see activations that are off by at most half a step, 1/254 of the largest of their 64 neighbours.
+
+Tensors are float32 / float16 / bfloat16 on the GPU; work is queued on the current stream of their device; there is no CPU fallback.
+"""
+from __future__ import annotations
+
+import threading
+
+import torch
+
+from . import native
+from .policy import DTYPES, _gpu
+
+GROUP = 64
+_active = threading.local()
+
+
+def _stream(t):
+    return torch.cuda.current_stream(t.device).cuda_stream
+
+
+def _float_gpu(t, what):
+    _gpu(t, what)
+    if t.dtype not in DTYPES:
+        raise TypeError(f"{what} must be float32, float16 or bfloat16, not {t.dtype}")
+
+
+class PackedActivation:
+    """Codes int8 [planes, groups, 64], scales float32 [planes, groups], and the shape and type that ``unpack`` restores."""
+    __slots__ = ("codes", "scales", "shape", "dtype")
+
+    def __init__(self, codes, scales, shape, dtype):
+        self.codes, self.scales, self.shape, self.dtype = codes, scales, shape, dtype
+
+    def _size(self):
+        return _planes(self.shape)[1]
+
+    def unpack(self):
+        x = torch.empty(self.shape, dtype=self.dtype, device=self.codes.device)
+        if x.numel():
+            lib = native.load()
+            native.check(lib, lib.ur5_act8_unpack(self.codes.data_ptr(), self.scales.data_ptr(), self.codes.shape[0], self._size(), x.data_ptr(), DTYPES[self.dtype],
+                                                  x.device.index, _stream(x)), "ur5_act8_unpack")
+        return x
+
+    def weight_grad(self, dy, bias=True):
+        """For a pointwise convolution y[n, o] = sum_c w[o, c] x[n, c] + b[o] of the packed x [N, C, ...]: (dw float32 [O, C], db float32 [O]) from dy [N, O, ...] -- sums over images
+        and pixels, the same every time. bias=False: (dw, None)."""
+        _float_gpu(dy, "dy")
+        if len(self.shape) < 3 or dy.dim() != len(self.shape) or dy.shape[0] != self.shape[0] or dy.shape[2:] != self.shape[2:] or dy.device != self.codes.device:
+            raise ValueError(f"dy must be [N, O, ...] like the packed {tuple(self.shape)} on {self.codes.device}, not {tuple(dy.shape)} on {dy.device}")
+        n, cin, cout = self.shape[0], self.shape[1], dy.shape[1]
+        dw = torch.empty((cout, cin), dtype=torch.float32, device=dy.device)
+        db = torch.empty(cout, dtype=torch.float32, device=dy.device) if bias else None
+        if dy.numel() == 0 or cin == 0:
+            return dw.zero_(), db.zero_() if bias else None
+        dy = dy.detach().contiguous()
+        lib = native.load()
+        work = torch.empty(max(1, lib.ur5_act8_wgrad_work_bytes(n, cin, cout, self._size())), dtype=torch.uint8, device=dy.device)
+        native.check(lib, lib.ur5_act8_wgrad(self.codes.data_ptr(), self.scales.data_ptr(), dy.data_ptr(), DTYPES[dy.dtype], n, cin, cout, self._size(), dw.data_ptr(),
+                                             db.data_ptr() if bias else None, work.data_ptr(), work.numel(), dy.device.index, _stream(dy)), "ur5_act8_wgrad")
+        return dw, db
+
+
+def _planes(shape):
+    """(planes, values per plane): groups never reach over a plane's end. [N, C, ...] has N C planes, a matrix its rows, a vector is one plane."""
+    lead = min(2, len(shape) - 1)
+    planes = size = 1
+    for d in shape[:lead]:
+        planes *= d
+    for d in shape[lead:]:
+        size *= d
+    return planes, size
+
+
+def pack(x):
+    """``PackedActivation`` of a tensor of any shape (at least one dimension): per group of 64 neighbouring values of a plane, scale = largest magnitude / 127 and code = the nearest
+    integer to value / scale. A group that holds an infinity or a NaN is restored as NaN throughout, one below 1e-30 as zeros."""
+    _float_gpu(x, "x")
+    if x.dim() < 1:
+        raise ValueError("a scalar has no activations to pack")
+    planes, size = _planes(x.shape)
+    groups = -(-size // GROUP)
+    codes = torch.empty((planes, groups, GROUP), dtype=torch.int8, device=x.device)
+    scales = torch.empty((planes, groups), dtype=torch.float32, device=x.device)
+    if x.numel():
+        lib, src = native.load(), x.detach().contiguous()
+        native.check(lib, lib.ur5_act8_pack(src.data_ptr(), DTYPES[x.dtype], planes, size, codes.data_ptr(), scales.data_ptr(), x.device.index, _stream(x)), "ur5_act8_pack")
+    return PackedActivation(codes, scales, x.shape, x.dtype)
+
+
+class _PointwiseConv(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias):
+        n, c = x.shape[:2]
+        w = weight.reshape(weight.shape[0], c)
+        y = torch.matmul(w, x.reshape(n, c, -1))
+        if bias is not None:
+            y = y + bias.view(1, -1, 1)
+        kept = pack(x)
+        ctx.save_for_backward(kept.codes, kept.scales, weight)
+        ctx.shape, ctx.dtype, ctx.has_bias = x.shape, x.dtype, bias is not None
+        return y.view(n, w.shape[0], *x.shape[2:])
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        codes, scales, weight = ctx.saved_tensors
+        dx = dw = db = None
+        n, cin, cout = ctx.shape[0], ctx.shape[1], weight.shape[0]
+        if ctx.needs_input_grad[0]:
+            dx = torch.matmul(weight.reshape(cout, cin).t().contiguous(), dy.reshape(n, cout, -1)).view(ctx.shape)
+        if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
+            dw, db = PackedActivation(codes, scales, ctx.shape, ctx.dtype).weight_grad(dy, bias=ctx.has_bias)
+            dw = dw.view(weight.shape).to(weight.dtype)
+            db = db.to(weight.dtype) if ctx.has_bias else None
+        return dx, dw, db
+
+
+def pointwise_conv(x, weight, bias=None):
+    """1 x 1 convolution [N, C, ...] -> [N, O, ...] (weight [O, C] or [O, C, 1, 1]) whose input is kept in 8 bits for the weight gradient. Same result and input gradient as the
+    plain layer."""
+    _float_gpu(x, "x")
+    if x.dim() < 3 or weight.numel() != weight.shape[0] * x.shape[1] or weight.dtype != x.dtype or weight.device != x.device:
+        raise ValueError(f"weight {tuple(weight.shape)} {weight.dtype} does not fit x {tuple(x.shape)} {x.dtype}")
+    return _PointwiseConv.apply(x, weight, bias)
+
+
+class _Relu(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x):
+        y = torch.relu(x)
+        ctx.save_for_backward(y > 0)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        return dy * ctx.saved_tensors[0]
+
+
+def relu(x):
+    """ReLU that keeps which values are positive (a byte each) for its backward pass, not the values: a checkpoint rounds the smallest positive ones to zero, about 1 % of them, and
+    without their gradient a layer's would be off by 10 % where its other values' rounding costs 0.3 %."""
+    return _Relu.apply(x)
+
+
+def active():
+    """Whether this thread is inside ``saved_activations``."""
+    return getattr(_active, "depth", 0) > 0
+
+
+class saved_activations:
+    """Context manager for a forward pass: floating-point GPU tensors of three or more dimensions (activations; parameters are left alone) that autograd saves inside it are kept as
+    8-bit checkpoints of at least ``min_values`` values and restored when their backward runs. In it, ``qnet``'s pointwise convolutions keep theirs for ``weight_grad`` and its ReLUs which values are positive (``relu``)."""
+
+    def __init__(self, min_values=4096):
+        self.min_values = int(min_values)
+
+    def _pack(self, t):
+        if not (t.is_cuda and t.dtype in DTYPES and t.dim() >= 3 and t.numel() >= self.min_values) or (t.is_leaf and t.requires_grad):
+            return t
+        return pack(t)
+
+    @staticmethod
+    def _unpack(t):
+        return t.unpack() if isinstance(t, PackedActivation) else t
+
+    def __enter__(self):
+        self._hooks = torch.autograd.graph.saved_tensors_hooks(self._pack, self._unpack)
+        self._hooks.__enter__()
+        _active.depth = getattr(_active, "depth", 0) + 1
+        return self
+
+    def __exit__(self, *exc):
+        _active.depth -= 1
+        return self._hooks.__exit__(*exc)

@@ -1,0 +1,292 @@
+// ur5learn.hip -- C ABI of include/ur5learn.h: argument checks, launch shapes and dispatch over types for the device code of ur5_policy.h and ur5_act8.h. Nothing of the
+// simulation engine is touched; the entry points share libur5sim.so and its error text.
+#include <hip/hip_runtime.h>
+#include <cstdint>
+#include <cstdio>
+#include "../../include/ur5learn.h"
+#include "ur5_act8.h"
+#include "ur5_policy.h"
+
+extern "C" int ur5_learn_fail(int code, const char* text);   // ur5sim.hip: the library's error text
+
+namespace {
+using namespace ur5policy;
+
+int fail(int code, const char* entry, const char* text) {
+  char line[256];
+  snprintf(line, sizeof line, "%s: %s", entry, text);
+  return ur5_learn_fail(code, line);
+}
+// the caller's current device stays what it was
+struct OnDevice {
+  int before = -1;
+  hipError_t error = hipSuccess;
+  explicit OnDevice(int device) {
+    int now = -1;
+    error = hipGetDevice(&now);
+    if (error == hipSuccess && now != device && (error = hipSetDevice(device)) == hipSuccess) before = now;
+  }
+  ~OnDevice() { if (before >= 0) (void)hipSetDevice(before); }
+};
+int launched(const char* entry) {
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? 0 : fail(UR5_ERR_DEVICE, entry, hipGetErrorString(e));
+}
+int no_device(const char* entry, hipError_t e) {
+  return e == hipErrorNoDevice ? fail(UR5_ERR_NOGPU, entry, "no HIP device visible: libur5sim.so runs on an MI355X (gfx950) only, there is no CPU fallback") : fail(UR5_ERR_DEVICE, entry, hipGetErrorString(e));
+}
+
+// ---- how rows are cut. A piece is `per` tiles of 2048 actions. About 4096 pieces in all keep 256 CUs busy to the end (8 workgroups fit on a CU); a row of a large batch
+// is not cut finer than that needs, and never into pieces of more than 16 tiles, so that a thread's fp32 sums stay short.
+constexpr int64_t WANTED = 4096, MOST_PER = 16;
+void cut(int64_t rows, int64_t actions, int* splits, int* per) {
+  const int64_t tiles = (actions + TILE - 1) / TILE;
+  int64_t p = rows * tiles / WANTED;
+  p = p < 1 ? 1 : p > MOST_PER ? MOST_PER : p;
+  *splits = (int)((tiles + p - 1) / p);
+  *per = (int)p;
+}
+// workspace: records | a flag per row | states and log ratios of the preference loss
+struct Work { Part* parts; int* counts; RowState* state; double* ratio; };
+int64_t lay_out(int64_t rows, int64_t actions, void* base, Work* w) {
+  int splits, per;
+  cut(rows, actions, &splits, &per);
+  char* p = (char*)base;
+  const int64_t parts = rows * splits * (int64_t)sizeof(Part), state = rows * (int64_t)sizeof(RowState), ratio = (rows + 1) / 2 * 16, counts = (rows + 3) / 4 * 16;
+  if (w) *w = Work{(Part*)p, (int*)(p + parts + state + ratio), (RowState*)(p + parts), (double*)(p + parts + state)};
+  return parts + state + ratio + counts;
+}
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+constexpr int64_t MOST = 0x7fffffff;
+
+// checks what every entry point over rows checks; launches nothing
+const char* check_rows(const ur5_rows* r, Rows* R, Work* w) {
+  if (!r) return "no rows";
+  if (r->dtype != UR5_F32 && r->dtype != UR5_F16 && r->dtype != UR5_BF16) return "dtype must be UR5_F32, UR5_F16 or UR5_BF16";
+  if (r->rows < 0 || r->actions < 1) return "rows must be at least 0 and actions at least 1";
+  if (r->actions > MOST - 2 * TILE * MOST_PER || r->rows > MOST / 64) return "too many rows or actions (2^31 - 65537 actions, 2^25 rows)";
+  int splits, per;
+  cut(r->rows, r->actions, &splits, &per);
+  if (r->rows * splits > MOST - FIRST) return "too many logits in one call";
+  if (r->stride < r->actions && r->rows > 1) return "the row stride is smaller than a row";
+  if (r->ref && r->ref_stride < r->actions && r->rows > 1) return "the reference's row stride is smaller than a row";
+  if (r->mask && (r->mask_len < 1 || r->actions % r->mask_len || r->mask_stride < 0)) return "mask_len must divide actions, and mask_stride be at least 0";
+  if (r->rows && !r->logits) return "no logits";
+  if (r->rows && (!r->work || !aligned16(r->work) || r->work_bytes < lay_out(r->rows, r->actions, nullptr, nullptr))) return "the workspace is missing, not 16-byte aligned, or smaller than ur5_policy_work_bytes";
+  *R = Rows{r->logits, r->ref, r->mask, r->stride, r->ref_stride, r->mask_stride, (int)r->rows, (int)r->actions, (int)(r->mask ? r->mask_len : r->actions), splits, per};
+  if (w) lay_out(r->rows, r->actions, r->work, w);
+  return nullptr;
+}
+
+template <typename F> void by_type(int dtype, F f) { dtype == UR5_F32 ? f(f32_t{}) : dtype == UR5_F16 ? f(f16_t{}) : f(bf16_t{}); }
+struct yes { static constexpr bool value = true; };
+struct no { static constexpr bool value = false; };
+template <typename F> void by_flag(bool b, F f) { b ? f(yes{}) : f(no{}); }
+
+const char* check_clip(const ur5_rows* r, const ur5_clip* c) {
+  if (!c || (r->rows && (!c->action || !c->old_logp || !c->advantage))) return "action, old_logp and advantage are needed";
+  if (!(c->clip_low >= 0 && c->clip_low <= 1) || !(c->clip_high >= 0)) return "clip_low must lie in [0, 1] and clip_high be at least 0";
+  if (!(c->kl_coef >= 0) || c->entropy_coef != c->entropy_coef) return "kl_coef must be at least 0 and entropy_coef a number";
+  if (c->kl_coef > 0 && !r->ref && r->rows) return "kl_coef needs reference logits";
+  return nullptr;
+}
+Clip clip_of(const ur5_clip* c) { return Clip{c->action, c->old_logp, c->advantage, c->clip_low, c->clip_high, c->kl_coef, c->entropy_coef, c->grad_scale, c->upstream}; }
+const char* check_prefer(const ur5_rows* r, const ur5_prefer* p) {
+  if (!p || (r->rows && (!p->action || !p->ref_logp))) return "action and ref_logp are needed";
+  if (p->pairs < 1 || p->pairs > MOST / 4 || !p->offsets) return "pairs must be at least 1, with 2 pairs + 1 offsets";
+  if (!(p->beta > 0) || !(p->label_smoothing >= 0 && p->label_smoothing <= 0.5)) return "beta must be above 0 and label_smoothing lie in [0, 0.5]";
+  return nullptr;
+}
+Prefer prefer_of(const ur5_prefer* p) { return Prefer{p->action, p->ref_logp, p->offsets, (int)p->pairs, p->beta, p->label_smoothing, p->grad_scale, p->upstream}; }
+
+void stats(const Rows& R, int dtype, hipStream_t s, const int64_t* action, const Work& w) {
+  if (!R.rows) return;
+  by_type(dtype, [&](auto t) { by_flag(R.mask, [&](auto m) { by_flag(R.ref, [&](auto q) {
+    ur5_policy_stats<decltype(t), decltype(m)::value, decltype(q)::value><<<R.rows * R.splits, THREADS, 0, s>>>(R, action, w.parts, w.counts);
+  }); }); });
+}
+void clip_grad(const Rows& R, int dtype, hipStream_t s, const Clip& C, const Work& w, void* grad, float* loss, float* logp, float* kl, float* entropy) {
+  by_type(dtype, [&](auto t) { by_flag(R.mask, [&](auto m) { by_flag(R.ref, [&](auto q) {
+    ur5_policy_clip_grad<decltype(t), decltype(m)::value, decltype(q)::value><<<FIRST + R.rows * R.splits, THREADS, 0, s>>>(R, C, w.parts, w.counts, grad, loss, logp, kl, entropy);
+  }); }); });
+}
+}  // namespace
+
+#define CHECK(text) do { const char* why_ = (text); if (why_) return fail(UR5_ERR_ARG, __func__, why_); } while (0)
+#define ON(device) OnDevice on_(device); if (on_.error != hipSuccess) return no_device(__func__, on_.error)
+
+extern "C" {
+
+int64_t ur5_policy_work_bytes(int64_t rows, int64_t actions) {
+  if (rows < 0 || actions < 1 || rows > MOST / 64 || actions > MOST) return 0;
+  return lay_out(rows, actions, nullptr, nullptr);
+}
+
+int ur5_policy_sample(const ur5_rows* r, uint64_t offset, const int64_t* gids, int64_t* action, float* logp) {
+  Rows R; Work w;
+  CHECK(check_rows(r, &R, &w));
+  if (!R.rows) return 0;
+  if (!gids || !action || !logp) return fail(UR5_ERR_ARG, __func__, "gids, action and logp are needed");
+  ON(r->device);
+  const hipStream_t s = (hipStream_t)r->stream;
+  Draw* draws = (Draw*)w.parts;
+  by_type(r->dtype, [&](auto t) {
+    by_flag(R.mask, [&](auto m) { ur5_policy_sample<decltype(t), decltype(m)::value><<<R.rows * R.splits, THREADS, 0, s>>>(R, offset, gids, draws, action, logp); });
+    if (R.splits > 1) ur5_policy_sample_rows<decltype(t)><<<(R.rows + 3) / 4, THREADS, 0, s>>>(R, draws, action, logp);
+  });
+  return launched(__func__);
+}
+
+int ur5_policy_logp(const ur5_rows* r, const int64_t* action, float* logp, float* entropy) {
+  Rows R; Work w;
+  CHECK(check_rows(r, &R, &w));
+  if (!R.rows) return 0;
+  if (!action || !logp) return fail(UR5_ERR_ARG, __func__, "action and logp are needed");
+  ON(r->device);
+  const hipStream_t s = (hipStream_t)r->stream;
+  by_type(r->dtype, [&](auto t) {
+    by_flag(R.mask, [&](auto m) { ur5_policy_logp<decltype(t), decltype(m)::value><<<R.rows * R.splits, THREADS, 0, s>>>(R, action, w.parts, logp, entropy); });
+    if (R.splits > 1) ur5_policy_logp_rows<decltype(t)><<<(R.rows + 3) / 4, THREADS, 0, s>>>(R, action, w.parts, logp, entropy);
+  });
+  return launched(__func__);
+}
+
+int ur5_policy_clip_loss(const ur5_rows* r, const ur5_clip* c, float* loss, float* logp, float* kl, float* entropy) {
+  Rows R; Work w;
+  CHECK(check_rows(r, &R, &w));
+  CHECK(check_clip(r, c));
+  if (!loss || (R.rows && (!logp || !kl || !entropy))) return fail(UR5_ERR_ARG, __func__, "loss, logp, kl and entropy are needed");
+  ON(r->device);
+  const hipStream_t s = (hipStream_t)r->stream;
+  stats(R, r->dtype, s, c->action, w);
+  by_type(r->dtype, [&](auto t) { by_flag(R.ref, [&](auto q) {
+    ur5_policy_clip_loss<decltype(t), decltype(q)::value><<<1, THREADS, 0, s>>>(R, clip_of(c), w.parts, w.counts, loss, logp, kl, entropy);
+  }); });
+  return launched(__func__);
+}
+
+int ur5_policy_clip_grad(const ur5_rows* r, const ur5_clip* c, void* grad) {
+  Rows R; Work w;
+  CHECK(check_rows(r, &R, &w));
+  CHECK(check_clip(r, c));
+  if (!R.rows) return 0;
+  if (!grad) return fail(UR5_ERR_ARG, __func__, "grad is needed");
+  ON(r->device);
+  clip_grad(R, r->dtype, (hipStream_t)r->stream, clip_of(c), w, grad, nullptr, nullptr, nullptr, nullptr);
+  return launched(__func__);
+}
+
+int ur5_policy_clip_loss_grad(const ur5_rows* r, const ur5_clip* c, float* loss, float* logp, float* kl, float* entropy, void* grad) {
+  Rows R; Work w;
+  CHECK(check_rows(r, &R, &w));
+  CHECK(check_clip(r, c));
+  if (!loss || (R.rows && (!logp || !kl || !entropy || !grad))) return fail(UR5_ERR_ARG, __func__, "loss, logp, kl, entropy and grad are needed");
+  ON(r->device);
+  stats(R, r->dtype, (hipStream_t)r->stream, c->action, w);
+  clip_grad(R, r->dtype, (hipStream_t)r->stream, clip_of(c), w, grad, loss, logp, kl, entropy);
+  return launched(__func__);
+}
+
+int ur5_policy_prefer_loss(const ur5_rows* r, const ur5_prefer* p, float* loss, float* margin) {
+  Rows R; Work w;
+  CHECK(check_rows(r, &R, &w));
+  CHECK(check_prefer(r, p));
+  if (!loss || !margin) return fail(UR5_ERR_ARG, __func__, "loss and margin are needed");
+  R.ref = nullptr;
+  ON(r->device);
+  const hipStream_t s = (hipStream_t)r->stream;
+  stats(R, r->dtype, s, p->action, w);
+  by_type(r->dtype, [&](auto t) { ur5_policy_prefer_pairs<decltype(t)><<<1, PAIR_THREADS, 0, s>>>(R, prefer_of(p), w.parts, w.counts, w.state, w.ratio, loss, margin); });
+  return launched(__func__);
+}
+
+int ur5_policy_prefer_grad(const ur5_rows* r, const ur5_prefer* p, void* grad) {
+  Rows R; Work w;
+  CHECK(check_rows(r, &R, &w));
+  CHECK(check_prefer(r, p));
+  if (!R.rows) return 0;
+  if (!grad) return fail(UR5_ERR_ARG, __func__, "grad is needed");
+  R.ref = nullptr;
+  ON(r->device);
+  const hipStream_t s = (hipStream_t)r->stream;
+  by_type(r->dtype, [&](auto t) { by_flag(R.mask, [&](auto m) {
+    ur5_policy_prefer_grad<decltype(t), decltype(m)::value><<<R.rows * R.splits, THREADS, 0, s>>>(R, prefer_of(p), w.state, grad);
+  }); });
+  return launched(__func__);
+}
+
+// ---- 8-bit checkpoints
+static const char* check_planes(int dtype, int64_t planes, int64_t size) {
+  if (dtype != UR5_F32 && dtype != UR5_F16 && dtype != UR5_BF16) return "dtype must be UR5_F32, UR5_F16 or UR5_BF16";
+  if (planes < 0 || size < 1 || size > MOST - ur5act8::GROUP || planes > MOST || planes * ((size + ur5act8::GROUP - 1) / ur5act8::GROUP) > MOST) return "planes must be at least 0, a plane of 1 .. 2^31 - 65 values, and all groups below 2^31";
+  return nullptr;
+}
+int ur5_act8_pack(const void* x, int dtype, int64_t planes, int64_t size, int8_t* codes, float* scales, int device, void* stream) {
+  CHECK(check_planes(dtype, planes, size));
+  if (!planes) return 0;
+  if (!x || !codes || !scales || !aligned16(codes)) return fail(UR5_ERR_ARG, __func__, "x, codes (16-byte aligned) and scales are needed");
+  ON(device);
+  const unsigned groups = (unsigned)((size + ur5act8::GROUP - 1) / ur5act8::GROUP), total = (unsigned)(planes * groups), per = ur5act8::THREADS / ur5act8::LANES;
+  by_type(dtype, [&](auto t) {
+    using T = decltype(t);
+    ur5act8::ur5_act8_pack<T><<<(total + per - 1) / per, ur5act8::THREADS, 0, (hipStream_t)stream>>>((const typename T::raw*)x, groups, total, size, codes, scales);
+  });
+  return launched(__func__);
+}
+int ur5_act8_unpack(const int8_t* codes, const float* scales, int64_t planes, int64_t size, void* x, int dtype, int device, void* stream) {
+  CHECK(check_planes(dtype, planes, size));
+  if (!planes) return 0;
+  if (!x || !codes || !scales || !aligned16(codes)) return fail(UR5_ERR_ARG, __func__, "x, codes (16-byte aligned) and scales are needed");
+  ON(device);
+  const unsigned groups = (unsigned)((size + ur5act8::GROUP - 1) / ur5act8::GROUP), total = (unsigned)(planes * groups), per = ur5act8::THREADS / ur5act8::LANES;
+  by_type(dtype, [&](auto t) {
+    using T = decltype(t);
+    ur5act8::ur5_act8_unpack<T><<<(total + per - 1) / per, ur5act8::THREADS, 0, (hipStream_t)stream>>>(codes, scales, groups, total, size, (typename T::raw*)x);
+  });
+  return launched(__func__);
+}
+
+// ---- weight gradient: how the pixels are split. A wavefront of the kernel fills a SIMD's registers, so 256 workgroups fill the card; a multiple of 8 ranges, one set per XCD.
+struct WgradPlan { int o_tiles, c_tiles, wide, splits; int64_t part, bytes; };
+static WgradPlan wgrad_plan(int64_t n, int64_t cin, int64_t cout, int64_t size) {
+  WgradPlan p;
+  p.wide = cin > 64;                                    // 128 input channels per tile, or 64 where there are no more
+  p.o_tiles = (int)((cout + ur5act8::TO - 1) / ur5act8::TO);
+  p.c_tiles = (int)((cin + (p.wide ? 127 : 63)) / (p.wide ? 128 : 64));
+  const int64_t groups = n * ((size + ur5act8::GROUP - 1) / ur5act8::GROUP), tiles = (int64_t)p.o_tiles * p.c_tiles;
+  int64_t s = (256 + tiles - 1) / tiles;
+  if (s > (groups + 3) / 4) s = (groups + 3) / 4;       // a range of at least one group for every wavefront
+  p.splits = (int)((s + 7) / 8 * 8);
+  p.part = ((int64_t)p.splits * cin * cout * 4 + 15) / 16 * 16;
+  p.bytes = p.part + (int64_t)p.splits * 4 * cout * 4;
+  return p;
+}
+static const char* check_wgrad(int64_t n, int64_t cin, int64_t cout, int64_t size) {
+  if (n < 0 || cin < 1 || cout < 1 || cin > 65536 || cout > 65536 || cin * cout > MOST / 8) return "n must be at least 0, channels 1 .. 65536 and their product below 2^28";
+  if (n > 65536) return "n must be at most 65536";
+  return check_planes(UR5_F32, n * (cin > cout ? cin : cout), size);
+}
+int64_t ur5_act8_wgrad_work_bytes(int64_t n, int64_t cin, int64_t cout, int64_t size) { return check_wgrad(n, cin, cout, size) ? 0 : wgrad_plan(n, cin, cout, size).bytes; }
+int ur5_act8_wgrad(const int8_t* codes, const float* scales, const void* dy, int dtype, int64_t n, int64_t cin, int64_t cout, int64_t size, float* dw, float* db,
+                   void* work, int64_t work_bytes, int device, void* stream) {
+  CHECK(check_planes(dtype, n, size));
+  CHECK(check_wgrad(n, cin, cout, size));
+  const WgradPlan p = wgrad_plan(n, cin, cout, size);
+  if (!dw || (n && (!codes || !scales || !dy || !aligned16(codes)))) return fail(UR5_ERR_ARG, __func__, "codes (16-byte aligned), scales, dy and dw are needed");
+  if (!work || !aligned16(work) || work_bytes < p.bytes) return fail(UR5_ERR_ARG, __func__, "the workspace is missing, not 16-byte aligned, or smaller than ur5_act8_wgrad_work_bytes");
+  ON(device);
+  const hipStream_t s = (hipStream_t)stream;
+  float* part = (float*)work;
+  float* part_bias = db ? (float*)((char*)work + p.part) : nullptr;
+  const ur5act8::Wgrad W{codes, scales, dy, size, (int)((size + ur5act8::GROUP - 1) / ur5act8::GROUP), (int)n, (int)cin, (int)cout, p.splits, p.o_tiles, p.c_tiles, part, part_bias};
+  by_type(dtype, [&](auto t) {
+    using T = decltype(t);
+    const int grid = p.splits * p.o_tiles * p.c_tiles;
+    if (p.wide) ur5act8::ur5_act8_wgrad<T, 128><<<grid, ur5act8::THREADS, 0, s>>>(W);
+    else ur5act8::ur5_act8_wgrad<T, 64><<<grid, ur5act8::THREADS, 0, s>>>(W);
+  });
+  const int weights = (int)(cin * cout), outs = weights + (db ? (int)cout : 0);
+  ur5act8::ur5_act8_wgrad_sum<<<(outs + ur5act8::THREADS - 1) / ur5act8::THREADS, ur5act8::THREADS, 0, s>>>(part, part_bias, p.splits, weights, (int)cout, dw, db);
+  return launched(__func__);
+}
+}

@@ -263,3 +263,10 @@ static int be_sync(ur5_sim* h) {
   be_resolve(h, b);
   return 0;
 }
+
+#ifndef UR5_MANY
+// the error text is this unit's: ur5learn.hip sets it through here
+extern "C" __attribute__((visibility("hidden"))) int ur5_learn_fail(int code, const char* text) {
+  try { return ur5host::fail(code, text); } catch (...) { return code; }
+}
+#endif

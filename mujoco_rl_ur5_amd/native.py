@@ -23,6 +23,9 @@ EXPORTS = ["ur5_last_error", "ur5_create", "ur5_destroy", "ur5_num_envs", "ur5_n
            "ur5_get_counters", "ur5_body_xpos", "ur5_render", "ur5_render_dev", "ur5_state_device_ptr"]
 TEST_EXPORTS = ["ur5_forward_debug", "ur5_set_step_cap_dev", "ur5_model_uploads"]   # include/ur5sim_test.h: introspection for tests/ and tools/, not part of the boundary
 
+LEARN_EXPORTS = ["ur5_policy_work_bytes", "ur5_policy_sample", "ur5_policy_logp", "ur5_policy_clip_loss", "ur5_policy_clip_grad", "ur5_policy_clip_loss_grad",
+                 "ur5_policy_prefer_loss", "ur5_policy_prefer_grad", "ur5_act8_pack", "ur5_act8_unpack", "ur5_act8_wgrad_work_bytes", "ur5_act8_wgrad"]   # include/ur5learn.h
+
 
 class Config(C.Structure):
     _fields_ = [("ee_body", C.c_int), ("contacts_enabled", C.c_int), ("pid_dt", C.c_double)]
@@ -34,6 +37,25 @@ class AimRule(C.Structure):
                 ("plate_half_x", C.c_double), ("plate_centre_y", C.c_double), ("plate_half_y", C.c_double), ("z_min", C.c_double), ("z_max", C.c_double),
                 ("grasp_z", C.c_double), ("fallback_x", C.c_double), ("fallback_y", C.c_double),
                 ("z_from_depth", C.c_int), ("pad", C.c_int), ("cam_x0", C.c_double), ("cam_y0", C.c_double), ("cam_dx", C.c_double), ("cam_dy", C.c_double), ("cam_z", C.c_double)]
+
+
+class Rows(C.Structure):
+    """ur5_rows of include/ur5learn.h: rows of logits, where they live and the workspace of the call."""
+    _fields_ = [("logits", C.c_void_p), ("ref", C.c_void_p), ("mask", C.c_void_p), ("stride", C.c_int64), ("ref_stride", C.c_int64), ("mask_stride", C.c_int64),
+                ("rows", C.c_int64), ("actions", C.c_int64), ("mask_len", C.c_int64), ("dtype", C.c_int32), ("device", C.c_int32), ("stream", C.c_void_p),
+                ("work", C.c_void_p), ("work_bytes", C.c_int64)]
+
+
+class Clip(C.Structure):
+    """ur5_clip of include/ur5learn.h."""
+    _fields_ = [("action", C.c_void_p), ("old_logp", C.c_void_p), ("advantage", C.c_void_p), ("clip_low", C.c_float), ("clip_high", C.c_float),
+                ("kl_coef", C.c_float), ("entropy_coef", C.c_float), ("grad_scale", C.c_float), ("upstream", C.c_void_p)]
+
+
+class Prefer(C.Structure):
+    """ur5_prefer of include/ur5learn.h."""
+    _fields_ = [("action", C.c_void_p), ("ref_logp", C.c_void_p), ("offsets", C.c_void_p), ("pairs", C.c_int64), ("beta", C.c_double),
+                ("label_smoothing", C.c_double), ("grad_scale", C.c_float), ("upstream", C.c_void_p)]
 
 
 _libs = {}
@@ -91,8 +113,28 @@ def load(path=None):
         L.ur5_model_uploads.restype = C.c_long
     L.ur5_render.argtypes = [vp, C.c_int, C.c_int, C.c_int, C.c_int, C.POINTER(C.c_uint8), C.POINTER(C.c_float)]
     L.ur5_render_dev.argtypes = [vp, C.c_int, C.c_int, C.c_int, C.c_int, vp, vp]
+    if hasattr(L, "ur5_policy_sample"):                        # the engine's host builds (tests) hold no learning operators
+        i64, i32, rows = C.c_int64, C.c_int, C.POINTER(Rows)
+        L.ur5_policy_work_bytes.argtypes, L.ur5_policy_work_bytes.restype = [i64, i64], i64
+        L.ur5_policy_sample.argtypes = [rows, C.c_uint64, vp, vp, vp]
+        L.ur5_policy_logp.argtypes = [rows, vp, vp, vp]
+        L.ur5_policy_clip_loss.argtypes = [rows, C.POINTER(Clip), vp, vp, vp, vp]
+        L.ur5_policy_clip_grad.argtypes = [rows, C.POINTER(Clip), vp]
+        L.ur5_policy_clip_loss_grad.argtypes = [rows, C.POINTER(Clip), vp, vp, vp, vp, vp]
+        L.ur5_policy_prefer_loss.argtypes = [rows, C.POINTER(Prefer), vp, vp]
+        L.ur5_policy_prefer_grad.argtypes = [rows, C.POINTER(Prefer), vp]
+        L.ur5_act8_pack.argtypes = [vp, i32, i64, i64, vp, vp, i32, vp]
+        L.ur5_act8_unpack.argtypes = [vp, vp, i64, i64, vp, i32, i32, vp]
+        L.ur5_act8_wgrad_work_bytes.argtypes, L.ur5_act8_wgrad_work_bytes.restype = [i64] * 4, i64
+        L.ur5_act8_wgrad.argtypes = [vp, vp, vp, i32, i64, i64, i64, i64, vp, vp, vp, i64, i32, vp]
     _libs[path] = L
     return L
+
+
+def check(lib, rc, what):
+    """Raises what a negative return code of an entry point stands for."""
+    if rc != 0:
+        raise RuntimeError(f"{what} failed ({rc}): {lib.ur5_last_error().decode()}")
 
 
 def _dp(a):

@@ -1,0 +1,322 @@
+"""8-bit activation checkpoints (mujoco_rl_ur5_amd/checkpoint8.py, include/ur5learn.h) against plain implementations in 64 bits, and their use in a network's backward pass."""
+import math
+
+import pytest
+import torch
+import torch.nn as nn
+
+from mujoco_rl_ur5_amd import checkpoint8, native, qnet
+
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+# ------------------------------------------------------------------ host side
+def test_entry_points_refuse_bad_arguments():
+    """Every check runs before the device is asked for anything: no pointer below is ever used."""
+    lib = native.load()
+    ok = dict(x=4096, dtype=0, planes=3, size=100, codes=4096, scales=4096)
+    for change in (dict(x=None), dict(dtype=5), dict(planes=-1), dict(size=0), dict(size=1 << 31), dict(planes=1 << 30, size=1000), dict(codes=None), dict(codes=4100), dict(scales=None)):
+        a = {**ok, **change}
+        assert lib.ur5_act8_pack(a["x"], a["dtype"], a["planes"], a["size"], a["codes"], a["scales"], 0, None) == -1, change
+        assert lib.ur5_act8_unpack(a["codes"], a["scales"], a["planes"], a["size"], a["x"], a["dtype"], 0, None) == -1 and lib.ur5_last_error().startswith(b"ur5_act8_unpack"), change
+    need = lib.ur5_act8_wgrad_work_bytes(2, 3, 5, 100)
+    assert need > 0 and lib.ur5_act8_wgrad_work_bytes(2, 0, 5, 100) == 0 and lib.ur5_act8_wgrad_work_bytes(2, 1 << 17, 5, 100) == 0
+    ok = dict(codes=4096, scales=4096, dy=4096, dtype=0, n=2, cin=3, cout=5, size=100, dw=4096, db=4096, work=4096, bytes=need)
+    for change in (dict(codes=None), dict(codes=4104), dict(scales=None), dict(dy=None), dict(dtype=-1), dict(n=-1), dict(n=1 << 20), dict(cin=0), dict(cout=0), dict(cin=60000, cout=60000), dict(size=0),
+                   dict(dw=None), dict(work=None), dict(work=4100), dict(bytes=need - 1)):
+        a = {**ok, **change}
+        assert lib.ur5_act8_wgrad(*[a[k] for k in ("codes", "scales", "dy", "dtype", "n", "cin", "cout", "size", "dw", "db", "work", "bytes")], 0, None) == -1, change
+
+
+def test_no_cpu_fallback():
+    x = torch.zeros(2, 3, 8)
+    for call in (lambda: checkpoint8.pack(x), lambda: checkpoint8.pointwise_conv(x, torch.zeros(4, 3))):
+        with pytest.raises(ValueError, match="no CPU fallback"):
+            call()
+
+
+def test_host_tensors_and_parameters_are_saved_as_they_are():
+    """Inside saved_activations a forward pass on the host is the plain one, and the state of the context is what it was after leaving it, also by an exception."""
+    net = nn.Conv2d(3, 4, 1)
+    x = torch.randn(2, 3, 50, 50)
+    net(x).sum().backward()
+    want = net.weight.grad.clone()
+    net.zero_grad()
+    assert not checkpoint8.active()
+    with checkpoint8.saved_activations():
+        with checkpoint8.saved_activations():
+            assert checkpoint8.active()
+        assert checkpoint8.active()
+        loss = net(x).sum()
+    loss.backward()
+    assert torch.equal(net.weight.grad, want) and not checkpoint8.active()
+    with pytest.raises(KeyError):
+        with checkpoint8.saved_activations():
+            raise KeyError
+    assert not checkpoint8.active()
+
+
+# ------------------------------------------------------------------ the plain checkpoint, in 64 bits
+def _planes(x):
+    lead = min(2, x.dim() - 1)
+    return x.reshape(math.prod(x.shape[:lead]), -1)
+
+
+def _plain(x):
+    """(codes, scales, what they stand for in 64 bits) of the definition."""
+    v = _planes(x).double()
+    pad = -v.shape[1] % 64
+    v = torch.cat((v, v.new_zeros(v.shape[0], pad)), 1).reshape(v.shape[0], -1, 64)
+    most = v.abs().amax(2)
+    finite = torch.isfinite(v).all(2)
+    scale = torch.where(finite, torch.where(most >= 1e-30, most / 127, 0.0), math.nan).float()
+    top = torch.tensor(torch.finfo(torch.float32).max / 127, device=x.device)          # the scale stays where 127 of it is finite
+    scale = torch.minimum(scale, top if bool(torch.isfinite(127 * top)) else torch.nextafter(top, top.new_zeros(())))
+    live = (finite & (scale > 0))[..., None]
+    code = torch.where(live, torch.round(v / torch.where(live, scale[..., None].double(), 1.0)), 0.0)
+    return code.to(torch.int8), scale, (code * scale[..., None].double()).reshape(v.shape[0], -1)[:, :v.shape[1] * 64 - pad].reshape(x.shape)
+
+
+def _check_pack(x):
+    kept = checkpoint8.pack(x)
+    code, scale, value = _plain(x)
+    assert torch.equal(kept.codes, code) and torch.equal(torch.nan_to_num(kept.scales, nan=-1.0), torch.nan_to_num(scale, nan=-1.0))
+    back = kept.unpack()
+    assert back.shape == x.shape and back.dtype == x.dtype
+    assert torch.equal(torch.nan_to_num(back.float(), nan=-1e30), torch.nan_to_num(value.float().to(x.dtype).float(), nan=-1e30))   # one product, rounded to 32 bits and then to the type
+    return kept, value
+
+
+SHAPES = [(1,), (63,), (64,), (65,), (3, 129), (2, 3, 1), (2, 5, 7, 9), (3, 4, 50, 50), (2, 2, 8, 8, 8), (1, 300, 64), (7, 1, 4096)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", SHAPES)
+def test_pack_and_unpack(shape, dtype):
+    g = torch.Generator().manual_seed(1)
+    for x in (torch.randn(shape, generator=g), torch.relu(torch.randn(shape, generator=g)) * torch.exp(3 * torch.randn(shape, generator=g)), torch.zeros(shape)):
+        _check_pack(x.to(dtype).cuda())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_values_next_to_a_border_of_two_codes(dtype):
+    """Multiples of half a step and their neighbours: whole and half multiples of amax / 127, where the nearest code is decided by the last bit."""
+    amax = torch.tensor([1.0, 127.0, 3.7, 0.011, 1000.3]).to(dtype).float()[:, None]
+    half = torch.arange(-254, 255)[None].float()
+    x = (amax * half / 254).to(dtype).float()
+    bits = torch.cat([x.to(dtype), torch.nextafter(x, x + 1).to(dtype), torch.nextafter(x, x - 1).to(dtype)], dim=1)
+    rows = []
+    for r in range(bits.shape[0]):                              # every group of 64 starts with the largest magnitude
+        for part in bits[r].split(63):
+            rows.append(torch.cat((amax[r].to(dtype), part, part.new_zeros(63 - len(part)))))
+    _check_pack(torch.stack(rows).cuda())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_groups_that_are_tiny_or_not_finite(dtype):
+    x = torch.randn(6, 200, generator=torch.Generator().manual_seed(2)).to(dtype)
+    x[0, 70], x[1, 3], x[2, 199] = math.nan, math.inf, -math.inf
+    x[3] *= 0
+    x[3, 10] = torch.finfo(dtype).smallest_normal if dtype == torch.float16 else 1e-35
+    x[4] = torch.finfo(dtype).max * x[4].sign()
+    kept, _ = _check_pack(x.cuda())
+    back = kept.unpack().cpu()
+    assert torch.isnan(back[0, 64:128]).all() and torch.isfinite(back[0, :64]).all() and torch.isnan(back[1, :64]).all() and torch.isnan(back[2, 192:]).all()
+    assert torch.isfinite(back[4]).all() and (dtype == torch.float16 or (back[3] == 0).all())
+
+
+@pytest.mark.gpu
+def test_strides_offsets_and_empty_tensors():
+    x = torch.randn(4, 6, 9, 11, generator=torch.Generator().manual_seed(3)).cuda()
+    want = checkpoint8.pack(x).unpack()
+    assert torch.equal(checkpoint8.pack(x.to(memory_format=torch.channels_last)).unpack(), want)
+    for dtype in TYPES:
+        buf = torch.zeros(x.numel() + 3, dtype=dtype, device="cuda")
+        view = buf[3:].view(x.shape)                              # an odd number of elements into its buffer
+        view.copy_(x)
+        assert torch.equal(checkpoint8.pack(view).unpack(), checkpoint8.pack(view.clone()).unpack())
+    for shape in ((0,), (0, 5), (3, 0), (2, 0, 4), (2, 3, 0)):
+        e = torch.empty(shape, device="cuda")
+        assert checkpoint8.pack(e).unpack().shape == e.shape
+    with pytest.raises(ValueError):
+        checkpoint8.pack(torch.tensor(1.0).cuda())
+    with pytest.raises(TypeError):
+        checkpoint8.pack(torch.zeros(4, dtype=torch.double).cuda())
+
+
+# ------------------------------------------------------------------ weight gradient
+def _check_wgrad(x, dy, bias=True):
+    """Against 64 bits on the values that the codes stand for. An element is a sum of products that are exact; the kernel adds them in 32 bits, at most
+    64 * 3 within a group and then one per group of its share (plus 4 wavefronts, the splits are added in 64 bits): that many roundings of at most the sum of magnitudes."""
+    kept, value = checkpoint8.pack(x), _plain(x)[2]
+    dw, db = kept.weight_grad(dy, bias=bias)
+    n, cin, cout = x.shape[0], x.shape[1], dy.shape[1]
+    v, d = value.reshape(n, cin, -1).transpose(0, 1).reshape(cin, -1), dy.double().reshape(n, cout, -1).transpose(0, 1).reshape(cout, -1)
+    groups = n * kept.codes.shape[1]
+    roundings = 192 + groups + 8
+    assert dw.shape == (cout, cin) and dw.dtype == torch.float32
+    tol = roundings * 2.0 ** -24 * (d.abs() @ v.abs().t().contiguous()) + 1e-37
+    assert ((dw.double() - d @ v.t().contiguous()).abs() <= tol).all()
+    if bias:
+        assert ((db.double() - d.sum(1)).abs() <= (32 * groups + 8) * 2.0 ** -24 * d.abs().sum(1) + 1e-37).all()
+    else:
+        assert db is None
+    return dw, db
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,cin,cout,size", [(1, 1, 1, 1), (1, 3, 5, 63), (2, 31, 33, 64), (3, 64, 64, 65), (2, 65, 64, 130), (5, 64, 6, 1600), (2, 130, 129, 77), (12, 64, 128, 2500), (40, 17, 200, 10),
+                                             (1, 200, 70, 9001), (300, 5, 7, 3)])
+def test_weight_gradient(n, cin, cout, size, dtype):
+    g = torch.Generator().manual_seed(n + cin + size)
+    x = (torch.relu(torch.randn(n, cin, size, generator=g)) * torch.exp(torch.randn(1, cin, 1, generator=g))).to(dtype).cuda()
+    dy = (1e-3 * torch.randn(n, cout, size, generator=g)).to(dtype).cuda()
+    _check_wgrad(x, dy)
+
+
+@pytest.mark.gpu
+def test_weight_gradient_of_structured_inputs():
+    """Every (output, input) channel pair and pixel is its own: exact small integers, so a swapped lane, row or pixel cannot cancel."""
+    n, cin, cout, size = 3, 70, 67, 150
+    x = torch.zeros(n, cin, size)
+    c, p = torch.arange(cin), torch.arange(cin) * 2 % size
+    x[1, c, p] = 127.0                                          # one pixel per input channel: code 127, scale 1
+    dy = torch.arange(n * cout * size).reshape(n, cout, size).remainder(4093).float()
+    kept = checkpoint8.pack(x.cuda())
+    dw, db = kept.weight_grad(dy.cuda())
+    assert torch.equal(dw.cpu(), 127 * dy[1][:, p]) and torch.equal(db.cpu(), dy.sum(dim=(0, 2)))
+
+
+@pytest.mark.gpu
+def test_weight_gradient_details():
+    g = torch.Generator().manual_seed(4)
+    x, dy = torch.randn(2, 66, 5, 13, generator=g).cuda(), torch.randn(2, 40, 5, 13, generator=g).cuda()
+    dw, db = _check_wgrad(x, dy)
+    assert torch.equal(_check_wgrad(x, dy, bias=False)[0], dw)
+    kept = checkpoint8.pack(x)
+    assert all(torch.equal(kept.weight_grad(dy)[0], dw) for _ in range(5))                                  # the same every time
+    assert torch.equal(kept.weight_grad(dy.to(memory_format=torch.channels_last))[0], dw)
+    odd = torch.zeros(dy.numel() + 1, device="cuda")[1:].view(dy.shape).copy_(dy)                            # rows that are only 4-byte aligned
+    assert torch.equal(kept.weight_grad(odd)[0], dw)
+    for t in (torch.float16, torch.bfloat16):                                                                # the gradient's type need not be the activation's
+        assert torch.allclose(kept.weight_grad(dy.to(t))[0], checkpoint8.pack(x).weight_grad(dy.to(t).float())[0], rtol=1e-4, atol=1e-5)
+    tail = dy.clone()
+    tail[0, 3, -1, -1] = math.inf                                                                            # behind a plane's end there is the next plane: it must not leak
+    bad = kept.weight_grad(tail)[0]
+    rows = torch.arange(40).cuda() != 3
+    assert torch.equal(bad[rows], dw[rows]) and not torch.isfinite(bad[3]).any()
+    y = x.clone()
+    y[1, 7, 2, 2] = math.nan                                                                                 # a group without a scale: its channel is NaN, no other
+    bad = checkpoint8.pack(y).weight_grad(dy)[0]
+    cols = torch.arange(66).cuda() != 7
+    assert torch.equal(bad[:, cols], dw[:, cols]) and torch.isnan(bad[:, 7]).all()
+    e = checkpoint8.pack(torch.empty(0, 4, 9).cuda()).weight_grad(torch.empty(0, 3, 9).cuda())
+    assert torch.equal(e[0], torch.zeros(3, 4).cuda()) and torch.equal(e[1], torch.zeros(3).cuda())
+    for wrong in (dy[:1], dy[:, :, :4], dy.reshape(2, 40, 65), dy.double(), dy.cpu()):
+        with pytest.raises((ValueError, TypeError)):
+            kept.weight_grad(wrong)
+    with pytest.raises(ValueError):
+        checkpoint8.pack(x[0, 0]).weight_grad(x[0, 0])
+
+
+# ------------------------------------------------------------------ in a network
+@pytest.mark.gpu
+@pytest.mark.parametrize("bias", [True, False])
+def test_pointwise_conv(bias):
+    g = torch.Generator().manual_seed(5)
+    x = torch.randn(3, 20, 9, 14, generator=g).cuda().requires_grad_()
+    w = torch.randn(11, 20, 1, 1, generator=g).cuda().requires_grad_()
+    b = torch.randn(11, generator=g).cuda().requires_grad_() if bias else None
+    up = torch.randn(3, 11, 9, 14, generator=g).cuda()
+    y = checkpoint8.pointwise_conv(x, w, b)
+    grads = torch.autograd.grad(y, [t for t in (x, w, b) if t is not None], up)
+    plain = nn.functional.conv2d(x.double(), w.double(), None if b is None else b.double())
+    assert torch.allclose(y.double(), plain, rtol=0, atol=1e-4)
+    want = torch.autograd.grad(plain, [t for t in (x, w, b) if t is not None], up.double())
+    assert torch.allclose(grads[0].double(), want[0].double(), rtol=0, atol=1e-4)
+    assert torch.equal(grads[1].reshape(11, 20), checkpoint8.pack(x).weight_grad(up)[0])
+    # the definition's gradient is the plain one on the restored input
+    back = _plain(x.detach())[2].reshape(3, 20, -1)
+    exact = sum(u @ v.t().contiguous() for u, v in zip(up.double().reshape(3, 11, -1), back))
+    assert torch.allclose(grads[1].reshape(11, 20).double(), exact, rtol=0, atol=1e-3)
+    with pytest.raises(ValueError):
+        checkpoint8.pointwise_conv(x, torch.zeros(11, 19).cuda())
+
+
+def _gradients(net, x, weight, context):
+    net.zero_grad(set_to_none=True)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    with context:
+        y = net(x)
+    kept = torch.cuda.memory_allocated() - before
+    (y * weight).sum().backward()
+    return y.detach(), [p.grad.clone() for p in net.parameters()], kept
+
+
+class _PlainPacked(checkpoint8.PackedActivation):
+    """The checkpoint by the plain definition."""
+
+    def unpack(self):
+        size = math.prod(self.shape[min(2, len(self.shape) - 1):])
+        return (self.codes.double() * self.scales[..., None].double()).reshape(self.codes.shape[0], -1)[:, :size].float().to(self.dtype).reshape(self.shape)
+
+
+class _PlainPointwise(torch.autograd.Function):
+    """checkpoint8.pointwise_conv's forward pass, and its backward pass in 64 bits on the plain checkpoint."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias):
+        n, c = x.shape[:2]
+        y = torch.matmul(weight.reshape(weight.shape[0], c), x.reshape(n, c, -1))
+        ctx.kept, ctx.weight, ctx.bias, ctx.shape = _plain(x)[2].reshape(n, c, -1), weight, bias is not None, x.shape
+        return (y if bias is None else y + bias.view(1, -1, 1)).view(n, -1, *x.shape[2:])
+
+    @staticmethod
+    def backward(ctx, dy):
+        d = dy.double().reshape(dy.shape[0], dy.shape[1], -1)
+        w = ctx.weight.reshape(dy.shape[1], -1)
+        dx = torch.matmul(w.t().contiguous(), d.float()).view(ctx.shape) if ctx.needs_input_grad[0] else None
+        dw = sum(u @ v.t().contiguous() for u, v in zip(d, ctx.kept)).float().view(ctx.weight.shape)
+        return dx, dw, d.sum((0, 2)).float() if ctx.bias else None
+
+
+@pytest.mark.gpu
+def test_a_network_trains_from_packed_activations(monkeypatch):
+    """The grasp-Q network: same output, the gradients of a backward pass on plainly restored activations, near those of the exact one, and less than half of its memory
+    between forward and backward."""
+    import contextlib
+    torch.manual_seed(0)
+    net = qnet.MULTIDISCRETE_RESNET(6).cuda().train()
+    x = torch.rand(4, 4, 80, 80, device="cuda")
+    weight = torch.randn(4, 6, 80, 80, device="cuda")
+    with torch.no_grad():
+        for _ in range(2):
+            net(x)
+    y, grads, kept = _gradients(net, x, weight, contextlib.nullcontext())
+    y8, grads8, kept8 = _gradients(net, x, weight, checkpoint8.saved_activations())
+    monkeypatch.setattr(checkpoint8, "pack", lambda t: _PlainPacked(*_plain(t.detach())[:2], t.shape, t.dtype))
+    monkeypatch.setattr(checkpoint8, "pointwise_conv", lambda t, w, b=None: _PlainPointwise.apply(t, w, b))
+    _, plain8, _ = _gradients(net, x, weight, checkpoint8.saved_activations())
+    assert torch.allclose(y, y8, rtol=1e-4, atol=1e-5)
+    most = max(float(g.norm()) for g in grads)
+    for (name, _), a, b, c in zip(net.named_parameters(), grads, grads8, plain8):
+        if float(a.norm()) > 1e-3 * most:
+            # the library's convolutions add in another order every time, a few 1e-6 per layer, and a batch norm's backward pass subtracts means
+            assert float((b - c).norm() / c.norm()) < 1e-3, name
+            assert float((a - b).norm() / a.norm()) < 0.15, name
+    assert kept8 < 0.5 * kept
+
+
+@pytest.mark.gpu
+def test_relu_keeps_signs():
+    x = torch.randn(3, 5, 40, 41, generator=torch.Generator().manual_seed(6)).cuda().requires_grad_()
+    x.data.view(-1)[:7] = torch.tensor([0.0, -0.0, 1e-30, -1e-30, math.inf, -math.inf, 1e-3]).cuda()
+    up = torch.randn_like(x)
+    got, = torch.autograd.grad(checkpoint8.relu(x), x, up)
+    want, = torch.autograd.grad(torch.relu(x), x, up)
+    assert torch.equal(checkpoint8.relu(x), torch.relu(x)) and torch.equal(got, want)
