@@ -27,12 +27,13 @@ typedef struct ur5_rows {
   int64_t rows, actions, mask_len;
   int32_t dtype, device;
   void* stream;
-  void* work;                 /* workspace of at least ur5_policy_work_bytes(rows, actions) bytes, 16-byte aligned; contents before and after a call mean nothing,
-                                 except between ur5_policy_clip_loss and the ur5_policy_clip_grad of the same rows (and prefer_loss / prefer_grad), which reads it */
+  void* work;                 /* workspace of at least ur5_policy_work_bytes(...) bytes, 16-byte aligned; contents before and after a call mean nothing, except between
+                                 ur5_policy_clip_loss and the ur5_policy_clip_grad calls of the same rows (and prefer_loss / prefer_grad), which read it */
   int64_t work_bytes;
 } ur5_rows;
 
-int64_t ur5_policy_work_bytes(int64_t rows, int64_t actions);
+/* mask_len: 0 without a mask; pairs: of the preference loss, 0 for the others */
+int64_t ur5_policy_work_bytes(int64_t rows, int64_t actions, int64_t mask_len, int64_t pairs);
 
 /* action[i] ~ softmax(row i) among the allowed actions and its log-probability. The draw is a pure function of (offset, gids[i]): the noise of action j is the j-th number of
    sharding.scene_uniform (offset: its scalar key, gids: global scene ids), so a scene draws the same action however the scenes are sharded. Nothing allowed: -1 and 0. */
@@ -52,7 +53,7 @@ typedef struct ur5_clip {
 int ur5_policy_clip_loss(const ur5_rows* r, const ur5_clip* c, float* loss, float* logp, float* kl, float* entropy);
 /* grad [rows][actions] (dense, dtype of the logits) of the loss times grad_scale times *upstream, from the workspace that clip_loss left; rows that do not count get 0. */
 int ur5_policy_clip_grad(const ur5_rows* r, const ur5_clip* c, void* grad);
-/* both at once, in two launches. */
+/* both at once, in three launches. */
 int ur5_policy_clip_loss_grad(const ur5_rows* r, const ur5_clip* c, float* loss, float* logp, float* kl, float* entropy, void* grad);
 
 typedef struct ur5_prefer {
@@ -67,6 +68,7 @@ typedef struct ur5_prefer {
    Rows that do not count, or belong to no episode, add nothing. */
 int ur5_policy_prefer_loss(const ur5_rows* r, const ur5_prefer* p, float* loss, float* margin);
 int ur5_policy_prefer_grad(const ur5_rows* r, const ur5_prefer* p, void* grad);
+int ur5_policy_prefer_loss_grad(const ur5_rows* r, const ur5_prefer* p, float* loss, float* margin, void* grad);
 
 /* 8-bit activation checkpoints: planes [planes][size] of dtype become codes int8 [planes][groups][64] and scales float [planes][groups], groups = ceil(size / 64): scale = the group's
    largest magnitude / 127 (rounded to fp32, and at most the largest s with a finite 127 s), code = the integer nearest to value / scale (ties to even), what a code stands for is code * scale (rounded to fp32).

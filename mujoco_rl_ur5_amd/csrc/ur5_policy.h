@@ -1,25 +1,32 @@
 // ur5_policy.h -- device code of the policy operators (include/ur5learn.h): softmax statistics over rows of logits, sampling, log-probabilities, the clipped policy
 // loss and the preference loss with their gradients.
 //
-// A row holds one logit per action, action = rotation * pixels + pixel, and a mask of the pixels that every rotation shares (mask[j % mask_len]). Rows are long
-// (240 000 actions) and few (1 .. some thousands), so a row is cut into `splits` pieces of `per` tiles; each piece is one workgroup that reads its logits ONCE and
-// leaves a record of running sums relative to the piece's own maximum; whoever needs the row joins its records. All of it is bound by the bytes of the logits.
+// A row holds one logit per action, action = map * pixels + pixel (a map per wrist rotation), and a mask of the pixels that all maps share (mask[j % pixels]). Rows are long
+// (240 000 actions) and few (1 .. some thousands), so a row is cut into pieces, a workgroup each: some pixels of some maps. A piece reads its logits ONCE and leaves a record
+// of running sums relative to its own maximum; whoever needs the row joins its records. All of it is bound by the bytes of the logits and, next, by the instructions per logit.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <cstdint>
 
 namespace ur5policy {
 
-constexpr int THREADS = 256, VEC = 8, TILE = THREADS * VEC;   // a thread takes 8 neighbouring actions per tile: 2 (fp32) or 1 (16-bit) loads of 16 bytes, 8 mask bytes
+constexpr int THREADS = 256, VEC = 8;                         // a thread takes 8 neighbouring actions at a time: 2 (fp32) or 1 (16-bit) loads of 16 bytes, 8 mask bytes
+constexpr int TILE = THREADS * VEC;                           // pixels of a piece: `per` tiles of 2048
+constexpr int MOST_PER = 16, MOST_PER_MASKED = 4;             // (a masked piece lists its allowed pixels in LDS)
 constexpr float LOG2E = 1.44269504088896340736f;
-constexpr float LOWEST = -3.402823466e38f;                    // start of a running maximum: finite, so -inf logits give exp2(-inf) = 0 and never inf - inf
+constexpr float LOWEST = -3.402823466e38f;                    // start of a running maximum: finite, so -inf logits give 2^-inf = 0 and never inf - inf
 
 enum { F32 = 0, F16 = 1, BF16 = 2 };
+struct yes { static constexpr bool value = true; };
+struct no { static constexpr bool value = false; };
 
 struct Rows {                       // rows of logits as the kernels see them
   const void* logits; const void* ref; const uint8_t* mask;
   long long stride, ref_stride, mask_stride;   // elements between rows
-  int rows, actions, mask_len, splits, per;
+  int rows, actions;
+  int pixels, maps;                 // actions = pixels * maps; without a mask one map of all actions
+  int per, maps_per;                // a piece: per * TILE pixels of maps_per maps
+  int pieces_x, pieces;             // pieces along the pixels, and of a row
 };
 
 struct Sums {                       // of (a piece of) a row, with e = exp(z - m)
@@ -68,49 +75,132 @@ template <typename T> __device__ __forceinline__ void store8(T tag, uint16_t* p,
   *(U4*)p = a;
 }
 
-// a thread's place in a row: action j and its mask position j mod mask_len, advanced without a division
-struct Place {
-  int j, p;
-  __device__ __forceinline__ void next(int step_mod, int len) { j += TILE; p += step_mod; if (p >= len) p -= len; }
-};
-// one byte per action of the 8 at the place: may it be taken? Positions wrap inside the 8 where the mask does.
-__device__ __forceinline__ uint64_t allowed8(const uint8_t* mask, int p, int len) {
-  if (p + VEC <= len) return *(const U8*)(mask + p);
-  uint64_t b = 0;
-  for (int i = 0; i < VEC; i++) {
-    b |= (uint64_t)(mask[p] != 0) << (8 * i);
-    if (++p == len) p = 0;
-  }
-  return b;
-}
-// which of the 8 actions at the place may be taken, and logits with -inf where not; actions behind the row's end (!FULL) are not allowed either
-template <bool MASK, bool FULL> __device__ __forceinline__ uint64_t allowed_at(const Rows& R, const uint8_t* mask, const Place& at) {
-  return MASK && (FULL || at.j < R.actions) ? allowed8(mask, at.p, R.mask_len) : ~0ull;
-}
-template <typename T, bool MASK, bool FULL> __device__ __forceinline__ void take8(const Rows& R, const typename T::raw* row, uint64_t ok, const Place& at, float* z) {
-  if (FULL) {
-    load8(T{}, row + at.j, z);
-  } else {
+// 8 values from p on, of which the first `left` exist (whole: all)
+template <typename T> __device__ __forceinline__ void take8(const typename T::raw* p, int left, bool whole, float* v) {
+  if (whole) { load8(T{}, p, v); return; }
 #pragma unroll
-    for (int i = 0; i < VEC; i++) z[i] = at.j + i < R.actions ? widen(T{}, row[at.j + i]) : -INFINITY;
-  }
-  if (MASK) {
+  for (int i = 0; i < VEC; i++) v[i] = i < left ? widen(T{}, p[i]) : -INFINITY;
+}
+template <typename T> __device__ __forceinline__ void put8(typename T::raw* p, int left, bool whole, const float* v) {
+  if (whole) { store8(T{}, p, v); return; }
 #pragma unroll
-    for (int i = 0; i < VEC; i++) z[i] = (ok >> (8 * i)) & 0xff ? z[i] : -INFINITY;
-  }
+  for (int i = 0; i < VEC; i++) if (i < left) p[i] = narrow(T{}, v[i]);
+}
+// -inf where an action may not be taken: bit i of `allowed` is value i's. By the bits (v_bfe, v_bfi): a select would become eight branches round the loads.
+__device__ __forceinline__ float barred(uint32_t allowed, int i, float v) {
+  const uint32_t keep = (uint32_t)__builtin_amdgcn_sbfe((int)allowed, i, 1);
+  return __uint_as_float((__float_as_uint(v) & keep) | (0xff800000u & ~keep));
+}
+__device__ __forceinline__ void bar8(uint32_t allowed, float* v) {
+#pragma unroll
+  for (int i = 0; i < VEC; i++) v[i] = barred(allowed, i, v[i]);
 }
 // whether the row's action counts: inside the row, allowed, and of a logit above -inf (a NaN counts: it has to show)
-template <typename T> __device__ __forceinline__ bool action_counts(const Rows& R, int row, long long a, float* z_out) {
-  if (a < 0 || a >= R.actions) return false;
-  if (R.mask && !R.mask[row * R.mask_stride + a % R.mask_len]) return false;
-  const float z = widen(T{}, ((const typename T::raw*)R.logits)[row * R.stride + a]);
-  *z_out = z;
-  return !(z == -INFINITY);
+template <typename T> __device__ __forceinline__ float logit(const Rows& R, int row, long long a) { return widen(T{}, ((const typename T::raw*)R.logits)[row * R.stride + a]); }
+template <typename T> __device__ __forceinline__ bool action_counts(const Rows& R, int row, long long a) {
+  if (a < 0 || a >= R.actions || (R.mask && !R.mask[row * R.mask_stride + a % R.pixels])) return false;
+  return !(logit<T>(R, row, a) == -INFINITY);
 }
 
-// ---- reductions over lanes
-__device__ __forceinline__ float lanes_max(float v, int width = 64) { for (int o = width >> 1; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o)); return v; }
-template <typename S> __device__ __forceinline__ S lanes_sum(S v, int width = 64) { for (int o = width >> 1; o; o >>= 1) v += __shfl_xor(v, o); return v; }
+// ---- the 8s of a piece. visit(first action, allowed bits, values that exist, whole) for every 8 pixels of every map of the piece that hold an allowed one.
+// Logits that may not be taken are not read: the allowed 8s of the piece's pixels are listed in LDS once (the maps share them) and dealt to the threads from the list, so that no
+// lane idles where the mask has holes. A table of 42 % of the image: statistics of 513 bf16 rows 123 -> 87 us by not reading the rest.
+struct Piece { int first, pixels, map0, maps; };   // pixels first .. of maps map0 ..
+__device__ __forceinline__ Piece piece_of(const Rows& R, int piece) {
+  const int x = piece % R.pieces_x, y = piece / R.pieces_x;
+  Piece P{x * R.per * TILE, 0, y * R.maps_per, 0};
+  P.pixels = min(R.per * TILE, R.pixels - P.first);
+  P.maps = min(R.maps_per, R.maps - P.map0);
+  return P;
+}
+__device__ __forceinline__ uint32_t allowed8(const uint8_t* mask, int left, bool whole) {   // a byte per pixel -> a bit per pixel
+  uint64_t b = 0;
+  if (whole) b = *(const U8*)mask;
+  else for (int i = 0; i < left; i++) b |= (uint64_t)mask[i] << (8 * i);
+  uint32_t bits = 0;
+#pragma unroll
+  for (int i = 0; i < VEC; i++) bits |= (b >> (8 * i) & 0xff) ? 1u << i : 0u;
+  return bits;
+}
+template <bool MASK, typename V, typename N> __device__ __forceinline__ void for_piece(const Rows& R, int row, int piece, V visit, N none) {
+  const Piece P = piece_of(R, piece);
+  if (!MASK) {                      // one map: pixel = action
+    const int whole = P.pixels / VEC;
+#pragma unroll 2
+    for (int g = threadIdx.x; g < whole; g += THREADS) visit(P.first + g * VEC, 0xffu, VEC, yes{});
+    const int left = P.pixels % VEC;
+    if (left && threadIdx.x == whole % THREADS) visit(P.first + whole * VEC, (1u << left) - 1, left, no{});
+    return;
+  }
+  const uint8_t* mask = R.mask + row * R.mask_stride + P.first;
+  if (R.per == 1 && R.maps_per == 1) {   // a small batch, cut into pieces of an 8 per thread: latency counts, so the logits are asked for together with their mask
+    const int g = threadIdx.x, left = P.pixels - g * VEC, j = P.map0 * R.pixels + P.first + g * VEC;
+    if (left >= VEC) visit(j, allowed8(mask + g * VEC, VEC, true), VEC, yes{});
+    else if (left > 0) visit(j, allowed8(mask + g * VEC, left, false), left, no{});
+    return;
+  }
+  __shared__ uint32_t list[MOST_PER_MASKED * THREADS];      // group of 8 << 8 | bits, in the order of the pixels
+  __shared__ int share[MOST_PER_MASKED * THREADS / 64];     // entries of each wavefront of each tile
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint32_t bits[MOST_PER_MASKED];
+  int before[MOST_PER_MASKED];
+#pragma unroll
+  for (int t = 0; t < MOST_PER_MASKED; t++) {
+    const int g = t * THREADS + threadIdx.x, left = P.pixels - g * VEC;
+    bits[t] = left >= VEC ? allowed8(mask + g * VEC, VEC, true) : left > 0 ? allowed8(mask + g * VEC, left, false) : 0;
+    const uint64_t some = __ballot(bits[t] != 0);
+    before[t] = __popcll(some & ((1ull << lane) - 1));
+    if (lane == 0) share[t * (THREADS / 64) + wave] = __popcll(some);
+    if (!bits[t] && left > 0) none(P, g);
+  }
+  __syncthreads();
+  int n = 0;
+#pragma unroll
+  for (int t = 0; t < MOST_PER_MASKED; t++)
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; w++) {
+      if (w == wave && bits[t]) list[n + before[t]] = (uint32_t)(t * THREADS + threadIdx.x) << 8 | bits[t];
+      n += share[t * (THREADS / 64) + w];
+    }
+  __syncthreads();
+  const int all = n * P.maps;
+  const float per = __builtin_amdgcn_rcpf((float)n);
+  for (int i = threadIdx.x; i < all; i += THREADS) {
+    int m = (int)(((float)i + 0.5f) * per), k = i - m * n;             // map and list entry of item i; the estimate is off by at most one
+    if (k < 0) { m--; k += n; }
+    if (k >= n) { m++; k -= n; }
+    const uint32_t e = list[k];
+    const int p = P.first + (e >> 8) * VEC, left = R.pixels - p, j = (P.map0 + m) * R.pixels + p;
+    if (left >= VEC) visit(j, e & 0xff, VEC, yes{});
+    else visit(j, e & 0xff, left, no{});
+  }
+}
+
+// ---- reductions over 64 or 4 neighbouring lanes, in every lane, in a fixed order: lanes of a row of 16 exchange through DPP, the four rows through scalar registers
+// (through LDS, one exchange costs as much as all of a reduction here)
+template <int CTRL> __device__ __forceinline__ float dpp(float v) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true)); }
+template <int CTRL> __device__ __forceinline__ int dpp(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xf, 0xf, true); }
+template <int CTRL> __device__ __forceinline__ double dpp(double v) {
+  const int2 w = __builtin_bit_cast(int2, v);
+  return __builtin_bit_cast(double, int2{dpp<CTRL>(w.x), dpp<CTRL>(w.y)});
+}
+__device__ __forceinline__ int at_lane(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+__device__ __forceinline__ float at_lane(float v, int lane) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane)); }
+__device__ __forceinline__ double at_lane(double v, int lane) {
+  const int2 w = __builtin_bit_cast(int2, v);
+  return __builtin_bit_cast(double, int2{at_lane(w.x, lane), at_lane(w.y, lane)});
+}
+template <int WIDTH, typename S, typename F> __device__ __forceinline__ S lanes_fold(S v, F f) {
+  static_assert(WIDTH == 64 || WIDTH == 4, "widths in use");
+  v = f(v, dpp<0xB1>(v));             // quad_perm 1 0 3 2
+  v = f(v, dpp<0x4E>(v));             // quad_perm 2 3 0 1
+  if (WIDTH == 4) return v;
+  v = f(v, dpp<0x141>(v));            // row_half_mirror
+  v = f(v, dpp<0x140>(v));            // row_mirror
+  return f(f(at_lane(v, 0), at_lane(v, 16)), f(at_lane(v, 32), at_lane(v, 48)));
+}
+template <int WIDTH = 64> __device__ __forceinline__ float lanes_max(float v) { return lanes_fold<WIDTH>(v, [](float x, float y) { return fmaxf(x, y); }); }
+template <int WIDTH = 64, typename S> __device__ __forceinline__ S lanes_sum(S v) { return lanes_fold<WIDTH>(v, [](S x, S y) { return x + y; }); }
 // exp(d) for d <= 0 by the hardware's 2^x (results below 2^-126 are 0)
 __device__ __forceinline__ float fall(float d) { return __builtin_amdgcn_exp2f(d * LOG2E); }
 __device__ __forceinline__ float shrink(float from, float to) { return fall(from - to); }
@@ -133,47 +223,44 @@ __device__ __forceinline__ bool better(double s, int i, double than, int at) { r
 // running sums of one thread: fp32, over at most a few hundred terms
 struct Running { float m, s, t, k, mq, sq; };
 __device__ __forceinline__ Running nothing() { return Running{LOWEST, 0, 0, 0, LOWEST, 0}; }
-// z (and q): 8 logits, -inf where not allowed. One maximum per 8, one rescaling, then the sums relative to it.
+// z (and q): 8 logits, -inf where not allowed. One maximum per 8; the sums move to it where it is new (rare after a few 8s).
 template <bool REF, bool ENTROPY> __device__ __forceinline__ void add8(Running& a, const float* z, const float* q, float* e) {
-  float m = a.m;
+  float m = a.m, mq = a.mq;
 #pragma unroll
-  for (int i = 0; i < VEC; i++) m = fmaxf(m, z[i]);
-  const float f = shrink(a.m, m);
-  if (ENTROPY) a.t = f * (a.t + a.s * fmaxf(a.m - m, -1e30f));   // the sums move to the new maximum; an empty sum meets LOWEST - m: kept finite
-  a.s *= f;
-  if (REF) a.k *= f;
-  a.m = m;
+  for (int i = 0; i < VEC; i++) { m = fmaxf(m, z[i]); if (REF) mq = fmaxf(mq, q[i]); }
+  if (m > a.m) {
+    const float f = shrink(a.m, m);
+    if (ENTROPY) a.t = f * (a.t + a.s * fmaxf(a.m - m, -1e30f));   // an empty sum meets LOWEST - m: kept finite
+    a.s *= f;
+    if (REF) a.k *= f;
+    a.m = m;
+  }
+  if (REF && mq > a.mq) { a.sq *= shrink(a.mq, mq); a.mq = mq; }
 #pragma unroll
   for (int i = 0; i < VEC; i++) {
-    const float d = z[i] - m;
+    const float d = z[i] - a.m;
     e[i] = fall(d);
     a.s += e[i];
-    if (ENTROPY) a.t += e[i] * fmaxf(d, -1e4f);                 // e is 0 long before -1e4: 0 * -inf does not arise
-    if (REF) a.k += e[i] == 0.f ? 0.f : e[i] * (z[i] - q[i]);
-  }
-  if (REF) {
-    float mq = a.mq;
-#pragma unroll
-    for (int i = 0; i < VEC; i++) mq = fmaxf(mq, q[i]);
-    a.sq *= shrink(a.mq, mq);
-    a.mq = mq;
-#pragma unroll
-    for (int i = 0; i < VEC; i++) a.sq += fall(q[i] - mq);
+    if (ENTROPY) a.t += e[i] * fmaxf(d, -1e4f);                   // e is 0 long before -1e4 (and before -1e30 below): 0 * -inf does not arise
+    if (REF) {
+      a.k += e[i] * fmaxf(z[i] - q[i], -1e30f);
+      a.sq += fall(q[i] - a.mq);
+    }
   }
 }
 // From here on sums are 64 bits wide: a KL is a difference of two logarithms of sums, and what a few last additions lose in 32 bits (5e-8 of a sum, measured) would be
 // 1e-6 of it. Their factors come from the precise exp where a single one weighs (joining wavefronts and records).
 __device__ __forceinline__ double moved(double s, double t, float from, float to) { return t + s * fmaxf(from - to, -1e30f); }
-// sums of `width` neighbouring lanes joined, in every one of them
-__device__ __forceinline__ void join_lanes(Sums& a, int width, bool ref, bool entropy) {
-  const float m = lanes_max(a.m, width);
+// sums of neighbouring lanes joined, in every one of them
+template <int WIDTH> __device__ __forceinline__ void join_lanes(Sums& a, bool ref, bool entropy) {
+  const float m = lanes_max<WIDTH>(a.m);
   const double f = exp((double)a.m - m);
-  if (entropy) a.t = lanes_sum(f * moved(a.s, a.t, a.m, m), width);
-  a.s = lanes_sum(a.s * f, width);
+  if (entropy) a.t = lanes_sum<WIDTH>(f * moved(a.s, a.t, a.m, m));
+  a.s = lanes_sum<WIDTH>(a.s * f);
   if (ref) {
-    a.k = lanes_sum(a.k * f, width);
-    const float mq = lanes_max(a.mq, width);
-    a.sq = lanes_sum(a.sq * exp((double)a.mq - mq), width);
+    a.k = lanes_sum<WIDTH>(a.k * f);
+    const float mq = lanes_max<WIDTH>(a.mq);
+    a.sq = lanes_sum<WIDTH>(a.sq * exp((double)a.mq - mq));
     a.mq = mq;
   }
   a.m = m;
@@ -191,71 +278,55 @@ __device__ __forceinline__ Sums join_wave(const Running& r, bool ref, bool entro
   }
   return a;
 }
-
-// what a piece of a row is to its threads
-template <typename T, bool MASK> struct Piece {
-  const typename T::raw* z_row; const uint8_t* mask;
-  int tiles, whole, step_mod;       // tiles of the piece, and how many of them the row fills
-  Place at;
-  __device__ __forceinline__ Piece(const Rows& R, int row, int piece) {
-    z_row = (const typename T::raw*)R.logits + row * R.stride;
-    mask = MASK ? R.mask + row * R.mask_stride : nullptr;
-    const int begin = piece * R.per * TILE, left = R.actions - begin;
-    tiles = min(R.per, (left + TILE - 1) / TILE); whole = min(R.per, left / TILE);
-    at.j = begin + (int)threadIdx.x * VEC;
-    at.p = MASK ? at.j % R.mask_len : 0;
-    step_mod = MASK ? TILE % R.mask_len : 0;
-  }
-};
-// the workgroup's sums joined, in the first lanes of every wavefront
+// the workgroup's sums joined, in every thread
 __device__ __forceinline__ Sums join_workgroup(const Running& r, bool ref, bool entropy) {
   __shared__ Sums wave[THREADS / 64];
   Sums a = join_wave(r, ref, entropy);
   if ((threadIdx.x & 63) == 0) wave[threadIdx.x >> 6] = a;
   __syncthreads();
   a = wave[threadIdx.x & (THREADS / 64 - 1)];
-  join_lanes(a, THREADS / 64, ref, entropy);
+  join_lanes<THREADS / 64>(a, ref, entropy);
   return a;
 }
 
-// ---- statistics of the pieces of rows. Grid: rows * splits workgroups, the pieces of a row next to each other. fp32 sums: a thread adds at most 8 * per terms,
-// lanes and pieces join in trees.
+// ---- statistics of the pieces of rows
 template <typename T, bool MASK, bool REF, bool ENTROPY> __device__ __forceinline__ Sums piece_sums(const Rows& R, int row, int piece) {
-  Piece<T, MASK> P(R, row, piece);
+  const auto* z_row = (const typename T::raw*)R.logits + row * R.stride;
   const auto* q_row = REF ? (const typename T::raw*)R.ref + row * R.ref_stride : nullptr;
   Running a = nothing();
-  float z[VEC], q[VEC], e[VEC];
-#pragma unroll 2
-  for (int i = 0; i < P.whole; i++) {
-    const uint64_t ok = allowed_at<MASK, true>(R, P.mask, P.at);
-    take8<T, MASK, true>(R, P.z_row, ok, P.at, z);
-    if (REF) take8<T, MASK, true>(R, q_row, ok, P.at, q);
+  for_piece<MASK>(R, row, piece, [&](int j, uint32_t allowed, int left, auto whole) {
+    float z[VEC], q[VEC], e[VEC];
+    take8<T>(z_row + j, left, decltype(whole)::value, z);
+    if (REF) take8<T>(q_row + j, left, decltype(whole)::value, q);
+    if (MASK) { bar8(allowed, z); if (REF) bar8(allowed, q); }
     add8<REF, ENTROPY>(a, z, q, e);
-    P.at.next(P.step_mod, R.mask_len);
-  }
-  if (P.whole < P.tiles) {
-    const uint64_t ok = allowed_at<MASK, false>(R, P.mask, P.at);
-    take8<T, MASK, false>(R, P.z_row, ok, P.at, z);
-    if (REF) take8<T, MASK, false>(R, q_row, ok, P.at, q);
-    add8<REF, ENTROPY>(a, z, q, e);
-  }
+  }, [](const Piece&, int) {});
   return join_workgroup(a, REF, ENTROPY);
 }
 
-template <typename T, bool MASK, bool REF> __global__ void __launch_bounds__(THREADS) ur5_policy_stats(Rows R, const int64_t* action, Part* parts, int* counts) {
-  const int row = blockIdx.x / R.splits, piece = blockIdx.x % R.splits;
-  const Sums a = piece_sums<T, MASK, REF, true>(R, row, piece);
-  if (threadIdx.x == 0) {
-    parts[blockIdx.x] = Part{a, 0};
-    float z;
-    if (piece == 0) counts[row] = action_counts<T>(R, row, action[row], &z);
+// ---- what both losses have in common. Per row, dL/dz_j = p_j (c0 + kl (z_j - q_j - gap) + entropy (z_j - m - level)) + [j = action] take; p_j = exp(z_j - m) rs.
+// Three launches: statistics of the pieces -- a Slope per row and a term per row or pair of the loss -- the gradient, of which the first workgroup adds the terms up.
+// (Joining a row's records in every workgroup of the gradient instead saves a launch and costs each of them 3 us of double arithmetic before its first load.)
+struct Slope { float m, rs, c0, kl, gap, entropy, level, take; int on; };   // on: the row counts; anything else is unset where it does not
+struct Span { const int64_t* ends; int last; };   // the preference loss: rows outside [ends[0], ends[last]) belong to no episode and do not count; ends == null: all rows
+__device__ __forceinline__ bool in_span(const Span& s, int row) { return !s.ends || (row >= s.ends[0] && row < s.ends[s.last]); }
+// The pieces come after `front` workgroups (a multiple of 8, so that pieces keep their XCDs from kernel to kernel) that write which rows count, a thread each.
+template <typename T, bool MASK, bool REF> __global__ void __launch_bounds__(THREADS) ur5_policy_stats(Rows R, Span span, int front, const int64_t* action, Part* parts, Slope* slopes) {
+  if ((int)blockIdx.x < front) {
+    const int row = blockIdx.x * THREADS + threadIdx.x;
+    if (row < R.rows) slopes[row] = Slope{0, 0, 0, 0, 0, 0, 0, 0, in_span(span, row) && action_counts<T>(R, row, action[row])};
+    return;
   }
+  const int block = (int)blockIdx.x - front, row = block / R.pieces, piece = block % R.pieces;
+  const int64_t a = action[row];
+  if (a < 0 || a >= R.actions || !in_span(span, row)) return;
+  const Sums sums = piece_sums<T, MASK, REF, true>(R, row, piece);
+  if (threadIdx.x == 0) parts[block] = Part{sums, 0};
 }
-
-// the records of a row joined by `width` neighbouring lanes (`lane`: this one's place among them), in every one of them
-__device__ __forceinline__ Sums join_row(const Part* parts, int splits, int lane, int width, bool ref) {
+// the records of a row joined by a wavefront, in every lane
+__device__ __forceinline__ Sums join_row(const Part* parts, int pieces, bool ref) {
   Sums a{LOWEST, LOWEST, 0, 0, 0, 0};
-  for (int i = lane; i < splits; i += width) {
+  for (int i = threadIdx.x & 63; i < pieces; i += 64) {
     const Sums p = parts[i].sums;
     const float m = fmaxf(a.m, p.m), mq = fmaxf(a.mq, p.mq);
     const double f = exp((double)a.m - m), g = exp((double)p.m - m);
@@ -267,32 +338,157 @@ __device__ __forceinline__ Sums join_row(const Part* parts, int splits, int lane
     }
     a.m = m; a.mq = mq;
   }
-  join_lanes(a, width, ref, true);
+  join_lanes<64>(a, ref, true);
   return a;
 }
+constexpr int WAVES = THREADS / 64;
+// sums over the workgroup in a fixed order, in every thread
+template <typename S> __device__ __forceinline__ S workgroup_sum(S v) {
+  __shared__ S wave[WAVES];
+  v = lanes_sum(v);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) wave[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = wave[0];
+  for (int i = 1; i < WAVES; i++) v += wave[i];
+  return v;
+}
+__device__ __forceinline__ int counting_rows(const Slope* slopes, int rows) {
+  int n = 0;
+  for (int i = threadIdx.x; i < rows; i += THREADS) n += slopes[i].on;
+  return workgroup_sum(n);
+}
+// loss = sum of n terms / what they are a mean over (the rows that count, or `over`)
+struct Terms { const double* term; int n, over; const Slope* slopes; int rows; float* loss; };
+__device__ __forceinline__ void add_terms(const Terms& t) {
+  double sum = 0;
+  for (int i = threadIdx.x; i < t.n; i += THREADS) sum += t.term[i];
+  sum = workgroup_sum(sum);
+  const int over = t.over ? t.over : max(1, counting_rows(t.slopes, t.rows));
+  if (threadIdx.x == 0) *t.loss = (float)(sum / over);
+}
+// (a translation unit of its own kind: also launched alone, by a forward pass without a gradient)
+static __global__ void __launch_bounds__(THREADS) ur5_policy_loss(Terms t) { add_terms(t); }
+constexpr int FIRST = 8;             // workgroups before the pieces, as in the statistics; the first of them writes the loss if t.loss
+template <typename T, bool MASK, bool REF> __global__ void __launch_bounds__(THREADS) ur5_policy_grad(Rows R, Terms t, const int64_t* action, const Slope* slopes, float scale, const float* upstream, void* grad) {
+  const int block = (int)blockIdx.x - FIRST;
+  if (block < 0) {
+    if (t.loss && blockIdx.x == 0) add_terms(t);
+    return;
+  }
+  const int row = R.rows - 1 - block / R.pieces, piece = block % R.pieces;   // the rows that the statistics read last, and the 256 MB memory-side cache may hold, come first (513 bf16 rows: 121 -> 111 us)
+  Slope S = slopes[row];
+  typename T::raw* out = (typename T::raw*)grad + (long long)row * R.actions;
+  const float zero[VEC] = {};
+  const auto clear = [&](const Piece& P, int g) {          // 8 pixels of all maps of the piece
+    const int p = P.first + g * VEC, left = R.pixels - p;
+    for (int m = 0; m < P.maps; m++) put8<T>(out + (P.map0 + m) * R.pixels + p, left, left >= VEC, zero);
+  };
+  if (!S.on) {                                             // zeros; the logits are not read
+    const Piece P = piece_of(R, piece);
+    for (int g = threadIdx.x; g * VEC < P.pixels; g += THREADS) clear(P, g);
+    return;
+  }
+  const float factor = scale * (upstream ? *upstream : 1.f);
+  S.rs *= factor; S.take *= factor;
+  const int a = (int)action[row];
+  const auto* z_row = (const typename T::raw*)R.logits + row * R.stride;
+  const auto* q_row = REF ? (const typename T::raw*)R.ref + row * R.ref_stride : nullptr;
+  for_piece<MASK>(R, row, piece, [&](int j, uint32_t allowed, int left, auto whole) {
+    float z[VEC], q[VEC], g[VEC];
+    take8<T>(z_row + j, left, decltype(whole)::value, z);
+    if (REF) take8<T>(q_row + j, left, decltype(whole)::value, q);
+    if (MASK) bar8(allowed, z);
+#pragma unroll
+    for (int i = 0; i < VEC; i++) {
+      const float d = z[i] - S.m, p = fall(d) * S.rs;
+      float v = S.c0 + S.entropy * (d - S.level);
+      if (REF) v += S.kl * (z[i] - q[i] - S.gap);
+      g[i] = p == 0.f ? 0.f : p * v;                       // not allowed, or too unlikely for 32 bits: the limit, whatever q holds
+    }
+    if ((unsigned)(a - j) < VEC)
+#pragma unroll
+      for (int i = 0; i < VEC; i++) g[i] += a - j == i ? S.take : 0.f;
+    put8<T>(out + j, left, decltype(whole)::value, g);
+  }, clear);
+}
 
-// ---- log-probability of an action and entropy per row: a wavefront joins a row's records. logp 0 where the action lies outside the row (no action), -inf where it
-// may not be taken; entropy 0 where nothing may.
+// ---- clipped policy loss. Per row: ratio r = exp(logp - old), L = -min(r A, clip(r, 1 - lo, 1 + hi) A) + kl_coef KL(p || q) - entropy_coef H; the mean over the rows that count.
+struct Clip { const int64_t* action; const float* old_logp; const float* advantage; float lo, hi, kl_coef, entropy_coef; };
+// a wavefront per row. Normalisers in 64 bits: KL = k / s - (lse - lse_q) is a small difference of large numbers.
+template <typename T, bool REF> __global__ void __launch_bounds__(THREADS) ur5_policy_clip_rows(Rows R, Clip C, const Part* parts, Slope* slopes, double* term, float* logp, float* kl, float* entropy) {
+  const int n = counting_rows(slopes, R.rows), row = blockIdx.x * WAVES + (threadIdx.x >> 6);
+  if (row >= R.rows) return;
+  const bool on = slopes[row].on, writes = (threadIdx.x & 63) == 0;
+  if (!on) {
+    if (writes) { term[row] = 0; logp[row] = kl[row] = entropy[row] = 0; }
+    return;
+  }
+  const Sums a = join_row(parts + (size_t)row * R.pieces, R.pieces, REF);
+  if (!writes) return;
+  const double ls = log(a.s), shift = REF ? (double)a.m - a.mq + ls - log(a.sq) : 0;
+  const float adv = C.advantage[row], lp = (float)((double)logit<T>(R, row, C.action[row]) - a.m - ls), k = REF ? (float)(a.k / a.s - shift) : 0.f, h = (float)(ls - a.t / a.s);
+  const float ratio = expf(lp - C.old_logp[row]), free = ratio * adv, held = fminf(fmaxf(ratio, 1 - C.lo), 1 + C.hi) * adv;
+  const float take = held < free ? 0.f : -adv * ratio;   // the clipped branch has no slope; NaN stays
+  logp[row] = lp; kl[row] = k; entropy[row] = h;
+  term[row] = -(double)(held < free ? held : free) + (REF ? (double)C.kl_coef * k : 0.0) - (double)C.entropy_coef * h;
+  slopes[row] = Slope{a.m, (float)(1 / (a.s * n)), -take, C.kl_coef, (float)(shift + k), C.entropy_coef, (float)(ls - h), take / n, 1};
+}
+
+// ---- preference loss. Episodes are runs of rows: episode k holds the rows offsets[k] .. offsets[k + 1]. S_k = sum over its counting rows of logp - ref_logp,
+// margin_i = beta (S_2i - S_2i+1), loss = mean over pairs of (1 - eps) softplus(-margin) + eps softplus(margin).
+struct Prefer { const int64_t* action; const float* ref_logp; const int64_t* offsets; int pairs; double beta, eps; };
+// a workgroup per pair, a wavefront per row of it
+template <typename T> __global__ void __launch_bounds__(THREADS) ur5_policy_prefer_pairs(Rows R, Prefer P, const Part* parts, Slope* slopes, double* term, float* margin) {
+  const int i = blockIdx.x, wave = threadIdx.x >> 6;
+  int end[3];
+  for (int k = 0; k < 3; k++) end[k] = (int)min(max((long long)P.offsets[2 * i + k], 0ll), (long long)R.rows);   // offsets outside the rows are taken as their ends
+  double d = 0;
+  for (int half = 0; half < 2; half++)
+    for (int row = end[half] + wave; row < end[half + 1]; row += WAVES) {
+      if (!slopes[row].on) continue;
+      const Sums a = join_row(parts + (size_t)row * R.pieces, R.pieces, false);
+      const double ls = log(a.s), l = (double)logit<T>(R, row, P.action[row]) - a.m - ls - P.ref_logp[row];
+      d += half ? -l : l;
+      if ((threadIdx.x & 63) == 0) { slopes[row].m = a.m; slopes[row].rs = (float)(1 / a.s); }
+    }
+  const double mg = P.beta * workgroup_sum((threadIdx.x & 63) == 0 ? d : 0.0);
+  const double up = 1 / (1 + exp(mg));                                       // sigmoid(-margin)
+  const double soft = fmax(mg, 0.0) + log1p(exp(-fabs(mg)));                 // softplus(margin)
+  if (threadIdx.x == 0) {
+    margin[i] = (float)mg;
+    term[i] = (1 - P.eps) * (soft - mg) + P.eps * soft;
+  }
+  const float w = (float)(-P.beta * ((1 - P.eps) * up - P.eps * (1 - up)) / P.pairs);   // d loss / d logp of the preferred episode's rows
+  for (int half = 0; half < 2; half++)
+    for (int row = end[half] + threadIdx.x; row < end[half + 1]; row += THREADS) {
+      Slope& S = slopes[row];
+      S.take = half ? -w : w;
+      S.rs *= S.take;
+      S.c0 = -1.f;
+    }
+}
+
+// ---- log-probability of an action and entropy per row. logp 0 where the action lies outside the row (no action), -inf where it may not be taken; entropy 0 where
+// nothing may. A row of one piece is finished by its workgroup, others by a wavefront each.
 template <typename T> __device__ __forceinline__ void write_logp(const Rows& R, int row, const Sums& a, const int64_t* action, float* logp, float* entropy) {
   const long long at = action[row];
-  float z = 0;
-  const bool counts = action_counts<T>(R, row, at, &z);
   const double ls = a.s > 0 ? log(a.s) : a.s - a.s;   // a NaN sum stays NaN
-  logp[row] = counts ? (float)((double)z - a.m - ls) : at < 0 || at >= R.actions ? 0.f : -INFINITY;
+  logp[row] = action_counts<T>(R, row, at) ? (float)((double)logit<T>(R, row, at) - a.m - ls) : at < 0 || at >= R.actions ? 0.f : -INFINITY;
   if (entropy) entropy[row] = a.s == 0 ? 0.f : (float)(ls - a.t / a.s);
 }
 template <typename T, bool MASK> __global__ void __launch_bounds__(THREADS) ur5_policy_logp(Rows R, const int64_t* action, Part* parts, float* logp, float* entropy) {
-  const int row = blockIdx.x / R.splits, piece = blockIdx.x % R.splits;
+  const int row = blockIdx.x / R.pieces, piece = blockIdx.x % R.pieces;
   const Sums a = piece_sums<T, MASK, false, true>(R, row, piece);
   if (threadIdx.x) return;
-  if (R.splits == 1) write_logp<T>(R, row, a, action, logp, entropy);
+  if (R.pieces == 1) write_logp<T>(R, row, a, action, logp, entropy);
   else parts[blockIdx.x] = Part{a, 0};
 }
 template <typename T> __global__ void __launch_bounds__(THREADS) ur5_policy_logp_rows(Rows R, const int64_t* action, const Part* parts, float* logp, float* entropy) {
-  const int row = blockIdx.x * (THREADS / 64) + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int row = blockIdx.x * WAVES + (threadIdx.x >> 6);
   if (row >= R.rows) return;
-  const Sums a = join_row(parts + (size_t)row * R.splits, R.splits, lane, 64, false);
-  if (lane == 0) write_logp<T>(R, row, a, action, logp, entropy);
+  const Sums a = join_row(parts + (size_t)row * R.pieces, R.pieces, false);
+  if ((threadIdx.x & 63) == 0) write_logp<T>(R, row, a, action, logp, entropy);
 }
 
 // ---- sampling. argmax_j z_j - log(-log u_j) is a draw from softmax(z). Two logarithms in 64 bits per action would cost more than reading it, and nearly every action
@@ -322,27 +518,25 @@ __device__ __forceinline__ void missing8(uint64_t key, int j, uint32_t* w) {
     w[i] = ~(hi ^ (hi >> 31));
   }
 }
-template <typename T> __device__ __forceinline__ void draw8(const Rows& R, const typename T::raw* row, uint64_t key, const Place& at, const Running& a, const float* z,
-                                                            const float* e, bool first, int* bar, Best& best) {
+template <typename T> __device__ __forceinline__ void draw8(const typename T::raw* row, uint64_t key, int j, const Running& a, const float* z, const float* e, bool first, int* bar, Best& best) {
   uint32_t w[VEC];
-  missing8(key, at.j, w);
+  missing8(key, j, w);
   if (first) {   // no score yet: a bound from below, E <= (1 - u) / u, one fast logarithm per action
     float low = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < VEC; i++) low = fmaxf(low, z[i] - 0.693147181f * __log2f(((float)w[i] + 1.f) / (float)~w[i]));
-    low = lanes_max(low);
-    if ((threadIdx.x & 63) == 0) atomicMax(bar, ordered(below(low)));
+    for (int i = 0; i < VEC; i++) low = fmaxf(low, z[i] - 0.693147181f * __log2f(((float)w[i] + 1.f) * __builtin_amdgcn_rcpf((float)~w[i])));
+    atomicMax(bar, ordered(below(low)));
   }
   const float reach = fminf(__builtin_amdgcn_exp2f((a.m - unordered(__hip_atomic_load(bar, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP))) * LOG2E), 1e30f) * (1.0001f * 4294967296.f);
   uint32_t near = 0;
 #pragma unroll
   for (int i = 0; i < VEC; i++) near |= (e[i] > 0 && (float)w[i] <= e[i] * reach) ? 1u << i : 0u;
   while (near) {
-    const int j = at.j + __ffs(near) - 1;
+    const int at = j + __ffs(near) - 1;
     near &= near - 1;
-    const double s = noisy_score(widen(T{}, row[j]), key, j);
-    if (better(s, j, best.score, best.at)) {
-      best = Best{s, j};
+    const double s = noisy_score(widen(T{}, row[at]), key, at);
+    if (better(s, at, best.score, best.at)) {
+      best = Best{s, at};
       atomicMax(bar, ordered(below(s)));
     }
   }
@@ -351,244 +545,52 @@ template <typename T> __device__ __forceinline__ void draw8(const Rows& R, const
 template <typename T> __device__ __forceinline__ void write_draw(const Rows& R, int row, float m, double s, const Best& b, int64_t* action, float* logp) {
   const bool some = b.at >= 0 && b.at < R.actions;
   action[row] = some ? b.at : -1;
-  logp[row] = some ? (float)((double)widen(T{}, ((const typename T::raw*)R.logits)[row * R.stride + b.at]) - m - log(s)) : s == 0 ? 0.f : NAN;
+  logp[row] = some ? (float)((double)logit<T>(R, row, b.at) - m - log(s)) : s == 0 ? 0.f : NAN;
 }
 constexpr int NOBODY = 0x7fffffff;
 template <typename T, bool MASK> __global__ void __launch_bounds__(THREADS) ur5_policy_sample(Rows R, uint64_t offset, const int64_t* gids, Draw* draws, int64_t* action, float* logp) {
-  const int row = blockIdx.x / R.splits, piece = blockIdx.x % R.splits;
+  const int row = blockIdx.x / R.pieces, piece = blockIdx.x % R.pieces;
   const uint64_t key = mix64((uint64_t)gids[row] * GOLD + offset);
   __shared__ int bar;
-  __shared__ Best wave[THREADS / 64];
+  __shared__ Best wave[WAVES];
   if (threadIdx.x == 0) bar = ordered(-INFINITY);
   __syncthreads();
-  Piece<T, MASK> P(R, row, piece);
+  const auto* z_row = (const typename T::raw*)R.logits + row * R.stride;
   Running a = nothing();
   Best best{-INFINITY, NOBODY};
-  float z[VEC], e[VEC];
-  for (int i = 0; i < P.whole; i++) {
-    take8<T, MASK, true>(R, P.z_row, allowed_at<MASK, true>(R, P.mask, P.at), P.at, z);
+  bool first = true;
+  for_piece<MASK>(R, row, piece, [&](int j, uint32_t allowed, int left, auto whole) {
+    float z[VEC], e[VEC];
+    take8<T>(z_row + j, left, decltype(whole)::value, z);
+    if (MASK) bar8(allowed, z);
     add8<false, false>(a, z, nullptr, e);
-    draw8<T>(R, P.z_row, key, P.at, a, z, e, i == 0, &bar, best);
-    P.at.next(P.step_mod, R.mask_len);
-  }
-  if (P.whole < P.tiles) {
-    take8<T, MASK, false>(R, P.z_row, allowed_at<MASK, false>(R, P.mask, P.at), P.at, z);
-    add8<false, false>(a, z, nullptr, e);
-    draw8<T>(R, P.z_row, key, P.at, a, z, e, P.whole == 0, &bar, best);
-  }
+    draw8<T>(z_row, key, j, a, z, e, first, &bar, best);
+    first = false;
+  }, [](const Piece&, int) {});
   join_best(best, 64);
   if ((threadIdx.x & 63) == 0) wave[threadIdx.x >> 6] = best;
   const Sums sums = join_workgroup(a, false, false);   // (its barrier stands between the wavefronts' bests and their join)
-  best = wave[threadIdx.x & (THREADS / 64 - 1)];
-  join_best(best, THREADS / 64);
+  best = wave[threadIdx.x & (WAVES - 1)];
+  join_best(best, WAVES);
   if (threadIdx.x) return;
-  if (R.splits == 1) write_draw<T>(R, row, sums.m, sums.s, best, action, logp);
+  if (R.pieces == 1) write_draw<T>(R, row, sums.m, sums.s, best, action, logp);
   else draws[blockIdx.x] = Draw{best.score, sums.s, sums.m, best.at};
 }
 template <typename T> __global__ void __launch_bounds__(THREADS) ur5_policy_sample_rows(Rows R, const Draw* draws, int64_t* action, float* logp) {
-  const int row = blockIdx.x * (THREADS / 64) + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int row = blockIdx.x * WAVES + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (row >= R.rows) return;
   Sums a{LOWEST, LOWEST, 0, 0, 0, 0};
   Best best{-INFINITY, NOBODY};
-  for (int i = lane; i < R.splits; i += 64) {
-    const Draw d = draws[(size_t)row * R.splits + i];
+  for (int i = lane; i < R.pieces; i += 64) {
+    const Draw d = draws[(size_t)row * R.pieces + i];
     const float m = fmaxf(a.m, d.m);
     a.s = a.s * exp((double)a.m - m) + d.s * exp((double)d.m - m);
     a.m = m;
     if (better(d.score, d.best, best.score, best.at)) best = Best{d.score, d.best};
   }
-  join_lanes(a, 64, false, false);
+  join_lanes<64>(a, false, false);
   join_best(best, 64);
   if (lane == 0) write_draw<T>(R, row, a.m, a.s, best, action, logp);
-}
-
-// ---- gradients. Both losses have, per row, dL/dz_j = p_j (c0 + kl_coef (z_j - q_j - gap) + entropy_coef (z_j - m - level)) + [j = action] take, times one factor.
-struct Slope { float m, rs, c0, kl, gap, entropy, level, take; };
-
-template <typename T, bool MASK, bool REF, bool FULL>
-__device__ __forceinline__ void slope8(const Rows& R, const Piece<T, MASK>& P, const typename T::raw* q_row, const Slope& S, int action, typename T::raw* out) {
-  const Place& at = P.at;
-  float z[VEC], q[VEC], g[VEC];
-  const uint64_t ok = allowed_at<MASK, FULL>(R, P.mask, at);
-  take8<T, MASK, FULL>(R, P.z_row, ok, at, z);
-  if (REF) take8<T, MASK, FULL>(R, q_row, ok, at, q);
-#pragma unroll
-  for (int i = 0; i < VEC; i++) {
-    const float d = z[i] - S.m, p = fall(d) * S.rs;
-    float v = S.c0 + S.entropy * (d - S.level);
-    if (REF) v += S.kl * (z[i] - q[i] - S.gap);
-    g[i] = p == 0.f ? 0.f : p * v;                       // not allowed, or too unlikely for 32 bits: the limit, whatever q holds
-    if (at.j + i == action) g[i] += S.take;
-  }
-  if (FULL) {
-    store8(T{}, out + at.j, g);
-  } else {
-#pragma unroll
-    for (int i = 0; i < VEC; i++) if (at.j + i < R.actions) out[at.j + i] = narrow(T{}, g[i]);
-  }
-}
-// a piece of a row of the gradient; a row that does not count is zero and its logits are not read
-template <typename T, bool MASK, bool REF> __device__ __forceinline__ void write_slope(const Rows& R, int row, int piece, const Slope& S, long long action, bool counts, void* grad) {
-  typename T::raw* out = (typename T::raw*)grad + (long long)row * R.actions;
-  Piece<T, MASK> P(R, row, piece);
-  if (!counts) {
-    const float zero[VEC] = {};
-    for (int i = 0; i < P.tiles; i++, P.at.j += TILE) {
-      if (P.at.j + VEC <= R.actions) store8(T{}, out + P.at.j, zero);
-      else for (int n = P.at.j; n < R.actions; n++) out[n] = narrow(T{}, 0.f);
-    }
-    return;
-  }
-  const auto* q_row = REF ? (const typename T::raw*)R.ref + row * R.ref_stride : nullptr;
-#pragma unroll 2
-  for (int i = 0; i < P.whole; i++) {
-    slope8<T, MASK, REF, true>(R, P, q_row, S, (int)action, out);
-    P.at.next(P.step_mod, R.mask_len);
-  }
-  if (P.whole < P.tiles) slope8<T, MASK, REF, false>(R, P, q_row, S, (int)action, out);
-}
-
-// ---- clipped policy loss. Per row: ratio r = exp(logp - old), L = -min(r A, clip(r, 1 - lo, 1 + hi) A) + kl_coef KL(p || q) - entropy_coef H; the mean over the rows that count.
-struct Clip {
-  const int64_t* action; const float* old_logp; const float* advantage;
-  float lo, hi, kl_coef, entropy_coef, scale;   // scale: a factor of the gradient
-  const float* upstream;                        // another, on the device (autograd's), or null
-};
-struct ClipRow { float logp, kl, entropy, loss, take; double shift, ls; };
-// normalisers in 64 bits: KL = k / s - (lse - lse_q) is a small difference of large numbers
-template <typename T, bool REF> __device__ __forceinline__ ClipRow clip_row(const Rows& R, const Clip& C, int row, const Sums& a) {
-  ClipRow c{};
-  c.ls = log(a.s);
-  c.shift = REF ? (double)a.m - a.mq + c.ls - log(a.sq) : 0;
-  const float z = widen(T{}, ((const typename T::raw*)R.logits)[row * R.stride + C.action[row]]), adv = C.advantage[row];
-  c.logp = (float)((double)z - a.m - c.ls);
-  c.kl = REF ? (float)(a.k / a.s - c.shift) : 0;
-  c.entropy = (float)(c.ls - a.t / a.s);
-  const float ratio = expf(c.logp - C.old_logp[row]), free = ratio * adv, held = fminf(fmaxf(ratio, 1 - C.lo), 1 + C.hi) * adv;
-  c.take = held < free ? 0.f : -adv * ratio;     // the clipped branch has no slope; NaN stays
-  c.loss = -(held < free ? held : free) + (REF ? C.kl_coef * c.kl : 0.f) - C.entropy_coef * c.entropy;
-  return c;
-}
-__device__ __forceinline__ int count_rows(const int* counts, int rows) {   // of the workgroup, in every thread
-  __shared__ int wave[THREADS / 64];
-  int n = 0;
-  for (int i = threadIdx.x; i < rows; i += THREADS) n += counts[i];
-  n = lanes_sum(n);
-  if ((threadIdx.x & 63) == 0) wave[threadIdx.x >> 6] = n;
-  __syncthreads();
-  n = 0;
-  for (int i = 0; i < THREADS / 64; i++) n += wave[i];
-  return n;
-}
-// loss and per-row terms, by one workgroup: groups of `width` lanes join a row's records; row losses add up in 64 bits in a fixed order
-template <typename T, bool REF> __device__ __forceinline__ void clip_loss(const Rows& R, const Clip& C, const Part* parts, const int* counts, float* loss, float* logp, float* kl, float* entropy) {
-  int width = 1;
-  while (width < 64 && width < R.splits) width *= 2;
-  const int lane = threadIdx.x & (width - 1);
-  double sum = 0;
-  for (int base = 0; base < R.rows; base += THREADS / width) {     // every lane takes every turn: the joins shuffle
-    const int row = base + threadIdx.x / width;
-    const bool in = row < R.rows;
-    const Sums a = join_row(parts + (size_t)(in ? row : 0) * R.splits, R.splits, lane, width, REF);
-    if (!in || lane) continue;
-    ClipRow c{};
-    if (counts[row]) c = clip_row<T, REF>(R, C, row, a);
-    logp[row] = c.logp; kl[row] = c.kl; entropy[row] = c.entropy;
-    sum += c.loss;
-  }
-  __shared__ double wave[THREADS / 64];
-  sum = lanes_sum(sum);
-  if ((threadIdx.x & 63) == 0) wave[threadIdx.x >> 6] = sum;
-  const int n = count_rows(counts, R.rows);      // (its barrier)
-  if (threadIdx.x == 0) {
-    sum = 0;
-    for (int i = 0; i < THREADS / 64; i++) sum += wave[i];
-    *loss = (float)(sum / (n > 1 ? n : 1));
-  }
-}
-template <typename T, bool REF> __global__ void __launch_bounds__(THREADS) ur5_policy_clip_loss(Rows R, Clip C, const Part* parts, const int* counts, float* loss, float* logp, float* kl, float* entropy) {
-  clip_loss<T, REF>(R, C, parts, counts, loss, logp, kl, entropy);
-}
-// the gradient's pieces, in the statistics' order and, as 8 workgroups come before them, on the same XCD (whose L2 then holds a piece's logits if they fit). The first
-// of the 8 writes the loss, if asked for, while the others run.
-constexpr int FIRST = 8;
-template <typename T, bool MASK, bool REF> __global__ void __launch_bounds__(THREADS) ur5_policy_clip_grad(Rows R, Clip C, const Part* parts, const int* counts, void* grad, float* loss, float* logp, float* kl, float* entropy) {
-  const int block = (int)blockIdx.x - FIRST;
-  if (block < 0) {
-    if (loss && blockIdx.x == 0) clip_loss<T, REF>(R, C, parts, counts, loss, logp, kl, entropy);
-    return;
-  }
-  const int row = block / R.splits, piece = block % R.splits;
-  const bool on = counts[row];
-  __shared__ Slope shared;
-  const int n = count_rows(counts, R.rows);
-  if (on) {
-    const Sums a = join_row(parts + (size_t)row * R.splits, R.splits, threadIdx.x & 63, 64, REF);
-    if (threadIdx.x == 0) {
-      const ClipRow c = clip_row<T, REF>(R, C, row, a);
-      const float w = (C.upstream ? *C.upstream : 1.f) * C.scale / (float)n;
-      shared = Slope{a.m, (float)(w / a.s), -c.take, C.kl_coef, (float)(c.shift + c.kl), C.entropy_coef, (float)(c.ls - c.entropy), w * c.take};
-    }
-  }
-  __syncthreads();
-  write_slope<T, MASK, REF>(R, row, piece, shared, C.action[row], on, grad);
-}
-
-// ---- preference loss. Episodes are runs of rows: episode k holds the rows offsets[k] .. offsets[k + 1]. S_k = sum over its counting rows of logp - ref_logp,
-// margin_i = beta (S_2i - S_2i+1), loss = mean over pairs of (1 - eps) softplus(-margin) + eps softplus(margin).
-struct Prefer {
-  const int64_t* action; const float* ref_logp; const int64_t* offsets;
-  int pairs; double beta, eps; float scale; const float* upstream;
-};
-struct RowState { float m, rs, weight; int counts; };   // weight: d loss / d logp of the row
-constexpr int PAIR_THREADS = 1024;
-// one workgroup: log-probabilities of all rows, then a wavefront per pair
-template <typename T> __global__ void __launch_bounds__(PAIR_THREADS) ur5_policy_prefer_pairs(Rows R, Prefer P, const Part* parts, const int* counts, RowState* state, double* ratio, float* loss, float* margin) {
-  int width = 1;
-  while (width < 64 && width < R.splits) width *= 2;
-  const int sub = threadIdx.x & (width - 1);
-  for (int base = 0; base < R.rows; base += PAIR_THREADS / width) {
-    const int row = base + threadIdx.x / width;
-    const bool in = row < R.rows;
-    const Sums a = join_row(parts + (size_t)(in ? row : 0) * R.splits, R.splits, sub, width, false);
-    if (!in || sub) continue;
-    double l = 0;
-    if (counts[row]) l = (double)widen(T{}, ((const typename T::raw*)R.logits)[row * R.stride + P.action[row]]) - a.m - log(a.s) - P.ref_logp[row];
-    ratio[row] = l;
-    state[row] = RowState{a.m, (float)(1 / a.s), 0.f, counts[row]};
-  }
-  __syncthreads();
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  __shared__ double sums[PAIR_THREADS / 64];
-  double total = 0;
-  for (int i = wave; i < P.pairs; i += PAIR_THREADS / 64) {
-    long long end[3];
-    for (int k = 0; k < 3; k++) end[k] = min(max(P.offsets[2 * i + k], 0ll), (long long)R.rows);   // offsets outside the rows are taken as their ends
-    double d = 0;
-    for (long long r = end[0] + lane; r < end[1]; r += 64) d += ratio[r];
-    for (long long r = end[1] + lane; r < end[2]; r += 64) d -= ratio[r];
-    const double mg = P.beta * lanes_sum(d);
-    const double up = 1 / (1 + exp(mg));                                       // sigmoid(-margin)
-    const double soft = fmax(mg, 0.0) + log1p(exp(-fabs(mg)));                 // softplus(margin)
-    if (lane == 0) { margin[i] = (float)mg; total += (1 - P.eps) * (soft - mg) + P.eps * soft; }
-    const float w = (float)(-P.beta * ((1 - P.eps) * up - P.eps * (1 - up)) / P.pairs);
-    for (long long r = end[0] + lane; r < end[1]; r += 64) state[r].weight = w;
-    for (long long r = end[1] + lane; r < end[2]; r += 64) state[r].weight = -w;
-  }
-  if (lane == 0) sums[wave] = total;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    total = 0;
-    for (int k = 0; k < PAIR_THREADS / 64; k++) total += sums[k];
-    *loss = (float)(total / P.pairs);
-  }
-}
-template <typename T, bool MASK> __global__ void __launch_bounds__(THREADS) ur5_policy_prefer_grad(Rows R, Prefer P, const RowState* state, void* grad) {
-  const int row = blockIdx.x / R.splits, piece = blockIdx.x % R.splits;
-  const RowState s = state[row];
-  const float w = s.weight * (P.upstream ? *P.upstream : 1.f) * P.scale;
-  const Slope S{s.m, s.rs, -w, 0, 0, 0, 0, w};
-  write_slope<T, MASK, false>(R, row, piece, S, P.action[row], s.counts && s.weight != 0.f, grad);
 }
 
 }  // namespace ur5policy

@@ -36,51 +36,58 @@ int no_device(const char* entry, hipError_t e) {
   return e == hipErrorNoDevice ? fail(UR5_ERR_NOGPU, entry, "no HIP device visible: libur5sim.so runs on an MI355X (gfx950) only, there is no CPU fallback") : fail(UR5_ERR_DEVICE, entry, hipGetErrorString(e));
 }
 
-// ---- how rows are cut. A piece is `per` tiles of 2048 actions. About 4096 pieces in all keep 256 CUs busy to the end (8 workgroups fit on a CU); a row of a large batch
-// is not cut finer than that needs, and never into pieces of more than 16 tiles, so that a thread's fp32 sums stay short.
-constexpr int64_t WANTED = 4096, MOST_PER = 16;
-void cut(int64_t rows, int64_t actions, int* splits, int* per) {
-  const int64_t tiles = (actions + TILE - 1) / TILE;
-  int64_t p = rows * tiles / WANTED;
-  p = p < 1 ? 1 : p > MOST_PER ? MOST_PER : p;
-  *splits = (int)((tiles + p - 1) / p);
-  *per = (int)p;
+// ---- how rows are cut. Pieces grow from one turn of 256 threads first over the maps, which share a list of allowed pixels, then along the pixels, up to 64 turns, so that a
+// thread's fp32 sums stay short (512 terms); images of less than 2048 pixels take as many maps as fill a workgroup. How many pieces a call aims at: more fill the card's 256 CUs
+// (8 workgroups each) more evenly, fewer share what a piece costs before and after its loads. us of the kernel at 2048 / 4096 / 8192 / 16384 pieces wanted:
+// sample (512 fp32 rows) 103 / 106 / 126 / 169, logp (2000 x 40 000 bf16) 45 / 37 / 39 / 49, statistics (513 bf16 rows) 106 / 100 / 94 / 103, gradient 131 / 110 / 102 / 98.
+constexpr int64_t PIECES = 4096, PIECES_LOSS = 8192, PIECES_GRADIENT = 16384, MOST_TURNS = 64;
+int64_t clamp(int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : v > hi ? hi : v; }
+void cut(int64_t rows, int64_t actions, int64_t mask_len, int64_t wanted, Rows* R) {
+  const int64_t pixels = mask_len ? mask_len : actions, maps = actions / pixels, tiles = (pixels + TILE - 1) / TILE, groups = (pixels + VEC - 1) / VEC;
+  const int64_t turns = clamp(rows * tiles * maps / wanted, 1, MOST_TURNS);
+  int64_t maps_per = clamp(turns, 1, maps), per = clamp(turns / maps_per, 1, mask_len ? MOST_PER_MASKED : MOST_PER);
+  if (groups < THREADS) maps_per = clamp(THREADS / groups * maps_per, 1, maps);
+  R->rows = (int)rows; R->actions = (int)actions; R->pixels = (int)pixels; R->maps = (int)maps; R->per = (int)per; R->maps_per = (int)maps_per;
+  R->pieces_x = (int)((tiles + per - 1) / per);
+  R->pieces = (int)(R->pieces_x * ((maps + maps_per - 1) / maps_per));
 }
-// workspace: records | a flag per row | states and log ratios of the preference loss
-struct Work { Part* parts; int* counts; RowState* state; double* ratio; };
-int64_t lay_out(int64_t rows, int64_t actions, void* base, Work* w) {
-  int splits, per;
-  cut(rows, actions, &splits, &per);
+// workspace: records | slopes | terms of the loss (one per row; one per pair where there are more pairs than rows)
+struct Work { Part* parts; Slope* slopes; double* term; };
+int64_t lay_out(const Rows& R, int64_t terms, void* base, Work* w) {
   char* p = (char*)base;
-  const int64_t parts = rows * splits * (int64_t)sizeof(Part), state = rows * (int64_t)sizeof(RowState), ratio = (rows + 1) / 2 * 16, counts = (rows + 3) / 4 * 16;
-  if (w) *w = Work{(Part*)p, (int*)(p + parts + state + ratio), (RowState*)(p + parts), (double*)(p + parts + state)};
-  return parts + state + ratio + counts;
+  const int64_t n = R.rows, parts = n * R.pieces * (int64_t)sizeof(Part), slopes = (n * (int64_t)sizeof(Slope) + 15) / 16 * 16;
+  if (w) *w = Work{(Part*)p, (Slope*)(p + parts), (double*)(p + parts + slopes)};
+  return parts + slopes + (terms > n ? terms : n) * 8;
 }
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 constexpr int64_t MOST = 0x7fffffff;
 
+const char* check_size(int64_t rows, int64_t actions, int64_t mask_len, int64_t pairs, int64_t wanted, Rows* R) {
+  if (rows < 0 || actions < 1) return "rows must be at least 0 and actions at least 1";
+  if (actions > MOST - 2 * TILE * MOST_PER || rows > MOST / 64 || pairs > MOST / 64) return "too many rows, pairs (2^25) or actions (2^31 - 65537)";
+  if (mask_len < 0 || (mask_len && actions % mask_len)) return "mask_len must divide actions";
+  cut(rows, actions, mask_len, PIECES_GRADIENT, R);
+  const int64_t most = R->pieces;                    // the finest of the cuts
+  cut(rows, actions, mask_len, wanted, R);
+  if (rows * most > MOST - (rows + THREADS) / THREADS - FIRST) return "too many logits in one call";
+  return nullptr;
+}
 // checks what every entry point over rows checks; launches nothing
-const char* check_rows(const ur5_rows* r, Rows* R, Work* w) {
+const char* check_rows(const ur5_rows* r, int64_t pairs, int64_t wanted, Rows* R, Work* w) {
   if (!r) return "no rows";
   if (r->dtype != UR5_F32 && r->dtype != UR5_F16 && r->dtype != UR5_BF16) return "dtype must be UR5_F32, UR5_F16 or UR5_BF16";
-  if (r->rows < 0 || r->actions < 1) return "rows must be at least 0 and actions at least 1";
-  if (r->actions > MOST - 2 * TILE * MOST_PER || r->rows > MOST / 64) return "too many rows or actions (2^31 - 65537 actions, 2^25 rows)";
-  int splits, per;
-  cut(r->rows, r->actions, &splits, &per);
-  if (r->rows * splits > MOST - FIRST) return "too many logits in one call";
+  if (r->mask && (r->mask_len < 1 || r->mask_stride < 0)) return "mask_len must be at least 1 and mask_stride at least 0";
+  if (const char* why = check_size(r->rows, r->actions, r->mask ? r->mask_len : 0, pairs, wanted, R)) return why;
   if (r->stride < r->actions && r->rows > 1) return "the row stride is smaller than a row";
   if (r->ref && r->ref_stride < r->actions && r->rows > 1) return "the reference's row stride is smaller than a row";
-  if (r->mask && (r->mask_len < 1 || r->actions % r->mask_len || r->mask_stride < 0)) return "mask_len must divide actions, and mask_stride be at least 0";
   if (r->rows && !r->logits) return "no logits";
-  if (r->rows && (!r->work || !aligned16(r->work) || r->work_bytes < lay_out(r->rows, r->actions, nullptr, nullptr))) return "the workspace is missing, not 16-byte aligned, or smaller than ur5_policy_work_bytes";
-  *R = Rows{r->logits, r->ref, r->mask, r->stride, r->ref_stride, r->mask_stride, (int)r->rows, (int)r->actions, (int)(r->mask ? r->mask_len : r->actions), splits, per};
-  if (w) lay_out(r->rows, r->actions, r->work, w);
+  if ((r->rows || pairs) && (!r->work || !aligned16(r->work) || r->work_bytes < lay_out(*R, pairs, nullptr, nullptr))) return "the workspace is missing, not 16-byte aligned, or smaller than ur5_policy_work_bytes";
+  R->logits = r->logits; R->ref = r->ref; R->mask = r->mask; R->stride = r->stride; R->ref_stride = r->ref_stride; R->mask_stride = r->mask_stride;
+  lay_out(*R, pairs, r->work, w);
   return nullptr;
 }
 
 template <typename F> void by_type(int dtype, F f) { dtype == UR5_F32 ? f(f32_t{}) : dtype == UR5_F16 ? f(f16_t{}) : f(bf16_t{}); }
-struct yes { static constexpr bool value = true; };
-struct no { static constexpr bool value = false; };
 template <typename F> void by_flag(bool b, F f) { b ? f(yes{}) : f(no{}); }
 
 const char* check_clip(const ur5_rows* r, const ur5_clip* c) {
@@ -90,24 +97,37 @@ const char* check_clip(const ur5_rows* r, const ur5_clip* c) {
   if (c->kl_coef > 0 && !r->ref && r->rows) return "kl_coef needs reference logits";
   return nullptr;
 }
-Clip clip_of(const ur5_clip* c) { return Clip{c->action, c->old_logp, c->advantage, c->clip_low, c->clip_high, c->kl_coef, c->entropy_coef, c->grad_scale, c->upstream}; }
+Clip clip_of(const ur5_clip* c) { return Clip{c->action, c->old_logp, c->advantage, c->clip_low, c->clip_high, c->kl_coef, c->entropy_coef}; }
 const char* check_prefer(const ur5_rows* r, const ur5_prefer* p) {
   if (!p || (r->rows && (!p->action || !p->ref_logp))) return "action and ref_logp are needed";
-  if (p->pairs < 1 || p->pairs > MOST / 4 || !p->offsets) return "pairs must be at least 1, with 2 pairs + 1 offsets";
+  if (p->pairs < 1 ||  !p->offsets) return "pairs must be at least 1, with 2 pairs + 1 offsets";
   if (!(p->beta > 0) || !(p->label_smoothing >= 0 && p->label_smoothing <= 0.5)) return "beta must be above 0 and label_smoothing lie in [0, 0.5]";
   return nullptr;
 }
-Prefer prefer_of(const ur5_prefer* p) { return Prefer{p->action, p->ref_logp, p->offsets, (int)p->pairs, p->beta, p->label_smoothing, p->grad_scale, p->upstream}; }
+Prefer prefer_of(const ur5_prefer* p) { return Prefer{p->action, p->ref_logp, p->offsets, (int)p->pairs, p->beta, p->label_smoothing}; }
 
-void stats(const Rows& R, int dtype, hipStream_t s, const int64_t* action, const Work& w) {
+void stats(const Rows& R, int dtype, hipStream_t s, const Span& span, const int64_t* action, const Work& w) {
   if (!R.rows) return;
+  const int front = (R.rows + 8 * THREADS - 1) / (8 * THREADS) * 8;
   by_type(dtype, [&](auto t) { by_flag(R.mask, [&](auto m) { by_flag(R.ref, [&](auto q) {
-    ur5_policy_stats<decltype(t), decltype(m)::value, decltype(q)::value><<<R.rows * R.splits, THREADS, 0, s>>>(R, action, w.parts, w.counts);
+    ur5_policy_stats<decltype(t), decltype(m)::value, decltype(q)::value><<<front + R.rows * R.pieces, THREADS, 0, s>>>(R, span, front, action, w.parts, w.slopes);
   }); }); });
 }
-void clip_grad(const Rows& R, int dtype, hipStream_t s, const Clip& C, const Work& w, void* grad, float* loss, float* logp, float* kl, float* entropy) {
-  by_type(dtype, [&](auto t) { by_flag(R.mask, [&](auto m) { by_flag(R.ref, [&](auto q) {
-    ur5_policy_clip_grad<decltype(t), decltype(m)::value, decltype(q)::value><<<FIRST + R.rows * R.splits, THREADS, 0, s>>>(R, C, w.parts, w.counts, grad, loss, logp, kl, entropy);
+// the rows of the clipped loss, or the pairs of the preference loss: slopes and terms
+void clip_rows(const Rows& R, int dtype, hipStream_t s, const Clip& C, const Work& w, float* logp, float* kl, float* entropy) {
+  stats(R, dtype, s, Span{}, C.action, w);
+  if (R.rows) by_type(dtype, [&](auto t) { by_flag(R.ref, [&](auto q) {
+    ur5_policy_clip_rows<decltype(t), decltype(q)::value><<<(R.rows + WAVES - 1) / WAVES, THREADS, 0, s>>>(R, C, w.parts, w.slopes, w.term, logp, kl, entropy);
+  }); });
+}
+void prefer_pairs(const Rows& R, int dtype, hipStream_t s, const Prefer& P, const Work& w, float* margin) {
+  stats(R, dtype, s, Span{P.offsets, 2 * P.pairs}, P.action, w);
+  by_type(dtype, [&](auto t) { ur5_policy_prefer_pairs<decltype(t)><<<P.pairs, THREADS, 0, s>>>(R, P, w.parts, w.slopes, w.term, margin); });
+}
+void gradient(Rows R, int dtype, hipStream_t s, const Terms& t, const int64_t* action, const Work& w, float scale, const float* upstream, void* grad) {
+  cut(R.rows, R.actions, R.mask ? R.pixels : 0, PIECES_GRADIENT, &R);      // it leaves no records
+  by_type(dtype, [&](auto k) { by_flag(R.mask, [&](auto m) { by_flag(R.ref, [&](auto q) {
+    ur5_policy_grad<decltype(k), decltype(m)::value, decltype(q)::value><<<FIRST + R.rows * R.pieces, THREADS, 0, s>>>(R, t, action, w.slopes, scale, upstream, grad);
   }); }); });
 }
 }  // namespace
@@ -117,101 +137,106 @@ void clip_grad(const Rows& R, int dtype, hipStream_t s, const Clip& C, const Wor
 
 extern "C" {
 
-int64_t ur5_policy_work_bytes(int64_t rows, int64_t actions) {
-  if (rows < 0 || actions < 1 || rows > MOST / 64 || actions > MOST) return 0;
-  return lay_out(rows, actions, nullptr, nullptr);
+int64_t ur5_policy_work_bytes(int64_t rows, int64_t actions, int64_t mask_len, int64_t pairs) {
+  Rows R;
+  return pairs < 0 || check_size(rows, actions, mask_len, pairs, PIECES_LOSS, &R) ? 0 : lay_out(R, pairs, nullptr, nullptr);
 }
 
 int ur5_policy_sample(const ur5_rows* r, uint64_t offset, const int64_t* gids, int64_t* action, float* logp) {
   Rows R; Work w;
-  CHECK(check_rows(r, &R, &w));
+  CHECK(check_rows(r, 0, PIECES, &R, &w));
   if (!R.rows) return 0;
   if (!gids || !action || !logp) return fail(UR5_ERR_ARG, __func__, "gids, action and logp are needed");
   ON(r->device);
   const hipStream_t s = (hipStream_t)r->stream;
   Draw* draws = (Draw*)w.parts;
   by_type(r->dtype, [&](auto t) {
-    by_flag(R.mask, [&](auto m) { ur5_policy_sample<decltype(t), decltype(m)::value><<<R.rows * R.splits, THREADS, 0, s>>>(R, offset, gids, draws, action, logp); });
-    if (R.splits > 1) ur5_policy_sample_rows<decltype(t)><<<(R.rows + 3) / 4, THREADS, 0, s>>>(R, draws, action, logp);
+    by_flag(R.mask, [&](auto m) { ur5_policy_sample<decltype(t), decltype(m)::value><<<R.rows * R.pieces, THREADS, 0, s>>>(R, offset, gids, draws, action, logp); });
+    if (R.pieces > 1) ur5_policy_sample_rows<decltype(t)><<<(R.rows + WAVES - 1) / WAVES, THREADS, 0, s>>>(R, draws, action, logp);
   });
   return launched(__func__);
 }
 
 int ur5_policy_logp(const ur5_rows* r, const int64_t* action, float* logp, float* entropy) {
   Rows R; Work w;
-  CHECK(check_rows(r, &R, &w));
+  CHECK(check_rows(r, 0, PIECES, &R, &w));
   if (!R.rows) return 0;
   if (!action || !logp) return fail(UR5_ERR_ARG, __func__, "action and logp are needed");
   ON(r->device);
   const hipStream_t s = (hipStream_t)r->stream;
   by_type(r->dtype, [&](auto t) {
-    by_flag(R.mask, [&](auto m) { ur5_policy_logp<decltype(t), decltype(m)::value><<<R.rows * R.splits, THREADS, 0, s>>>(R, action, w.parts, logp, entropy); });
-    if (R.splits > 1) ur5_policy_logp_rows<decltype(t)><<<(R.rows + 3) / 4, THREADS, 0, s>>>(R, action, w.parts, logp, entropy);
+    by_flag(R.mask, [&](auto m) { ur5_policy_logp<decltype(t), decltype(m)::value><<<R.rows * R.pieces, THREADS, 0, s>>>(R, action, w.parts, logp, entropy); });
+    if (R.pieces > 1) ur5_policy_logp_rows<decltype(t)><<<(R.rows + WAVES - 1) / WAVES, THREADS, 0, s>>>(R, action, w.parts, logp, entropy);
   });
   return launched(__func__);
 }
 
 int ur5_policy_clip_loss(const ur5_rows* r, const ur5_clip* c, float* loss, float* logp, float* kl, float* entropy) {
   Rows R; Work w;
-  CHECK(check_rows(r, &R, &w));
+  CHECK(check_rows(r, 0, PIECES_LOSS, &R, &w));
   CHECK(check_clip(r, c));
   if (!loss || (R.rows && (!logp || !kl || !entropy))) return fail(UR5_ERR_ARG, __func__, "loss, logp, kl and entropy are needed");
   ON(r->device);
   const hipStream_t s = (hipStream_t)r->stream;
-  stats(R, r->dtype, s, c->action, w);
-  by_type(r->dtype, [&](auto t) { by_flag(R.ref, [&](auto q) {
-    ur5_policy_clip_loss<decltype(t), decltype(q)::value><<<1, THREADS, 0, s>>>(R, clip_of(c), w.parts, w.counts, loss, logp, kl, entropy);
-  }); });
+  clip_rows(R, r->dtype, s, clip_of(c), w, logp, kl, entropy);
+  ur5_policy_loss<<<1, THREADS, 0, s>>>(Terms{w.term, R.rows, 0, w.slopes, R.rows, loss});
   return launched(__func__);
 }
-
 int ur5_policy_clip_grad(const ur5_rows* r, const ur5_clip* c, void* grad) {
   Rows R; Work w;
-  CHECK(check_rows(r, &R, &w));
+  CHECK(check_rows(r, 0, PIECES_LOSS, &R, &w));
   CHECK(check_clip(r, c));
   if (!R.rows) return 0;
   if (!grad) return fail(UR5_ERR_ARG, __func__, "grad is needed");
   ON(r->device);
-  clip_grad(R, r->dtype, (hipStream_t)r->stream, clip_of(c), w, grad, nullptr, nullptr, nullptr, nullptr);
+  gradient(R, r->dtype, (hipStream_t)r->stream, Terms{}, c->action, w, c->grad_scale, c->upstream, grad);
   return launched(__func__);
 }
-
 int ur5_policy_clip_loss_grad(const ur5_rows* r, const ur5_clip* c, float* loss, float* logp, float* kl, float* entropy, void* grad) {
   Rows R; Work w;
-  CHECK(check_rows(r, &R, &w));
+  CHECK(check_rows(r, 0, PIECES_LOSS, &R, &w));
   CHECK(check_clip(r, c));
   if (!loss || (R.rows && (!logp || !kl || !entropy || !grad))) return fail(UR5_ERR_ARG, __func__, "loss, logp, kl, entropy and grad are needed");
   ON(r->device);
-  stats(R, r->dtype, (hipStream_t)r->stream, c->action, w);
-  clip_grad(R, r->dtype, (hipStream_t)r->stream, clip_of(c), w, grad, loss, logp, kl, entropy);
+  const hipStream_t s = (hipStream_t)r->stream;
+  clip_rows(R, r->dtype, s, clip_of(c), w, logp, kl, entropy);
+  gradient(R, r->dtype, s, Terms{w.term, R.rows, 0, w.slopes, R.rows, loss}, c->action, w, c->grad_scale, c->upstream, grad);
   return launched(__func__);
 }
 
 int ur5_policy_prefer_loss(const ur5_rows* r, const ur5_prefer* p, float* loss, float* margin) {
   Rows R; Work w;
-  CHECK(check_rows(r, &R, &w));
+  CHECK(check_rows(r, p ? p->pairs : 0, PIECES_LOSS, &R, &w));
   CHECK(check_prefer(r, p));
   if (!loss || !margin) return fail(UR5_ERR_ARG, __func__, "loss and margin are needed");
   R.ref = nullptr;
   ON(r->device);
   const hipStream_t s = (hipStream_t)r->stream;
-  stats(R, r->dtype, s, p->action, w);
-  by_type(r->dtype, [&](auto t) { ur5_policy_prefer_pairs<decltype(t)><<<1, PAIR_THREADS, 0, s>>>(R, prefer_of(p), w.parts, w.counts, w.state, w.ratio, loss, margin); });
+  prefer_pairs(R, r->dtype, s, prefer_of(p), w, margin);
+  ur5_policy_loss<<<1, THREADS, 0, s>>>(Terms{w.term, (int)p->pairs, (int)p->pairs, w.slopes, R.rows, loss});
   return launched(__func__);
 }
-
 int ur5_policy_prefer_grad(const ur5_rows* r, const ur5_prefer* p, void* grad) {
   Rows R; Work w;
-  CHECK(check_rows(r, &R, &w));
+  CHECK(check_rows(r, p ? p->pairs : 0, PIECES_LOSS, &R, &w));
   CHECK(check_prefer(r, p));
   if (!R.rows) return 0;
   if (!grad) return fail(UR5_ERR_ARG, __func__, "grad is needed");
   R.ref = nullptr;
   ON(r->device);
+  gradient(R, r->dtype, (hipStream_t)r->stream, Terms{}, p->action, w, p->grad_scale, p->upstream, grad);
+  return launched(__func__);
+}
+int ur5_policy_prefer_loss_grad(const ur5_rows* r, const ur5_prefer* p, float* loss, float* margin, void* grad) {
+  Rows R; Work w;
+  CHECK(check_rows(r, p ? p->pairs : 0, PIECES_LOSS, &R, &w));
+  CHECK(check_prefer(r, p));
+  if (!loss || !margin || (R.rows && !grad)) return fail(UR5_ERR_ARG, __func__, "loss, margin and grad are needed");
+  R.ref = nullptr;
+  ON(r->device);
   const hipStream_t s = (hipStream_t)r->stream;
-  by_type(r->dtype, [&](auto t) { by_flag(R.mask, [&](auto m) {
-    ur5_policy_prefer_grad<decltype(t), decltype(m)::value><<<R.rows * R.splits, THREADS, 0, s>>>(R, prefer_of(p), w.state, grad);
-  }); });
+  prefer_pairs(R, r->dtype, s, prefer_of(p), w, margin);
+  gradient(R, r->dtype, s, Terms{w.term, (int)p->pairs, (int)p->pairs, w.slopes, R.rows, loss}, p->action, w, p->grad_scale, p->upstream, grad);
   return launched(__func__);
 }
 

@@ -24,7 +24,7 @@ EXPORTS = ["ur5_last_error", "ur5_create", "ur5_destroy", "ur5_num_envs", "ur5_n
 TEST_EXPORTS = ["ur5_forward_debug", "ur5_set_step_cap_dev", "ur5_model_uploads"]   # include/ur5sim_test.h: introspection for tests/ and tools/, not part of the boundary
 
 LEARN_EXPORTS = ["ur5_policy_work_bytes", "ur5_policy_sample", "ur5_policy_logp", "ur5_policy_clip_loss", "ur5_policy_clip_grad", "ur5_policy_clip_loss_grad",
-                 "ur5_policy_prefer_loss", "ur5_policy_prefer_grad", "ur5_act8_pack", "ur5_act8_unpack", "ur5_act8_wgrad_work_bytes", "ur5_act8_wgrad"]   # include/ur5learn.h
+                 "ur5_policy_prefer_loss", "ur5_policy_prefer_grad", "ur5_policy_prefer_loss_grad", "ur5_act8_pack", "ur5_act8_unpack", "ur5_act8_wgrad_work_bytes", "ur5_act8_wgrad"]   # include/ur5learn.h
 
 
 class Config(C.Structure):
@@ -115,7 +115,7 @@ def load(path=None):
     L.ur5_render_dev.argtypes = [vp, C.c_int, C.c_int, C.c_int, C.c_int, vp, vp]
     if hasattr(L, "ur5_policy_sample"):                        # the engine's host builds (tests) hold no learning operators
         i64, i32, rows = C.c_int64, C.c_int, C.POINTER(Rows)
-        L.ur5_policy_work_bytes.argtypes, L.ur5_policy_work_bytes.restype = [i64, i64], i64
+        L.ur5_policy_work_bytes.argtypes, L.ur5_policy_work_bytes.restype = [i64] * 4, i64
         L.ur5_policy_sample.argtypes = [rows, C.c_uint64, vp, vp, vp]
         L.ur5_policy_logp.argtypes = [rows, vp, vp, vp]
         L.ur5_policy_clip_loss.argtypes = [rows, C.POINTER(Clip), vp, vp, vp, vp]
@@ -123,6 +123,7 @@ def load(path=None):
         L.ur5_policy_clip_loss_grad.argtypes = [rows, C.POINTER(Clip), vp, vp, vp, vp, vp]
         L.ur5_policy_prefer_loss.argtypes = [rows, C.POINTER(Prefer), vp, vp]
         L.ur5_policy_prefer_grad.argtypes = [rows, C.POINTER(Prefer), vp]
+        L.ur5_policy_prefer_loss_grad.argtypes = [rows, C.POINTER(Prefer), vp, vp, vp]
         L.ur5_act8_pack.argtypes = [vp, i32, i64, i64, vp, vp, i32, vp]
         L.ur5_act8_unpack.argtypes = [vp, vp, i64, i64, vp, i32, i32, vp]
         L.ur5_act8_wgrad_work_bytes.argtypes, L.ur5_act8_wgrad_work_bytes.restype = [i64] * 4, i64

@@ -91,8 +91,8 @@ def _reference(ref, z, shape):
     return q
 
 
-def _work(lib, z):
-    return torch.empty(lib.ur5_policy_work_bytes(z.shape[0], z.shape[1]), dtype=torch.uint8, device=z.device)
+def _work(lib, z, mask, pairs=0):
+    return torch.empty(lib.ur5_policy_work_bytes(z.shape[0], z.shape[1], mask.shape[1] if mask is not None else 0, pairs), dtype=torch.uint8, device=z.device)
 
 
 def _rows(z, mask, ref, work):
@@ -113,7 +113,7 @@ def sample_actions(logits, seed, gids, round_index, mask=None, stream=SAMPLE_STR
     lib = native.load()
     action = torch.empty(z.shape[0], dtype=torch.int64, device=z.device)
     logp = torch.empty(z.shape[0], dtype=torch.float32, device=z.device)
-    r = _rows(z, m, None, _w := _work(lib, z))
+    r = _rows(z, m, None, _w := _work(lib, z, m))
     native.check(lib, lib.ur5_policy_sample(C.byref(r), sharding.scene_key_offset(seed, round_index, stream), g.data_ptr(), action.data_ptr(), logp.data_ptr()), "ur5_policy_sample")
     return action, logp
 
@@ -126,7 +126,7 @@ def action_log_probs(logits, action, mask=None):
     lib = native.load()
     out = torch.empty((2, z.shape[0]), dtype=torch.float32, device=z.device)
     logp, entropy = out[0], out[1]
-    r = _rows(z, m, None, _w := _work(lib, z))
+    r = _rows(z, m, None, _w := _work(lib, z, m))
     native.check(lib, lib.ur5_policy_logp(C.byref(r), a.data_ptr(), logp.data_ptr(), entropy.data_ptr()), "ur5_policy_logp")
     return logp, entropy
 
@@ -158,7 +158,7 @@ class _ClippedPolicyLoss(torch.autograd.Function):
     def forward(ctx, logits, tensors, numbers):
         z, _, _, _, mask, ref = tensors
         lib = native.load()
-        work = _work(lib, z)
+        work = _work(lib, z, mask)
         terms = _clip_outputs(z)
         r, c = _rows(z, mask, ref, work), _clip_struct(tensors, numbers)
         native.check(lib, lib.ur5_policy_clip_loss(C.byref(r), C.byref(c), *(t.data_ptr() for t in terms)), "ur5_policy_clip_loss")
@@ -193,14 +193,14 @@ def clipped_policy_loss(logits, action, old_logp, advantage, mask=None, ref_logi
 
 
 def clipped_policy_grad(logits, action, old_logp, advantage, mask=None, ref_logits=None, clip=0.2, kl_coef=0.0, entropy_coef=0.0, grad_scale=1.0):
-    """(``PolicyLoss``, its gradient times ``grad_scale`` with respect to the logits, in their shape and type) in two launches, without an autograd graph: for
+    """(``PolicyLoss``, its gradient times ``grad_scale`` with respect to the logits, in their shape and type) in three launches, without an autograd graph: for
     ``logits.backward(grad)``. float16 logits want a ``grad_scale``: the entries are about p / N."""
     tensors, numbers = _clip_inputs(logits, action, old_logp, advantage, mask, ref_logits, clip, kl_coef, entropy_coef)
     z = tensors[0]
     lib = native.load()
     terms = _clip_outputs(z)
     grad = torch.empty(logits.shape, dtype=z.dtype, device=z.device)
-    r, c = _rows(z, tensors[4], tensors[5], _w := _work(lib, z)), _clip_struct(tensors, numbers, float(grad_scale))
+    r, c = _rows(z, tensors[4], tensors[5], _w := _work(lib, z, tensors[4])), _clip_struct(tensors, numbers, float(grad_scale))
     native.check(lib, lib.ur5_policy_clip_loss_grad(C.byref(r), C.byref(c), *(t.data_ptr() for t in terms), grad.data_ptr()), "ur5_policy_clip_loss_grad")
     return PolicyLoss(*terms), grad
 
@@ -242,7 +242,7 @@ class _PreferenceLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tensors, numbers):
         lib = native.load()
-        work = _work(lib, tensors[0])
+        work = _work(lib, tensors[0], tensors[4], tensors[3].shape[0] // 2)
         loss, margin = _prefer_forward(lib, tensors, numbers, work)
         ctx.save_for_backward(*tensors, work)
         ctx.numbers, ctx.shape = numbers, logits.shape
@@ -272,7 +272,11 @@ def preference_loss(logits, action, ref_logp, offsets, mask=None, beta=0.1, labe
 def preference_grad(logits, action, ref_logp, offsets, mask=None, beta=0.1, label_smoothing=0.0, grad_scale=1.0):
     """(``PreferenceLoss``, its gradient times ``grad_scale`` with respect to the logits) without an autograd graph: for ``logits.backward(grad)``."""
     tensors, numbers = _prefer_inputs(logits, action, ref_logp, offsets, mask, beta, label_smoothing)
+    z, pairs = tensors[0], offsets.shape[0] // 2
     lib = native.load()
-    work = _work(lib, tensors[0])
-    terms = PreferenceLoss(*_prefer_forward(lib, tensors, numbers, work))
-    return terms, _prefer_backward(lib, tensors, numbers, work, float(grad_scale), None).view(logits.shape)
+    loss = torch.empty((), dtype=torch.float32, device=z.device)
+    margin = torch.empty(pairs, dtype=torch.float32, device=z.device)
+    grad = torch.empty(logits.shape, dtype=z.dtype, device=z.device)
+    r, p = _rows(z, tensors[4], None, _w := _work(lib, z, tensors[4], pairs)), _prefer_struct(tensors, numbers, float(grad_scale))
+    native.check(lib, lib.ur5_policy_prefer_loss_grad(C.byref(r), C.byref(p), loss.data_ptr(), margin.data_ptr(), grad.data_ptr()), "ur5_policy_prefer_loss_grad")
+    return PreferenceLoss(loss, margin), grad

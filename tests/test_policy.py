@@ -38,7 +38,7 @@ def _good_rows(**kw):
     lib = native.load()
     n, a = kw.pop("rows", 4), kw.pop("actions", 90)
     d = dict(logits=4096, ref=None, mask=None, stride=a, ref_stride=0, mask_stride=0, rows=n, actions=a, mask_len=0, dtype=0, device=0, stream=None, work=4096,
-             work_bytes=max(16, lib.ur5_policy_work_bytes(n, a) if n >= 0 and a >= 1 else 0))
+             work_bytes=max(16, lib.ur5_policy_work_bytes(n, a, 0, 1)))
     d.update(kw)
     return native.Rows(*[d[f] for f, _ in native.Rows._fields_])
 
@@ -53,7 +53,8 @@ def test_entry_points_refuse_bad_rows(change):
     c, p = native.Clip(4096, 4096, 4096, 0.2, 0.2, 0.0, 0.0, 1.0, None), native.Prefer(4096, 4096, 4096, 1, 0.1, 0.0, 1.0, None)
     for rc in (lib.ur5_policy_sample(C.byref(r), 1, 4096, 4096, 4096), lib.ur5_policy_logp(C.byref(r), 4096, 4096, 4096), lib.ur5_policy_clip_loss(C.byref(r), C.byref(c), *[4096] * 4),
                lib.ur5_policy_clip_grad(C.byref(r), C.byref(c), 4096), lib.ur5_policy_clip_loss_grad(C.byref(r), C.byref(c), *[4096] * 5),
-               lib.ur5_policy_prefer_loss(C.byref(r), C.byref(p), 4096, 4096), lib.ur5_policy_prefer_grad(C.byref(r), C.byref(p), 4096)):
+               lib.ur5_policy_prefer_loss(C.byref(r), C.byref(p), 4096, 4096), lib.ur5_policy_prefer_grad(C.byref(r), C.byref(p), 4096),
+               lib.ur5_policy_prefer_loss_grad(C.byref(r), C.byref(p), 4096, 4096, 4096)):
         assert rc == -1 and b"ur5_policy_" in lib.ur5_last_error()
 
 
@@ -74,7 +75,7 @@ def test_entry_points_refuse_bad_numbers_and_missing_outputs():
     assert lib.ur5_policy_clip_loss(C.byref(r), clip(), None, 4096, 4096, 4096) == -1 and lib.ur5_policy_clip_grad(C.byref(r), clip(), None) == -1
     assert lib.ur5_policy_prefer_loss(C.byref(r), pref(), 4096, None) == -1 and lib.ur5_policy_prefer_grad(C.byref(r), pref(), None) == -1
     assert lib.ur5_policy_sample(C.byref(r), 0, None, 4096, 4096) == -1 and lib.ur5_policy_logp(C.byref(r), 4096, None, None) == -1 and lib.ur5_policy_sample(None, 0, 4096, 4096, 4096) == -1
-    assert lib.ur5_policy_work_bytes(-1, 5) == 0 and lib.ur5_policy_work_bytes(5, 0) == 0
+    assert all(lib.ur5_policy_work_bytes(*bad) == 0 for bad in ((-1, 5, 0, 0), (5, 0, 0, 0), (5, 6, 4, 0), (5, 6, -1, 0), (5, 6, 0, -1)))
 
 
 def test_no_gpu_is_an_error():
