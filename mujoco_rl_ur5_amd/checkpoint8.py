@@ -13,21 +13,23 @@ import threading
 
 import torch
 
-from . import native
-from .policy import DTYPES, _gpu
+from .policy import DTYPES, _check, _gpu, _library, _raw_stream
 
 GROUP = 64
 _active = threading.local()
-
-
-def _stream(t):
-    return torch.cuda.current_stream(t.device).cuda_stream
 
 
 def _float_gpu(t, what):
     _gpu(t, what)
     if t.dtype not in DTYPES:
         raise TypeError(f"{what} must be float32, float16 or bfloat16, not {t.dtype}")
+
+
+def _planes(shape):
+    """Planes of a tensor: groups never reach over a plane's end. [N, C, ...] has N C planes, a matrix its rows, a vector is one plane."""
+    if len(shape) > 2:
+        return shape[0] * shape[1]
+    return shape[0] if len(shape) == 2 else 1
 
 
 class PackedActivation:
@@ -37,61 +39,52 @@ class PackedActivation:
     def __init__(self, codes, scales, shape, dtype):
         self.codes, self.scales, self.shape, self.dtype = codes, scales, shape, dtype
 
-    def _size(self):
-        return _planes(self.shape)[1]
-
     def unpack(self):
         x = torch.empty(self.shape, dtype=self.dtype, device=self.codes.device)
-        if x.numel():
-            lib = native.load()
-            native.check(lib, lib.ur5_act8_unpack(self.codes.data_ptr(), self.scales.data_ptr(), self.codes.shape[0], self._size(), x.data_ptr(), DTYPES[self.dtype],
-                                                  x.device.index, _stream(x)), "ur5_act8_unpack")
+        count = x.numel()
+        if count:
+            planes, index = self.codes.shape[0], x.get_device()
+            _check(_library().ur5_act8_unpack(self.codes.data_ptr(), self.scales.data_ptr(), planes, count // planes, x.data_ptr(), DTYPES[self.dtype], index, _raw_stream(index)),
+                   "ur5_act8_unpack")
         return x
 
     def weight_grad(self, dy, bias=True):
         """For a pointwise convolution y[n, o] = sum_c w[o, c] x[n, c] + b[o] of the packed x [N, C, ...]: (dw float32 [O, C], db float32 [O]) from dy [N, O, ...] -- sums over images
         and pixels, the same every time. bias=False: (dw, None)."""
         _float_gpu(dy, "dy")
-        if len(self.shape) < 3 or dy.dim() != len(self.shape) or dy.shape[0] != self.shape[0] or dy.shape[2:] != self.shape[2:] or dy.device != self.codes.device:
-            raise ValueError(f"dy must be [N, O, ...] like the packed {tuple(self.shape)} on {self.codes.device}, not {tuple(dy.shape)} on {dy.device}")
-        n, cin, cout = self.shape[0], self.shape[1], dy.shape[1]
+        shape = self.shape
+        if len(shape) < 3 or shape[1] == 0 or dy.dim() != len(shape) or dy.shape[0] != shape[0] or dy.shape[2:] != shape[2:] or dy.get_device() != self.codes.get_device():
+            raise ValueError(f"dy must be [N, O, ...] like the packed {tuple(shape)} on {self.codes.device}, not {tuple(dy.shape)} on {dy.device}")
+        n, cin, cout = shape[0], shape[1], dy.shape[1]
         dw = torch.empty((cout, cin), dtype=torch.float32, device=dy.device)
         db = torch.empty(cout, dtype=torch.float32, device=dy.device) if bias else None
-        if dy.numel() == 0 or cin == 0:
+        if dy.numel() == 0:
             return dw.zero_(), db.zero_() if bias else None
         dy = dy.detach().contiguous()
-        lib = native.load()
-        work = torch.empty(max(1, lib.ur5_act8_wgrad_work_bytes(n, cin, cout, self._size())), dtype=torch.uint8, device=dy.device)
-        native.check(lib, lib.ur5_act8_wgrad(self.codes.data_ptr(), self.scales.data_ptr(), dy.data_ptr(), DTYPES[dy.dtype], n, cin, cout, self._size(), dw.data_ptr(),
-                                             db.data_ptr() if bias else None, work.data_ptr(), work.numel(), dy.device.index, _stream(dy)), "ur5_act8_wgrad")
+        size, index, lib = dy.numel() // (n * cout), dy.get_device(), _library()
+        work = torch.empty(max(1, lib.ur5_act8_wgrad_work_bytes(n, cin, cout, size)), dtype=torch.uint8, device=dy.device)
+        _check(lib.ur5_act8_wgrad(self.codes.data_ptr(), self.scales.data_ptr(), dy.data_ptr(), DTYPES[dy.dtype], n, cin, cout, size, dw.data_ptr(), db.data_ptr() if bias else None,
+                                  work.data_ptr(), work.numel(), index, _raw_stream(index)), "ur5_act8_wgrad")
         return dw, db
-
-
-def _planes(shape):
-    """(planes, values per plane): groups never reach over a plane's end. [N, C, ...] has N C planes, a matrix its rows, a vector is one plane."""
-    lead = min(2, len(shape) - 1)
-    planes = size = 1
-    for d in shape[:lead]:
-        planes *= d
-    for d in shape[lead:]:
-        size *= d
-    return planes, size
 
 
 def pack(x):
     """``PackedActivation`` of a tensor of any shape (at least one dimension): per group of 64 neighbouring values of a plane, scale = largest magnitude / 127 and code = the nearest
     integer to value / scale. A group that holds an infinity or a NaN is restored as NaN throughout, one below 1e-30 as zeros."""
     _float_gpu(x, "x")
-    if x.dim() < 1:
+    shape = x.shape
+    if not shape:
         raise ValueError("a scalar has no activations to pack")
-    planes, size = _planes(x.shape)
+    count = x.numel()
+    planes = _planes(shape)
+    size = count // planes if planes else 0
     groups = -(-size // GROUP)
     codes = torch.empty((planes, groups, GROUP), dtype=torch.int8, device=x.device)
     scales = torch.empty((planes, groups), dtype=torch.float32, device=x.device)
-    if x.numel():
-        lib, src = native.load(), x.detach().contiguous()
-        native.check(lib, lib.ur5_act8_pack(src.data_ptr(), DTYPES[x.dtype], planes, size, codes.data_ptr(), scales.data_ptr(), x.device.index, _stream(x)), "ur5_act8_pack")
-    return PackedActivation(codes, scales, x.shape, x.dtype)
+    if count:
+        src, index = x.contiguous(), x.get_device()
+        _check(_library().ur5_act8_pack(src.data_ptr(), DTYPES[x.dtype], planes, size, codes.data_ptr(), scales.data_ptr(), index, _raw_stream(index)), "ur5_act8_pack")
+    return PackedActivation(codes, scales, shape, x.dtype)
 
 
 class _PointwiseConv(torch.autograd.Function):

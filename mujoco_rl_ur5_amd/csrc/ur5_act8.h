@@ -5,7 +5,7 @@
 
 namespace ur5act8 {
 using ur5policy::load8; using ur5policy::store8; using ur5policy::widen; using ur5policy::narrow; using ur5policy::lanes_sum;
-using ur5policy::f32_t; using ur5policy::f16_t; using ur5policy::bf16_t;
+using ur5policy::f32_t; using ur5policy::f16_t; using ur5policy::bf16_t; using ur5policy::yes; using ur5policy::no;
 
 constexpr int GROUP = 64, THREADS = 256, LANES = 8;   // 8 lanes of 8 neighbouring values per group
 constexpr float ZERO_BELOW = 1e-30f;
@@ -59,9 +59,12 @@ template <typename T> __global__ void __launch_bounds__(THREADS) ur5_act8_unpack
 // Codes are small integers, exact in 16-bit floats, and a group's scale is a factor of 64 pixels of one input channel: v_mfma_f32_32x32x16 runs over the 64 pixels on
 // plain codes, and its 32 x 32 result is multiplied by the scales once -- a lane holds one column (one input channel) of it, so the scale is one register.
 // fp32 gradients go in as three bf16 terms whose sum is the value exactly (8 + 8 + 8 bits, cut off, not rounded), 16-bit gradients as they are.
-// A wavefront owns 64 output x TC input channels of a range of groups and loads its operands straight into the instruction's lane layout: lane l holds channel l % 32
-// and pixels 32 (l / 32) .. + 31 of the group (the order of the pixels is free as long as both operands agree). Four wavefronts split a workgroup's range and add up
-// through LDS; workgroups split the pixels `splits` ways and ur5_act8_wgrad_sum adds their parts in order: no atomics, the same result every time.
+// A workgroup owns TO output x TC input channels of a range of groups; its WO x WC wavefronts own A x B results of 32 x 32 each. Per group, its threads read the TO x 64
+// gradients in whole rows (256 bytes), cut them into terms and put them into LDS in the instruction's order -- 8 pixels of a channel are 16 bytes, channels next to each
+// other, so that writes and reads of 16 bytes are free of bank conflicts --, once instead of once per wavefront. Codes go straight from memory into the lanes that need
+// them: lane l holds channel l % 32 and pixels 32 (l / 32) .. + 31 of the group (the order of the pixels is free as long as both operands agree). Two buffers in LDS: while
+// the matrix instructions run over group g, group g + 1 is cut into the other buffer and group g + 2 is on its way; one barrier per group.
+// Ranges are `splits` in number, and ur5_act8_wgrad_sum adds their parts in order: no atomics, the same result every time.
 typedef float F16 __attribute__((ext_vector_type(16)));
 typedef __bf16 B8 __attribute__((ext_vector_type(8)));
 typedef _Float16 H8 __attribute__((ext_vector_type(8)));
@@ -71,12 +74,12 @@ __device__ __forceinline__ F16 mfma(f16_t, U4a a, U4a b, F16 c) { return __built
 template <typename T> struct Terms { static constexpr int N = 1; using kind = T; };
 template <> struct Terms<f32_t> { static constexpr int N = 3; using kind = bf16_t; };
 
-// 32 gradients of a lane as they come from memory
-template <typename T> struct Raw { uint32_t w[16]; };
-template <> struct Raw<f32_t> { uint32_t w[32]; };
-// first: the row's 32 values; left: how many of them lie inside the plane
+// 8 neighbouring gradients of a thread as they come from memory
+template <typename T> struct Raw { uint32_t w[4]; };
+template <> struct Raw<f32_t> { uint32_t w[8]; };
+// first: where the 8 lie; left: how many of them lie inside the plane
 template <typename T> __device__ __forceinline__ void fetch(Raw<T>& r, const typename T::raw* first, int left, bool whole) {
-  constexpr int PER = 4 / sizeof(typename T::raw), WORDS = 32 / PER;
+  constexpr int PER = 4 / sizeof(typename T::raw), WORDS = 8 / PER;
   if (whole) {
 #pragma unroll
     for (int i = 0; i < WORDS; i += 4) {
@@ -93,15 +96,15 @@ template <typename T> __device__ __forceinline__ void fetch(Raw<T>& r, const typ
   }
 }
 __device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302); }   // {a's high half, b's high half}
-// matrix operand of pixels 8 step .. 8 step + 7, and what it adds to the bias
-__device__ __forceinline__ float operand(const Raw<f32_t>& r, int step, U4a* term) {
+// the terms of 8 gradients, and what they add to the bias
+__device__ __forceinline__ float cut(const Raw<f32_t>& r, U4a* term) {
   float sum = 0;
 #pragma unroll
   for (int i = 0; i < 4; i++) {
     uint32_t part[3][2];
 #pragma unroll
     for (int k = 0; k < 2; k++) {
-      float v = __uint_as_float(r.w[8 * step + 2 * i + k]);
+      float v = __uint_as_float(r.w[2 * i + k]);
       sum += v;
 #pragma unroll
       for (int n = 0; n < 3; n++) {
@@ -114,25 +117,25 @@ __device__ __forceinline__ float operand(const Raw<f32_t>& r, int step, U4a* ter
   }
   return sum;
 }
-template <typename T> __device__ __forceinline__ float operand(const Raw<T>& r, int step, U4a* term) {
+template <typename T> __device__ __forceinline__ float cut(const Raw<T>& r, U4a* term) {
   float sum = 0;
 #pragma unroll
   for (int i = 0; i < 4; i++) {
-    const uint32_t w = r.w[4 * step + i];
-    term[0][i] = w;
-    sum += widen(T{}, (uint16_t)w) + widen(T{}, (uint16_t)(w >> 16));
+    term[0][i] = r.w[i];
+    sum += widen(T{}, (uint16_t)r.w[i]) + widen(T{}, (uint16_t)(r.w[i] >> 16));
   }
   return sum;
 }
-// 8 codes as 16-bit floats
+// 8 codes as 16-bit floats (a bf16 is the high half of the fp32 that holds so small an integer)
+__device__ __forceinline__ uint32_t pair(bf16_t, float a, float b) { return high_halves(__float_as_uint(a), __float_as_uint(b)); }
+__device__ __forceinline__ uint32_t pair(f16_t, float a, float b) { return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b)); }
 template <typename K> __device__ __forceinline__ U4a code_operand(uint32_t lo, uint32_t hi) {
   U4a out;
 #pragma unroll
   for (int i = 0; i < 4; i++) {
     const uint32_t w = i < 2 ? lo : hi;
     const int sh = 16 * (i & 1);
-    const float a = (float)(int8_t)(w >> sh), b = (float)(int8_t)(w >> (sh + 8));
-    out[i] = (uint32_t)narrow(K{}, a) | (uint32_t)narrow(K{}, b) << 16;
+    out[i] = pair(K{}, (float)(int8_t)(w >> sh), (float)(int8_t)(w >> (sh + 8)));
   }
   return out;
 }
@@ -140,105 +143,167 @@ template <typename K> __device__ __forceinline__ U4a code_operand(uint32_t lo, u
 struct Wgrad {
   const int8_t* codes; const float* scales; const void* dy;
   long long size; int groups, n, cin, cout, splits, o_tiles, c_tiles;
-  float* part; float* part_bias;      // [splits][cout][cin], [splits][4][cout]
+  float* part; float* part_bias;      // [splits][cout][cin], [splits][cout]
 };
-constexpr int TO = 64;
-template <typename T, int TC> __global__ void __launch_bounds__(THREADS, 1) ur5_act8_wgrad(Wgrad W) {
+// Groups that a plane fills come first; the planes' last, shorter groups are a second, plain loop.
+template <typename T, int A, int B, int WO, int WC> __global__ void __launch_bounds__(64 * WO * WC, 2) ur5_act8_wgrad(Wgrad W) {
   using K = typename Terms<T>::kind;
-  constexpr int N = Terms<T>::N, A = TO / 32, B = TC / 32;
-  // workgroups of one pixel range sit on one XCD and run together: they share the range's gradients and codes in its L2
+  using R = typename T::raw;
+  constexpr int N = Terms<T>::N, TO = 32 * A * WO, TC = 32 * B * WC, COUNT = 64 * WO * WC, ROWS = TO * 8 / COUNT;
+  __shared__ U4a shared[2][N][8][TO + 1];                                // [buffer][term][8 pixels][output channel]
+  // workgroups of one range sit on one XCD and run together: they share the range's gradients and codes in its L2
   const int tiles = W.o_tiles * W.c_tiles, b = blockIdx.x;
   const int split = (b & 7) + 8 * ((b >> 3) / tiles), tile = (b >> 3) % tiles;
-  if (split >= W.splits) return;
   const int o0 = tile / W.c_tiles * TO, c0 = tile % W.c_tiles * TC;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, half = lane >> 5;
-  const long long all = (long long)W.n * W.groups, ranges = 4ll * W.splits;
-  long long g = all * (4 * split + wave) / ranges;
-  const long long end = all * (4 * split + wave + 1) / ranges;
+  const int wave_o = wave / WC * 32 * A, wave_c = wave % WC * 32 * B;
+  const bool with_bias = W.part_bias && c0 == 0;
+
+  // this thread's share of the gradients: 8 pixels of ROWS rows; channels behind the last: its values again, their results are not kept
+  const int eight = threadIdx.x & 7, row = threadIdx.x >> 3;
+  const R* dy[ROWS];
+#pragma unroll
+  for (int i = 0; i < ROWS; i++) dy[i] = (const R*)W.dy + min(o0 + row + COUNT / 8 * i, W.cout - 1) * W.size + 8 * eight;
+  long long group[B];
+#pragma unroll
+  for (int k = 0; k < B; k++) group[k] = (long long)min(c0 + wave_c + 32 * k + col, W.cin - 1) * W.groups;
+
   F16 acc[A][B] = {};
-  float bias[A] = {};
-  int image = (int)(g / W.groups), at = (int)(g % W.groups);
-  for (; g < end; g++) {
-    Raw<T> raw[A];
-    const bool whole = (at + 1) * (long long)GROUP <= W.size;
-    const long long pixel = (long long)at * GROUP + 32 * half;
-    const int left = (int)min(32ll, max(0ll, W.size - pixel));
+  float bias[ROWS] = {};
+  struct Place { int image, at; };
+  const auto cut_rows = [&](const Raw<T>* raw, int buffer, bool counts) {
 #pragma unroll
-    for (int a = 0; a < A; a++) {
-      const int o = min(o0 + 32 * a + col, W.cout - 1);                  // channels behind the last: its values again, their results are not kept
-      fetch<T>(raw[a], (const typename T::raw*)W.dy + ((long long)image * W.cout + o) * W.size + pixel, left, whole);
+    for (int i = 0; i < ROWS; i++) {
+      U4a term[N];
+      const float v = cut(raw[i], term);
+      bias[i] += counts ? v : 0.f;
+#pragma unroll
+      for (int n = 0; n < N; n++) shared[buffer][n][eight][row + COUNT / 8 * i] = term[n];
     }
-    uint32_t code[B][8];
-    float scale[B];
+  };
+  const auto fetch_rows = [&](const Place& p, Raw<T>* raw) {
+    const long long plane = (long long)p.image * W.cout * W.size + (long long)p.at * GROUP;
+#pragma unroll
+    for (int i = 0; i < ROWS; i++) fetch<T>(raw[i], dy[i] + plane, 8, true);
+  };
+  struct Codes { U4a lo[B], hi[B]; float scale[B]; };
+  const auto fetch_codes = [&](const Place& p, Codes& c) {
+    const long long first = (long long)p.image * W.cin * W.groups + p.at;
 #pragma unroll
     for (int k = 0; k < B; k++) {
-      const int c = min(c0 + 32 * k + col, W.cin - 1);
-      const long long group = ((long long)image * W.cin + c) * W.groups + at;
-      const U4a* p = (const U4a*)(W.codes + group * GROUP + 32 * half);
-      const U4a u = p[0], v = p[1];
-#pragma unroll
-      for (int i = 0; i < 4; i++) { code[k][i] = u[i]; code[k][4 + i] = v[i]; }
-      scale[k] = W.scales[group];
+      const U4a* at = (const U4a*)(W.codes + (first + group[k]) * GROUP + 32 * half);
+      c.lo[k] = at[0]; c.hi[k] = at[1];
+      c.scale[k] = W.scales[first + group[k]];
     }
-    U4a term[A][4][N];
+  };
+  const auto multiply = [&](int buffer, const Codes& c) {
+    F16 sum[A][B] = {};
 #pragma unroll
-    for (int a = 0; a < A; a++)
-#pragma unroll
-      for (int s = 0; s < 4; s++) bias[a] += operand(raw[a], s, term[a][s]);
-#pragma unroll
-    for (int k = 0; k < B; k++) {
-      F16 sum[A] = {};
-#pragma unroll
-      for (int s = 0; s < 4; s++) {
-        const U4a x = code_operand<K>(code[k][2 * s], code[k][2 * s + 1]);
-#pragma unroll
-        for (int n = N - 1; n >= 0; n--)
-#pragma unroll
-          for (int a = 0; a < A; a++) sum[a] = mfma(K{}, term[a][s][n], x, sum[a]);
-      }
+    for (int q = 0; q < 4; q++) {
+      U4a term[A][N], v[B];
 #pragma unroll
       for (int a = 0; a < A; a++)
 #pragma unroll
-        for (int i = 0; i < 16; i++) acc[a][k][i] = fmaf(scale[k], sum[a][i], acc[a][k][i]);
+        for (int n = 0; n < N; n++) term[a][n] = shared[buffer][n][4 * half + q][wave_o + 32 * a + col];
+#pragma unroll
+      for (int k = 0; k < B; k++) {
+        const U4a& w = q < 2 ? c.lo[k] : c.hi[k];
+        v[k] = code_operand<K>(w[2 * (q & 1)], w[2 * (q & 1) + 1]);
+      }
+#pragma unroll
+      for (int n = N - 1; n >= 0; n--)
+#pragma unroll
+        for (int a = 0; a < A; a++)
+#pragma unroll
+          for (int k = 0; k < B; k++) sum[a][k] = mfma(K{}, term[a][n], v[k], sum[a][k]);
     }
-    if (++at == W.groups) { at = 0; image++; }
+#pragma unroll
+    for (int a = 0; a < A; a++)
+#pragma unroll
+      for (int k = 0; k < B; k++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) acc[a][k][i] = fmaf(c.scale[k], sum[a][k][i], acc[a][k][i]);
+  };
+
+  const int wholes = (int)(W.size / GROUP);
+  const long long all = (long long)W.n * wholes, first = all * split / W.splits, last = all * (split + 1) / W.splits;
+  if (first < last) {
+    const auto next = [&](Place& p, long long g) {                       // the group after p, or p again at the range's end (a load too many, of something that is there)
+      if (g + 1 < last && ++p.at == wholes) { p.at = 0; p.image++; }
+    };
+    Place ahead{(int)(first / wholes), (int)(first % wholes)}, now = ahead;
+    Raw<T> raw[ROWS];
+    Codes codes[2];
+    fetch_rows(ahead, raw);
+    fetch_codes(now, codes[0]);
+    cut_rows(raw, 0, true);
+    next(ahead, first);
+    fetch_rows(ahead, raw);
+    const auto step = [&](long long g, auto odd) {
+      constexpr int me = decltype(odd)::value ? 1 : 0;
+      __syncthreads();                                                   // group g is in its buffer, and everybody has read the other one
+      next(now, g);
+      fetch_codes(now, codes[me ^ 1]);
+      cut_rows(raw, me ^ 1, g + 1 < last);                               // (behind the last group: once more, not counted)
+      next(ahead, g + 1);
+      fetch_rows(ahead, raw);
+      multiply(me, codes[me]);
+    };
+    for (long long g = first; g < last; g += 2) {                        // by twos: what is on its way lands in registers of its own, nothing is moved (a move would wait for it)
+      step(g, no{});
+      if (g + 1 < last) step(g + 1, yes{});
+    }
   }
-  // the four wavefronts' tiles, 32 x 32 at a time
-  __shared__ float block[4][32][33];
+  if (W.size % GROUP) {                                                  // the planes' last groups
+    const int left = (int)min(8, max(0, (int)(W.size % GROUP) - 8 * eight));
+    for (Place p{(int)((long long)W.n * split / W.splits), wholes}; p.image < (int)((long long)W.n * (split + 1) / W.splits); p.image++) {
+      Raw<T> raw[ROWS];
+      Codes codes;
+      const long long plane = (long long)p.image * W.cout * W.size + (long long)p.at * GROUP;
+#pragma unroll
+      for (int i = 0; i < ROWS; i++) fetch<T>(raw[i], dy[i] + plane, left, false);
+      fetch_codes(p, codes);
+      __syncthreads();
+      cut_rows(raw, 0, true);
+      __syncthreads();
+      multiply(0, codes);
+    }
+  }
 #pragma unroll
   for (int a = 0; a < A; a++)
 #pragma unroll
-    for (int k = 0; k < B; k++) {
-      __syncthreads();
+    for (int k = 0; k < B; k++)
 #pragma unroll
-      for (int i = 0; i < 16; i++) block[wave][(i & 3) + 8 * (i >> 2) + 4 * half][col] = acc[a][k][i];
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const int r = (threadIdx.x >> 5) + 8 * i, c = threadIdx.x & 31, o = o0 + 32 * a + r, ci = c0 + 32 * k + c;
-        if (o < W.cout && ci < W.cin) W.part[((size_t)split * W.cout + o) * W.cin + ci] = block[0][r][c] + block[1][r][c] + block[2][r][c] + block[3][r][c];
+      for (int i = 0; i < 16; i++) {
+        const int o = o0 + wave_o + 32 * a + (i & 3) + 8 * (i >> 2) + 4 * half, c = c0 + wave_c + 32 * k + col;
+        if (o < W.cout && c < W.cin) W.part[((size_t)split * W.cout + o) * W.cin + c] = acc[a][k][i];
       }
-    }
-  if (W.part_bias && c0 == 0) {
+  if (with_bias) {
 #pragma unroll
-    for (int a = 0; a < A; a++) {
-      const float v = bias[a] + __shfl_xor(bias[a], 32);
-      const int o = o0 + 32 * a + col;
-      if (half == 0 && o < W.cout) W.part_bias[((size_t)split * 4 + wave) * W.cout + o] = v;
+    for (int i = 0; i < ROWS; i++) {
+      float v = bias[i];
+      for (int o = 4; o; o >>= 1) v += __shfl_xor(v, o);
+      const int o = o0 + row + COUNT / 8 * i;
+      if (eight == 0 && o < W.cout) W.part_bias[(size_t)split * W.cout + o] = v;
     }
   }
 }
-// parts in order, in 64 bits
+// parts in order, in 64 bits: 32 outputs per workgroup, eight threads each (few outputs and many parts want many loads at once: 128 parts of 8192 weights 120 us with one thread each)
 __global__ void __launch_bounds__(THREADS) ur5_act8_wgrad_sum(const float* part, const float* part_bias, int splits, int weights, int cout, float* dw, float* db) {
-  const int i = blockIdx.x * THREADS + threadIdx.x;
-  if (i < weights) {
-    double s = 0;
-    for (int k = 0; k < splits; k++) s += part[(size_t)k * weights + i];
-    dw[i] = (float)s;
-  } else if (db && i - weights < cout) {
-    double s = 0;
-    for (int k = 0; k < 4 * splits; k++) s += part_bias[(size_t)k * cout + i - weights];
-    db[i - weights] = (float)s;
-  }
+  const int i = blockIdx.x * 32 + (threadIdx.x & 31), share = threadIdx.x >> 5;
+  const bool is_weight = i < weights, is_bias = !is_weight && db && i - weights < cout;
+  const float* p = is_weight ? part + i : part_bias + (i - weights);
+  const size_t step = is_weight ? weights : cout;
+  double s = 0;
+  if (is_weight || is_bias)
+#pragma unroll 4
+    for (int k = share; k < splits; k += 8) s += p[k * step];
+  __shared__ double sums[8][32];
+  sums[share][threadIdx.x & 31] = s;
+  __syncthreads();
+  if (share) return;
+  for (int k = 1; k < 8; k++) s += sums[k][threadIdx.x];
+  if (is_weight) dw[i] = (float)s;
+  else if (is_bias) db[i - weights] = (float)s;
 }
 }  // namespace ur5act8

@@ -271,19 +271,19 @@ int ur5_act8_unpack(const int8_t* codes, const float* scales, int64_t planes, in
   return launched(__func__);
 }
 
-// ---- weight gradient: how the pixels are split. A wavefront of the kernel fills a SIMD's registers, so 256 workgroups fill the card; a multiple of 8 ranges, one set per XCD.
-struct WgradPlan { int o_tiles, c_tiles, wide, splits; int64_t part, bytes; };
+// ---- weight gradient: how the work is split. Tiles of 128 output x 256 input channels (of half the outputs, and of half or a quarter of the inputs where there are no more),
+// and as many ranges of the pixels as give every CU a workgroup (two of the smaller ones), a multiple of 8: one set per XCD.
+constexpr int64_t WORKGROUPS = 256;
+struct WgradPlan { int to, tc, o_tiles, c_tiles, splits; int64_t part, bytes; };
 static WgradPlan wgrad_plan(int64_t n, int64_t cin, int64_t cout, int64_t size) {
   WgradPlan p;
-  p.wide = cin > 64;                                    // 128 input channels per tile, or 64 where there are no more
-  p.o_tiles = (int)((cout + ur5act8::TO - 1) / ur5act8::TO);
-  p.c_tiles = (int)((cin + (p.wide ? 127 : 63)) / (p.wide ? 128 : 64));
+  p.to = cout > 64 ? 128 : 64; p.tc = cin > 128 ? 256 : cin > 64 ? 128 : 64;
+  p.o_tiles = (int)((cout + p.to - 1) / p.to); p.c_tiles = (int)((cin + p.tc - 1) / p.tc);
   const int64_t groups = n * ((size + ur5act8::GROUP - 1) / ur5act8::GROUP), tiles = (int64_t)p.o_tiles * p.c_tiles;
-  int64_t s = (256 + tiles - 1) / tiles;
-  if (s > (groups + 3) / 4) s = (groups + 3) / 4;       // a range of at least one group for every wavefront
+  const int64_t s = clamp((WORKGROUPS * (p.to == 64 ? 2 : 1) + tiles - 1) / tiles, 1, groups > 0 ? groups : 1);
   p.splits = (int)((s + 7) / 8 * 8);
   p.part = ((int64_t)p.splits * cin * cout * 4 + 15) / 16 * 16;
-  p.bytes = p.part + (int64_t)p.splits * 4 * cout * 4;
+  p.bytes = p.part + (int64_t)p.splits * cout * 4;
   return p;
 }
 static const char* check_wgrad(int64_t n, int64_t cin, int64_t cout, int64_t size) {
@@ -307,11 +307,12 @@ int ur5_act8_wgrad(const int8_t* codes, const float* scales, const void* dy, int
   by_type(dtype, [&](auto t) {
     using T = decltype(t);
     const int grid = p.splits * p.o_tiles * p.c_tiles;
-    if (p.wide) ur5act8::ur5_act8_wgrad<T, 128><<<grid, ur5act8::THREADS, 0, s>>>(W);
-    else ur5act8::ur5_act8_wgrad<T, 64><<<grid, ur5act8::THREADS, 0, s>>>(W);
+    const auto run = [&](auto kernel, int threads) { kernel<<<grid, threads, 0, s>>>(W); };
+    if (p.to == 128) p.tc == 256 ? run(ur5act8::ur5_act8_wgrad<T, 2, 2, 2, 4>, 512) : p.tc == 128 ? run(ur5act8::ur5_act8_wgrad<T, 1, 2, 4, 2>, 512) : run(ur5act8::ur5_act8_wgrad<T, 1, 1, 4, 2>, 512);
+    else p.tc == 256 ? run(ur5act8::ur5_act8_wgrad<T, 1, 2, 2, 4>, 512) : p.tc == 128 ? run(ur5act8::ur5_act8_wgrad<T, 1, 1, 2, 4>, 512) : run(ur5act8::ur5_act8_wgrad<T, 1, 1, 2, 2>, 256);
   });
   const int weights = (int)(cin * cout), outs = weights + (db ? (int)cout : 0);
-  ur5act8::ur5_act8_wgrad_sum<<<(outs + ur5act8::THREADS - 1) / ur5act8::THREADS, ur5act8::THREADS, 0, s>>>(part, part_bias, p.splits, weights, (int)cout, dw, db);
+  ur5act8::ur5_act8_wgrad_sum<<<(outs + 31) / 32, ur5act8::THREADS, 0, s>>>(part, part_bias, p.splits, weights, (int)cout, dw, db);
   return launched(__func__);
 }
 }

@@ -114,16 +114,16 @@ def load(path=None):
     L.ur5_render.argtypes = [vp, C.c_int, C.c_int, C.c_int, C.c_int, C.POINTER(C.c_uint8), C.POINTER(C.c_float)]
     L.ur5_render_dev.argtypes = [vp, C.c_int, C.c_int, C.c_int, C.c_int, vp, vp]
     if hasattr(L, "ur5_policy_sample"):                        # the engine's host builds (tests) hold no learning operators
-        i64, i32, rows = C.c_int64, C.c_int, C.POINTER(Rows)
+        i64, i32, rows = C.c_int64, C.c_int, vp                   # structs go in by reference (byref of Rows, Clip, Prefer) or as their packed bytes
         L.ur5_policy_work_bytes.argtypes, L.ur5_policy_work_bytes.restype = [i64] * 4, i64
         L.ur5_policy_sample.argtypes = [rows, C.c_uint64, vp, vp, vp]
         L.ur5_policy_logp.argtypes = [rows, vp, vp, vp]
-        L.ur5_policy_clip_loss.argtypes = [rows, C.POINTER(Clip), vp, vp, vp, vp]
-        L.ur5_policy_clip_grad.argtypes = [rows, C.POINTER(Clip), vp]
-        L.ur5_policy_clip_loss_grad.argtypes = [rows, C.POINTER(Clip), vp, vp, vp, vp, vp]
-        L.ur5_policy_prefer_loss.argtypes = [rows, C.POINTER(Prefer), vp, vp]
-        L.ur5_policy_prefer_grad.argtypes = [rows, C.POINTER(Prefer), vp]
-        L.ur5_policy_prefer_loss_grad.argtypes = [rows, C.POINTER(Prefer), vp, vp, vp]
+        L.ur5_policy_clip_loss.argtypes = [rows, vp, vp, vp, vp, vp]
+        L.ur5_policy_clip_grad.argtypes = [rows, vp, vp]
+        L.ur5_policy_clip_loss_grad.argtypes = [rows, vp, vp, vp, vp, vp, vp]
+        L.ur5_policy_prefer_loss.argtypes = [rows, vp, vp, vp]
+        L.ur5_policy_prefer_grad.argtypes = [rows, vp, vp]
+        L.ur5_policy_prefer_loss_grad.argtypes = [rows, vp, vp, vp, vp]
         L.ur5_act8_pack.argtypes = [vp, i32, i64, i64, vp, vp, i32, vp]
         L.ur5_act8_unpack.argtypes = [vp, vp, i64, i64, vp, i32, i32, vp]
         L.ur5_act8_wgrad_work_bytes.argtypes, L.ur5_act8_wgrad_work_bytes.restype = [i64] * 4, i64

@@ -14,7 +14,7 @@ Everything is queued on the current stream of the logits' device and can be capt
 """
 from __future__ import annotations
 
-import ctypes as C
+import struct
 from collections import namedtuple
 
 import torch
@@ -27,19 +27,23 @@ SAMPLE_STREAM = 6                     # random stream of the sampled actions (sh
 PolicyLoss = namedtuple("PolicyLoss", "loss logp kl entropy")
 PreferenceLoss = namedtuple("PreferenceLoss", "loss margin")
 
+# A call on a small batch takes as long as its Python: argument structs are packed bytes (native.Rows, Clip and Prefer spell them out), tensors that need no copy are not
+# touched, and the current stream is asked for by its handle.
+_ROWS, _CLIP, _PREFER = struct.Struct("@PPPqqqqqqiiPPq"), struct.Struct("@PPPfffffP"), struct.Struct("@PPPqddfP")
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+_handle = None
 
-def _flat(t, what):
-    """[N, ...] as [N, A] with neighbouring elements, without a copy where the rows allow it."""
-    n = t.shape[0]
-    width = 1
-    for d in t.shape[1:]:
-        width *= d
-    if width == 0:
-        raise ValueError(f"{what} has no actions: {tuple(t.shape)}")
-    if t.is_contiguous():
-        return t.view(n, width)
-    t = t.reshape(n, width)
-    return t if t.stride(1) == 1 and (n <= 1 or t.stride(0) >= width) or width == 1 and (n <= 1 or t.stride(0) >= 1) else t.contiguous()
+
+def _library():
+    global _handle
+    if _handle is None:
+        _handle = native.load()
+    return _handle
+
+
+def _check(rc, what):
+    if rc:
+        native.check(_library(), rc, what)
 
 
 def _gpu(t, what):
@@ -49,11 +53,42 @@ def _gpu(t, what):
         raise ValueError(f"{what} is on {t.device}: the policy operators run on the GPU, there is no CPU fallback")
 
 
-def _vector(t, n, dtype, device, what):
+class _Flat:
+    """Rows of a tensor [N, ...]: n rows of `width` neighbouring elements, `stride` apart. `tensor` keeps the memory (a copy where the rows are not contiguous)."""
+    __slots__ = ("tensor", "n", "width", "stride")
+
+    def __init__(self, t, what):
+        self.n = n = t.shape[0]
+        if n:
+            self.width = width = t.numel() // n
+        else:
+            self.width = width = 1
+            for d in t.shape[1:]:
+                width *= d
+            self.width = width
+        if width == 0:
+            raise ValueError(f"{what} has no actions: {tuple(t.shape)}")
+        self.stride = width
+        if not t.is_contiguous():
+            t = t.reshape(n, width)
+            if (width > 1 and t.stride(1) != 1) or (n > 1 and t.stride(0) < width):
+                t = t.contiguous()
+            self.stride = t.stride(0) if n > 1 else width
+        self.tensor = t
+
+    def matrix(self):
+        """The rows as a two-dimensional tensor without a history."""
+        t = self.tensor.detach()
+        return t if t.dim() == 2 else t.view(self.n, self.width)
+
+
+def _vector(t, n, dtype, index, what):
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{what} must be a tensor")
-    if t.shape != (n,) or t.device != device:
-        raise ValueError(f"{what} must be a [{n}] tensor on {device}, not {tuple(t.shape)} on {t.device}")
+    if t.dim() != 1 or t.shape[0] != n or not t.is_cuda or t.get_device() != index:
+        raise ValueError(f"{what} must be a [{n}] tensor on cuda:{index}, not {tuple(t.shape)} on {t.device}")
+    if t.dtype is dtype and t.is_contiguous():
+        return t
     if t.dtype.is_floating_point != dtype.is_floating_point or t.dtype == torch.bool:
         raise TypeError(f"{what} must hold {dtype}, not {t.dtype}")
     return t.detach().to(dtype).contiguous()
@@ -65,20 +100,20 @@ def _logits(logits, what="logits"):
         raise TypeError(f"{what} must be float32, float16 or bfloat16, not {logits.dtype}")
     if logits.dim() < 2:
         raise ValueError(f"{what} must be [N, ...], not {tuple(logits.shape)}")
-    return _flat(logits.detach(), what)
+    return _Flat(logits, what)
 
 
 def _mask(mask, z):
     if mask is None:
         return None
     _gpu(mask, "mask")
-    if mask.dtype not in (torch.bool, torch.uint8):
+    if mask.dtype is not torch.bool and mask.dtype is not torch.uint8:
         raise TypeError(f"mask must be bool or uint8, not {mask.dtype}")
-    if mask.device != z.device or mask.dim() < 2 or mask.shape[0] not in (1, z.shape[0]):
-        raise ValueError(f"mask must be [{z.shape[0]} or 1, ...] on {z.device}, not {tuple(mask.shape)} on {mask.device}")
-    m = _flat(mask, "mask")
-    if z.shape[1] % m.shape[1]:
-        raise ValueError(f"a mask of {m.shape[1]} pixels does not divide {z.shape[1]} actions")
+    if mask.get_device() != z.tensor.get_device() or mask.dim() < 2 or mask.shape[0] not in (1, z.n):
+        raise ValueError(f"mask must be [{z.n} or 1, ...] on {z.tensor.device}, not {tuple(mask.shape)} on {mask.device}")
+    m = _Flat(mask, "mask")
+    if z.width % m.width:
+        raise ValueError(f"a mask of {m.width} pixels does not divide {z.width} actions")
     return m
 
 
@@ -86,22 +121,22 @@ def _reference(ref, z, shape):
     if ref is None:
         return None
     q = _logits(ref, "ref_logits")
-    if ref.shape != shape or q.dtype != z.dtype or q.device != z.device:
-        raise ValueError(f"ref_logits must be {tuple(shape)} {z.dtype} on {z.device} like the logits, not {tuple(ref.shape)} {q.dtype} on {q.device}")
+    if ref.shape != shape or ref.dtype != z.tensor.dtype or ref.get_device() != z.tensor.get_device():
+        raise ValueError(f"ref_logits must be {tuple(shape)} {z.tensor.dtype} on {z.tensor.device} like the logits, not {tuple(ref.shape)} {ref.dtype} on {ref.device}")
     return q
 
 
-def _work(lib, z, mask, pairs=0):
-    return torch.empty(lib.ur5_policy_work_bytes(z.shape[0], z.shape[1], mask.shape[1] if mask is not None else 0, pairs), dtype=torch.uint8, device=z.device)
+def _work(z, mask, pairs=0):
+    return torch.empty(_library().ur5_policy_work_bytes(z.n, z.width, 0 if mask is None else mask.width, pairs), dtype=torch.uint8, device=z.tensor.device)
 
 
 def _rows(z, mask, ref, work):
-    """The C view of checked tensors (kept alive by the caller)."""
-    n, a = z.shape
-    return native.Rows(z.data_ptr(), ref.data_ptr() if ref is not None else None, mask.data_ptr() if mask is not None else None,
-                       z.stride(0), ref.stride(0) if ref is not None else 0, mask.stride(0) if mask is not None and mask.shape[0] > 1 else 0,
-                       n, a, mask.shape[1] if mask is not None else 0, DTYPES[z.dtype], z.device.index, torch.cuda.current_stream(z.device).cuda_stream,
-                       work.data_ptr(), work.numel())
+    """ur5_rows of checked tensors (kept alive by the caller)."""
+    t = z.tensor
+    index = t.get_device()
+    return _ROWS.pack(t.data_ptr(), 0 if ref is None else ref.tensor.data_ptr(), 0 if mask is None else mask.tensor.data_ptr(), z.stride, 0 if ref is None else ref.stride,
+                      0 if mask is None or mask.n == 1 else mask.stride, z.n, z.width, 0 if mask is None else mask.width, DTYPES[t.dtype], index, _raw_stream(index),
+                      work.data_ptr(), work.numel())
 
 
 def sample_actions(logits, seed, gids, round_index, mask=None, stream=SAMPLE_STREAM):
@@ -109,12 +144,13 @@ def sample_actions(logits, seed, gids, round_index, mask=None, stream=SAMPLE_STR
     ``sharding.scene_uniform(seed, gids, round_index, stream, A, dtype=float64)``, evaluated where it is needed: a pure function of the GLOBAL scene ids ``gids`` (int64 [N]), so a
     scene draws the same action however the scenes are sharded or chunked. A row that allows nothing gives (-1, 0)."""
     z = _logits(logits)
-    m, g = _mask(mask, z), _vector(gids, z.shape[0], torch.int64, z.device, "gids")
-    lib = native.load()
-    action = torch.empty(z.shape[0], dtype=torch.int64, device=z.device)
-    logp = torch.empty(z.shape[0], dtype=torch.float32, device=z.device)
-    r = _rows(z, m, None, _w := _work(lib, z, m))
-    native.check(lib, lib.ur5_policy_sample(C.byref(r), sharding.scene_key_offset(seed, round_index, stream), g.data_ptr(), action.data_ptr(), logp.data_ptr()), "ur5_policy_sample")
+    t = z.tensor
+    m, g = _mask(mask, z), _vector(gids, z.n, torch.int64, t.get_device(), "gids")
+    action = torch.empty(z.n, dtype=torch.int64, device=t.device)
+    logp = torch.empty(z.n, dtype=torch.float32, device=t.device)
+    work = _work(z, m)
+    _check(_library().ur5_policy_sample(_rows(z, m, None, work), sharding.scene_key_offset(seed, round_index, stream), g.data_ptr(), action.data_ptr(), logp.data_ptr()),
+           "ur5_policy_sample")
     return action, logp
 
 
@@ -122,62 +158,71 @@ def action_log_probs(logits, action, mask=None):
     """(log-probability of ``action`` (int64 [N]), entropy of the row), float32 [N] each, without a gradient: what a loss needs of the behaviour and reference policies.
     An action outside [0, A) has log-probability 0, one that is not allowed -inf; a row that allows nothing has entropy 0."""
     z = _logits(logits)
-    m, a = _mask(mask, z), _vector(action, z.shape[0], torch.int64, z.device, "action")
-    lib = native.load()
-    out = torch.empty((2, z.shape[0]), dtype=torch.float32, device=z.device)
-    logp, entropy = out[0], out[1]
-    r = _rows(z, m, None, _w := _work(lib, z, m))
-    native.check(lib, lib.ur5_policy_logp(C.byref(r), a.data_ptr(), logp.data_ptr(), entropy.data_ptr()), "ur5_policy_logp")
+    t = z.tensor
+    m, a = _mask(mask, z), _vector(action, z.n, torch.int64, t.get_device(), "action")
+    logp = torch.empty(z.n, dtype=torch.float32, device=t.device)
+    entropy = torch.empty(z.n, dtype=torch.float32, device=t.device)
+    work = _work(z, m)
+    _check(_library().ur5_policy_logp(_rows(z, m, None, work), a.data_ptr(), logp.data_ptr(), entropy.data_ptr()), "ur5_policy_logp")
     return logp, entropy
 
 
 # ------------------------------------------------------------------ clipped policy loss
-def _clip_inputs(logits, action, old_logp, advantage, mask, ref_logits, clip, kl_coef, entropy_coef):
-    z = _logits(logits)
-    n = z.shape[0]
-    low, high = (float(clip[0]), float(clip[1])) if isinstance(clip, (tuple, list)) else (float(clip), float(clip))
-    if kl_coef and ref_logits is None:
-        raise ValueError("kl_coef needs ref_logits")
-    tensors = (z, _vector(action, n, torch.int64, z.device, "action"), _vector(old_logp, n, torch.float32, z.device, "old_logp"),
-               _vector(advantage, n, torch.float32, z.device, "advantage"), _mask(mask, z), _reference(ref_logits, z, logits.shape))
-    return tensors, (low, high, float(kl_coef), float(entropy_coef))
+class _Clip:
+    """Checked arguments of a clipped loss."""
+    __slots__ = ("z", "action", "old", "advantage", "mask", "ref", "numbers")
+
+    def __init__(self, logits, action, old_logp, advantage, mask, ref_logits, clip, kl_coef, entropy_coef):
+        self.z = z = _logits(logits)
+        n, index = z.n, z.tensor.get_device()
+        low, high = (float(clip[0]), float(clip[1])) if isinstance(clip, (tuple, list)) else (float(clip), float(clip))
+        if kl_coef and ref_logits is None:
+            raise ValueError("kl_coef needs ref_logits")
+        self.action = _vector(action, n, torch.int64, index, "action")
+        self.old = _vector(old_logp, n, torch.float32, index, "old_logp")
+        self.advantage = _vector(advantage, n, torch.float32, index, "advantage")
+        self.mask, self.ref = _mask(mask, z), _reference(ref_logits, z, logits.shape)
+        self.numbers = (low, high, float(kl_coef), float(entropy_coef))
+
+    def pack(self, scale=1.0, upstream=0):
+        return _CLIP.pack(self.action.data_ptr(), self.old.data_ptr(), self.advantage.data_ptr(), *self.numbers, scale, upstream)
+
+    def outputs(self):
+        device = self.z.tensor.device
+        return (torch.empty((), dtype=torch.float32, device=device),) + torch.empty((3, self.z.n), dtype=torch.float32, device=device).unbind()
 
 
-def _clip_struct(tensors, numbers, scale=1.0, upstream=None):
-    _, action, old, adv, _, _ = tensors
-    return native.Clip(action.data_ptr(), old.data_ptr(), adv.data_ptr(), *numbers, scale, upstream)
+def _saved(ctx, z, mask, ref, *others):
+    """Keeps what a backward pass reads. Rows go in as matrices: checkpoint8.saved_activations keeps two-dimensional tensors as they are."""
+    ctx.save_for_backward(z.matrix(), mask and mask.matrix(), ref and ref.matrix(), *others)
 
 
-def _clip_outputs(z):
-    out = torch.empty((3, z.shape[0]), dtype=torch.float32, device=z.device)
-    return torch.empty((), dtype=torch.float32, device=z.device), out[0], out[1], out[2]
+def _restored(ctx):
+    """(z, mask, ref, others) as they were."""
+    z, mask, ref, *others = ctx.saved_tensors
+    return _Flat(z, "logits"), None if mask is None else _Flat(mask, "mask"), None if ref is None else _Flat(ref, "ref_logits"), others
 
 
 class _ClippedPolicyLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, tensors, numbers):
-        z, _, _, _, mask, ref = tensors
-        lib = native.load()
-        work = _work(lib, z, mask)
-        terms = _clip_outputs(z)
-        r, c = _rows(z, mask, ref, work), _clip_struct(tensors, numbers)
-        native.check(lib, lib.ur5_policy_clip_loss(C.byref(r), C.byref(c), *(t.data_ptr() for t in terms)), "ur5_policy_clip_loss")
-        ctx.save_for_backward(*tensors, work)                  # (the logits as [N, A]: checkpoint8.saved_activations keeps two-dimensional tensors as they are)
-        ctx.numbers, ctx.shape = numbers, logits.shape
-        ctx.mark_non_differentiable(*terms[1:])
-        return terms
+    def forward(ctx, logits, c):
+        work = _work(c.z, c.mask)
+        loss, logp, kl, entropy = c.outputs()
+        _check(_library().ur5_policy_clip_loss(_rows(c.z, c.mask, c.ref, work), c.pack(), loss.data_ptr(), logp.data_ptr(), kl.data_ptr(), entropy.data_ptr()), "ur5_policy_clip_loss")
+        _saved(ctx, c.z, c.mask, c.ref, c.action, c.old, c.advantage, work)
+        ctx.numbers, ctx.shape = c.numbers, logits.shape
+        ctx.mark_non_differentiable(logp, kl, entropy)
+        return loss, logp, kl, entropy
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, upstream, *_):
-        *tensors, work = ctx.saved_tensors
-        z, _, _, _, mask, ref = tensors
-        lib = native.load()
-        grad = torch.empty(z.shape, dtype=z.dtype, device=z.device)
+        z, mask, ref, (action, old, advantage, work) = _restored(ctx)
+        grad = torch.empty(ctx.shape, dtype=z.tensor.dtype, device=z.tensor.device)
         upstream = upstream.float().contiguous()
-        r, c = _rows(z, mask, ref, work), _clip_struct(tensors, ctx.numbers, 1.0, upstream.data_ptr())
-        native.check(lib, lib.ur5_policy_clip_grad(C.byref(r), C.byref(c), grad.data_ptr()), "ur5_policy_clip_grad")
-        return grad.view(ctx.shape), None, None
+        c = _CLIP.pack(action.data_ptr(), old.data_ptr(), advantage.data_ptr(), *ctx.numbers, 1.0, upstream.data_ptr())
+        _check(_library().ur5_policy_clip_grad(_rows(z, mask, ref, work), c, grad.data_ptr()), "ur5_policy_clip_grad")
+        return grad, None
 
 
 def clipped_policy_loss(logits, action, old_logp, advantage, mask=None, ref_logits=None, clip=0.2, kl_coef=0.0, entropy_coef=0.0):
@@ -188,73 +233,64 @@ def clipped_policy_loss(logits, action, old_logp, advantage, mask=None, ref_logi
     action int64 [N] (-1: the row does not count), old_logp / advantage A float [N] (constants); ``ref_logits`` like the logits: the KL is exact, over all allowed actions (+inf where
     the reference gives probability 0 to an action of positive probability). ``clip``: one number or (low, high). logp, kl, entropy: float32 [N], no gradient, 0 in rows that do not
     count (kl is 0 without ref_logits)."""
-    tensors, numbers = _clip_inputs(logits, action, old_logp, advantage, mask, ref_logits, clip, kl_coef, entropy_coef)
-    return PolicyLoss(*_ClippedPolicyLoss.apply(logits, tensors, numbers))
+    return PolicyLoss(*_ClippedPolicyLoss.apply(logits, _Clip(logits, action, old_logp, advantage, mask, ref_logits, clip, kl_coef, entropy_coef)))
 
 
 def clipped_policy_grad(logits, action, old_logp, advantage, mask=None, ref_logits=None, clip=0.2, kl_coef=0.0, entropy_coef=0.0, grad_scale=1.0):
     """(``PolicyLoss``, its gradient times ``grad_scale`` with respect to the logits, in their shape and type) in three launches, without an autograd graph: for
     ``logits.backward(grad)``. float16 logits want a ``grad_scale``: the entries are about p / N."""
-    tensors, numbers = _clip_inputs(logits, action, old_logp, advantage, mask, ref_logits, clip, kl_coef, entropy_coef)
-    z = tensors[0]
-    lib = native.load()
-    terms = _clip_outputs(z)
-    grad = torch.empty(logits.shape, dtype=z.dtype, device=z.device)
-    r, c = _rows(z, tensors[4], tensors[5], _w := _work(lib, z, tensors[4])), _clip_struct(tensors, numbers, float(grad_scale))
-    native.check(lib, lib.ur5_policy_clip_loss_grad(C.byref(r), C.byref(c), *(t.data_ptr() for t in terms), grad.data_ptr()), "ur5_policy_clip_loss_grad")
-    return PolicyLoss(*terms), grad
+    c = _Clip(logits, action, old_logp, advantage, mask, ref_logits, clip, kl_coef, entropy_coef)
+    loss, logp, kl, entropy = c.outputs()
+    grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    work = _work(c.z, c.mask)
+    _check(_library().ur5_policy_clip_loss_grad(_rows(c.z, c.mask, c.ref, work), c.pack(float(grad_scale)), loss.data_ptr(), logp.data_ptr(), kl.data_ptr(), entropy.data_ptr(),
+                                                grad.data_ptr()), "ur5_policy_clip_loss_grad")
+    return PolicyLoss(loss, logp, kl, entropy), grad
 
 
 # ------------------------------------------------------------------ preference loss
-def _prefer_inputs(logits, action, ref_logp, offsets, mask, beta, label_smoothing):
-    z = _logits(logits)
-    n = z.shape[0]
-    if not isinstance(offsets, torch.Tensor) or offsets.dim() != 1 or offsets.shape[0] < 3 or offsets.shape[0] % 2 == 0:
-        raise ValueError("offsets must be [2 pairs + 1] row numbers of the episodes' ends, with at least one pair")
-    tensors = (z, _vector(action, n, torch.int64, z.device, "action"), _vector(ref_logp, n, torch.float32, z.device, "ref_logp"),
-               _vector(offsets, offsets.shape[0], torch.int64, z.device, "offsets"), _mask(mask, z))
-    return tensors, (float(beta), float(label_smoothing))
+class _Prefer:
+    """Checked arguments of a preference loss."""
+    __slots__ = ("z", "action", "ref_logp", "offsets", "mask", "pairs", "numbers")
 
+    def __init__(self, logits, action, ref_logp, offsets, mask, beta, label_smoothing):
+        self.z = z = _logits(logits)
+        n, index = z.n, z.tensor.get_device()
+        if not isinstance(offsets, torch.Tensor) or offsets.dim() != 1 or offsets.shape[0] < 3 or offsets.shape[0] % 2 == 0:
+            raise ValueError("offsets must be [2 pairs + 1] row numbers of the episodes' ends, with at least one pair")
+        self.action = _vector(action, n, torch.int64, index, "action")
+        self.ref_logp = _vector(ref_logp, n, torch.float32, index, "ref_logp")
+        self.offsets = _vector(offsets, offsets.shape[0], torch.int64, index, "offsets")
+        self.mask, self.pairs, self.numbers = _mask(mask, z), offsets.shape[0] // 2, (float(beta), float(label_smoothing))
 
-def _prefer_struct(tensors, numbers, scale=1.0, upstream=None):
-    _, action, ref_logp, offsets, _ = tensors
-    return native.Prefer(action.data_ptr(), ref_logp.data_ptr(), offsets.data_ptr(), offsets.shape[0] // 2, *numbers, scale, upstream)
+    def pack(self, scale=1.0):
+        return _PREFER.pack(self.action.data_ptr(), self.ref_logp.data_ptr(), self.offsets.data_ptr(), self.pairs, *self.numbers, scale, 0)
 
-
-def _prefer_forward(lib, tensors, numbers, work):
-    z, _, _, offsets, mask = tensors
-    loss = torch.empty((), dtype=torch.float32, device=z.device)
-    margin = torch.empty(offsets.shape[0] // 2, dtype=torch.float32, device=z.device)
-    r, p = _rows(z, mask, None, work), _prefer_struct(tensors, numbers)
-    native.check(lib, lib.ur5_policy_prefer_loss(C.byref(r), C.byref(p), loss.data_ptr(), margin.data_ptr()), "ur5_policy_prefer_loss")
-    return loss, margin
-
-
-def _prefer_backward(lib, tensors, numbers, work, scale, upstream):
-    z, _, _, _, mask = tensors
-    grad = torch.empty(z.shape, dtype=z.dtype, device=z.device)
-    r, p = _rows(z, mask, None, work), _prefer_struct(tensors, numbers, scale, upstream)
-    native.check(lib, lib.ur5_policy_prefer_grad(C.byref(r), C.byref(p), grad.data_ptr()), "ur5_policy_prefer_grad")
-    return grad
+    def outputs(self):
+        device = self.z.tensor.device
+        return torch.empty((), dtype=torch.float32, device=device), torch.empty(self.pairs, dtype=torch.float32, device=device)
 
 
 class _PreferenceLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, tensors, numbers):
-        lib = native.load()
-        work = _work(lib, tensors[0], tensors[4], tensors[3].shape[0] // 2)
-        loss, margin = _prefer_forward(lib, tensors, numbers, work)
-        ctx.save_for_backward(*tensors, work)
-        ctx.numbers, ctx.shape = numbers, logits.shape
+    def forward(ctx, logits, p):
+        work = _work(p.z, p.mask, p.pairs)
+        loss, margin = p.outputs()
+        _check(_library().ur5_policy_prefer_loss(_rows(p.z, p.mask, None, work), p.pack(), loss.data_ptr(), margin.data_ptr()), "ur5_policy_prefer_loss")
+        _saved(ctx, p.z, p.mask, None, p.action, p.ref_logp, p.offsets, work)
+        ctx.numbers, ctx.shape = p.numbers, logits.shape
         ctx.mark_non_differentiable(margin)
         return loss, margin
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, upstream, _):
-        *tensors, work = ctx.saved_tensors
+        z, mask, _, (action, ref_logp, offsets, work) = _restored(ctx)
+        grad = torch.empty(ctx.shape, dtype=z.tensor.dtype, device=z.tensor.device)
         upstream = upstream.float().contiguous()
-        return _prefer_backward(native.load(), tensors, ctx.numbers, work, 1.0, upstream.data_ptr()).view(ctx.shape), None, None
+        p = _PREFER.pack(action.data_ptr(), ref_logp.data_ptr(), offsets.data_ptr(), offsets.shape[0] // 2, *ctx.numbers, 1.0, upstream.data_ptr())
+        _check(_library().ur5_policy_prefer_grad(_rows(z, mask, None, work), p, grad.data_ptr()), "ur5_policy_prefer_grad")
+        return grad, None
 
 
 def preference_loss(logits, action, ref_logp, offsets, mask=None, beta=0.1, label_smoothing=0.0):
@@ -265,18 +301,15 @@ def preference_loss(logits, action, ref_logp, offsets, mask=None, beta=0.1, labe
         margin_i = beta (sum over episode 2 i of (logp - ref_logp) - the same over episode 2 i + 1),    loss = mean_i (1 - eps) softplus(-margin_i) + eps softplus(margin_i)
 
     with eps = ``label_smoothing``. Rows of no episode get a zero gradient."""
-    tensors, numbers = _prefer_inputs(logits, action, ref_logp, offsets, mask, beta, label_smoothing)
-    return PreferenceLoss(*_PreferenceLoss.apply(logits, tensors, numbers))
+    return PreferenceLoss(*_PreferenceLoss.apply(logits, _Prefer(logits, action, ref_logp, offsets, mask, beta, label_smoothing)))
 
 
 def preference_grad(logits, action, ref_logp, offsets, mask=None, beta=0.1, label_smoothing=0.0, grad_scale=1.0):
     """(``PreferenceLoss``, its gradient times ``grad_scale`` with respect to the logits) without an autograd graph: for ``logits.backward(grad)``."""
-    tensors, numbers = _prefer_inputs(logits, action, ref_logp, offsets, mask, beta, label_smoothing)
-    z, pairs = tensors[0], offsets.shape[0] // 2
-    lib = native.load()
-    loss = torch.empty((), dtype=torch.float32, device=z.device)
-    margin = torch.empty(pairs, dtype=torch.float32, device=z.device)
-    grad = torch.empty(logits.shape, dtype=z.dtype, device=z.device)
-    r, p = _rows(z, tensors[4], None, _w := _work(lib, z, tensors[4], pairs)), _prefer_struct(tensors, numbers, float(grad_scale))
-    native.check(lib, lib.ur5_policy_prefer_loss_grad(C.byref(r), C.byref(p), loss.data_ptr(), margin.data_ptr(), grad.data_ptr()), "ur5_policy_prefer_loss_grad")
+    p = _Prefer(logits, action, ref_logp, offsets, mask, beta, label_smoothing)
+    loss, margin = p.outputs()
+    grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    work = _work(p.z, p.mask, p.pairs)
+    _check(_library().ur5_policy_prefer_loss_grad(_rows(p.z, p.mask, None, work), p.pack(float(grad_scale)), loss.data_ptr(), margin.data_ptr(), grad.data_ptr()),
+           "ur5_policy_prefer_loss_grad")
     return PreferenceLoss(loss, margin), grad
