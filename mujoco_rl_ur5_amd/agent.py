@@ -26,15 +26,17 @@ output states the ratio it ran at (``update_to_data``).
 """
 from __future__ import annotations
 
+import contextlib
+import copy
 import math
 
 import numpy as np
 import torch
 import torch.nn.functional as F
 
-from . import sharding
+from . import checkpoint8, policy, sharding
 from .envs import GraspEnv
-from .qnet import MULTIDISCRETE_RESNET, ReplayBuffer, per_sample_statistics
+from .qnet import MULTIDISCRETE_POLICY_RESNET, MULTIDISCRETE_RESNET, ReplayBuffer, per_sample_statistics
 
 MEMORY_SIZE = 2000            # Grasping_Agent_multidiscrete.py:26-38
 BATCH_SIZE = 12
@@ -109,12 +111,21 @@ def color_jitter(rgb, generator=None, brightness=0.5, contrast=0.5, saturation=0
     return out
 
 
+def _saving(activations):
+    """The context of a forward pass whose backward pass follows: activations = None keeps them as they are, "int8" as 8-bit checkpoints (checkpoint8.saved_activations)."""
+    if activations not in (None, "int8"):
+        raise ValueError(f"activations must be None or 'int8', not {activations!r}")
+    return contextlib.nullcontext() if activations is None else checkpoint8.saved_activations()
+
+
 class Learner:
     """Replay buffer + optimiser step of ``Grasp_Agent`` (Grasping_Agent_multidiscrete.py:140-156, 388-446, 551-556) without the environment:
     what ``tests/test_qnet.py`` replays against a transition stream run through the reference's own ``Modules.ReplayBuffer`` and network."""
 
     def __init__(self, policy_net, height, width, device, learning_rate=LEARNING_RATE, mem_size=MEMORY_SIZE, batch_size=BATCH_SIZE,
-                 transitions_per_update=1, max_updates_per_round=64):
+                 transitions_per_update=1, max_updates_per_round=64, activations=None):
+        _saving(activations)
+        self.activations = activations                                                                   # "int8": the backward pass reads 8-bit checkpoints (checkpoint8.py), less than half of the memory
         self.policy_net, self.device, self.batch_size = policy_net, torch.device(device), int(batch_size)
         self.memory = ReplayBuffer(mem_size, height, width, device=self.device)                          # :140-142
         self.optimizer = torch.optim.Adam(self.policy_net.parameters(), lr=learning_rate, weight_decay=0.00002)   # :153-156
@@ -127,7 +138,8 @@ class Learner:
             return None
         state, action, reward = self.memory.sample(self.batch_size)
         self.policy_net.train()
-        q_pred = self.policy_net(state).reshape(self.batch_size, -1).gather(1, action)                   # :424-426
+        with _saving(self.activations):
+            q_pred = self.policy_net(state).reshape(self.batch_size, -1).gather(1, action)               # :424-426
         loss = F.binary_cross_entropy(q_pred, reward.float())                                            # :439
         loss.backward()
         self.optimizer.step()
@@ -190,10 +202,94 @@ class Learner:
         return losses, (len(losses) / n if n else 0.0)
 
 
+class PolicyLearner:
+    """Optimiser steps of a stochastic grasp policy: a network that ends in logits per (rotation, pixel) (``qnet.MULTIDISCRETE_POLICY_RESNET``; the reference's POLICY_RESNET,
+    Modules.py:304-305, has the head and no trainer), sampled and trained through the operators of ``policy.py``. Batch norm uses every image's own statistics throughout
+    (``qnet.per_sample_statistics``): the log-probabilities of a batch do not depend on what shares it, and a first step's ratios are 1.
+
+    kl_coef > 0 holds the policy to a frozen copy of the network it starts from. GPU only (policy.py)."""
+
+    def __init__(self, policy_net, device, learning_rate=LEARNING_RATE, batch_size=BATCH_SIZE, epochs=1, clip=0.2, kl_coef=0.0, entropy_coef=0.0, activations=None):
+        _saving(activations)
+        self.policy_net, self.device, self.batch_size, self.epochs, self.activations = policy_net, torch.device(device), int(batch_size), int(epochs), activations
+        self.clip, self.kl_coef, self.entropy_coef = clip, float(kl_coef), float(entropy_coef)
+        self.reference = None
+        if self.kl_coef > 0:
+            self.reference = copy.deepcopy(policy_net).train()
+            for p in self.reference.parameters():
+                p.requires_grad_(False)
+        self.optimizer = torch.optim.Adam(self.policy_net.parameters(), lr=learning_rate, weight_decay=0.00002)   # as Learner
+        self.last_loss, self.updates_done = None, 0
+
+    def logits(self, state, net=None):
+        """[N, 4, H, W] -> [N, R * H * W] (a view of the network's maps)."""
+        net = self.policy_net if net is None else net
+        net.train()
+        with per_sample_statistics():
+            return net(state).reshape(state.shape[0], -1)
+
+    def act(self, state, seed, gids, round_index, mask=None, chunk=256):
+        """(action [N], log-probability [N]) drawn for the scenes with global ids ``gids`` (``policy.sample_actions``); ``mask`` [N, H, W] or [N, H * W]: the pixels that may be chosen."""
+        parts = []
+        with torch.no_grad():
+            for i in range(0, state.shape[0], chunk):
+                part = slice(i, i + chunk)
+                parts.append(policy.sample_actions(self.logits(state[part]), seed, gids[part], round_index, mask=None if mask is None else mask[part]))
+        return torch.cat([a for a, _ in parts]), torch.cat([lp for _, lp in parts])
+
+    def log_probs(self, state, action, mask=None, net=None, chunk=256):
+        """Log-probabilities [N] of given actions, without a gradient (of another network with ``net``)."""
+        with torch.no_grad():
+            return torch.cat([policy.action_log_probs(self.logits(state[i:i + chunk], net), action[i:i + chunk], mask=None if mask is None else mask[i:i + chunk])[0]
+                              for i in range(0, state.shape[0], chunk)])
+
+    def _step(self, logits, grad):
+        logits.backward(grad)
+        self.optimizer.step()
+        self.optimizer.zero_grad()
+        self.updates_done += 1
+
+    def update(self, state, action, old_logp, advantage, mask=None):
+        """``epochs`` passes over N transitions in scene order, ``batch_size`` at a time, an optimiser step on the clipped policy loss each. Returns the losses."""
+        losses = []
+        for _ in range(self.epochs):
+            for i in range(0, state.shape[0], self.batch_size):
+                part = slice(i, i + self.batch_size)
+                ref = None
+                if self.reference is not None:
+                    with torch.no_grad():
+                        ref = self.logits(state[part], self.reference)
+                with _saving(self.activations):
+                    logits = self.logits(state[part])
+                terms, grad = policy.clipped_policy_grad(logits, action[part], old_logp[part], advantage[part], mask=None if mask is None else mask[part], ref_logits=ref,
+                                                         clip=self.clip, kl_coef=self.kl_coef, entropy_coef=self.entropy_coef)
+                self._step(logits, grad)
+                losses.append(terms.loss)
+        losses = torch.stack(losses).tolist() if losses else []
+        self.last_loss = losses[-1] if losses else None
+        return losses
+
+    def prefer(self, state, action, ref_logp, offsets, mask=None, beta=0.1, label_smoothing=0.0):
+        """One optimiser step on the preference loss over pairs of episodes (``policy.preference_loss``: rows are steps, offsets their episodes' ends). Returns (loss, margins)."""
+        with _saving(self.activations):
+            logits = self.logits(state)
+        terms, grad = policy.preference_grad(logits, action, ref_logp, offsets, mask=mask, beta=beta, label_smoothing=label_smoothing)
+        self._step(logits, grad)
+        self.last_loss = float(terms.loss)
+        return self.last_loss, terms.margin
+
+
 class BatchedGraspAgent:
     def __init__(self, env: GraspEnv = None, n_envs=1, device=None, learning_rate=LEARNING_RATE, mem_size=MEMORY_SIZE, eps_start=EPS_START,
                  eps_end=EPS_END, eps_decay=EPS_DECAY, seed=20, load_path=None, first_scene_id=0, n_total=None, transitions_per_update=1,
-                 max_updates_per_round=64, pipeline_groups=1, **env_kwargs):
+                 max_updates_per_round=64, pipeline_groups=1, objective="q", activations=None, policy_options=None, **env_kwargs):
+        # objective: "q" is the reference's (epsilon-greedy on a Q map, binary cross entropy from a replay buffer); "policy" samples the actions of a stochastic policy over the table's
+        # pixels and trains it on its own rounds (PolicyLearner, policy_options: its keyword arguments; advantage = reward minus the round's mean). activations="int8": 8-bit checkpoints.
+        if objective not in ("q", "policy"):
+            raise ValueError(f"objective must be 'q' or 'policy', not {objective!r}")
+        if objective == "policy" and (pipeline_groups > 1 or sharding.collectives_active()):
+            raise ValueError("objective='policy' trains one group of scenes on one rank")
+        self.objective = objective
         torch.manual_seed(seed)                                                        # :76-79
         np.random.seed(seed)
         self.device = torch.device(device if device is not None else ("cuda" if torch.cuda.is_available() else "cpu"))
@@ -232,16 +328,23 @@ class BatchedGraspAgent:
         self.N, self.H, self.W = sum(e.n_envs for e in self.envs), self.env.IMAGE_HEIGHT, self.env.IMAGE_WIDTH
         self.n_actions_1, self.n_actions_2 = int(self.env.action_space.nvec[0]), int(self.env.action_space.nvec[1])   # :97-100
         self.output = self.n_actions_1 * self.n_actions_2
-        self.policy_net = MULTIDISCRETE_RESNET(number_actions_dim_2=self.n_actions_2).to(self.device)     # :103
+        self.policy_net = (MULTIDISCRETE_RESNET if objective == "q" else MULTIDISCRETE_POLICY_RESNET)(number_actions_dim_2=self.n_actions_2).to(self.device)     # :103
         checkpoint = None
         if load_path is not None:                                                      # :109-114
             checkpoint = torch.load(load_path, map_location=self.device)
             self.policy_net.load_state_dict(checkpoint["model_state_dict"])
         self.depth_threshold = float(np.round(self.env.model.cam_pos0[self.env.model.camera_name2id("top_down")][2]
                                               - self.env.TABLE_HEIGHT + 0.01, decimals=3))   # :131-136
-        self.learner = Learner(self.policy_net, self.H, self.W, self.device, learning_rate, mem_size, BATCH_SIZE, transitions_per_update,
-                               max_updates_per_round)                                  # :140-156
-        self.memory, self.optimizer = self.learner.memory, self.learner.optimizer
+        if objective == "policy":
+            if self.device.type != "cuda":
+                raise ValueError("objective='policy' runs on the GPU (policy.py)")
+            self.learner = PolicyLearner(self.policy_net, self.device, learning_rate, activations=activations, **(policy_options or {}))
+            self.memory = None
+        else:
+            self.learner = Learner(self.policy_net, self.H, self.W, self.device, learning_rate, mem_size, BATCH_SIZE, transitions_per_update,
+                                   max_updates_per_round, activations)                 # :140-156
+            self.memory = self.learner.memory
+        self.optimizer = self.learner.optimizer
         self.eps_start, self.eps_end, self.eps_decay = eps_start, eps_end, eps_decay
         self.steps_done, self.eps_threshold = 0, eps_start
         # :165-180 / :215-217 / :448-465: how often the greedy policy chose each rotation, and the successes per rotation of greedy and of random actions. Kept as device
@@ -309,15 +412,19 @@ class BatchedGraspAgent:
         u = sharding.scene_uniform(self.seed, gids, self.rounds_done, 1, 3, dtype=torch.float64)         # explore?, which table pixel, which rotation
         explore = u[:, 0] <= self.eps_threshold
         greedy_action = self._q_all(state)[1]
-        world = env.pixel_world_device(observation["depth"], self.device)                                # [N,H,W,3]
-        on_table = (world[..., 2] >= env.TABLE_HEIGHT - 0.01).reshape(n, -1)
-        on_table = torch.where(on_table.any(dim=1, keepdim=True), on_table, torch.ones_like(on_table))
+        on_table = self._on_table(observation, env)
         cdf = on_table.cumsum(dim=1, dtype=torch.int32)                                                  # uniform over the table pixels: inverse CDF of the draw (int32: 40 000 pixels)
         want = torch.floor(u[:, 1] * cdf[:, -1].double()).to(torch.int32) + 1                            # the want-th table pixel, 1-based
         pixel = torch.searchsorted(cdf, want[:, None]).squeeze(1).clamp(max=self.n_actions_1 - 1)
         rot = torch.floor(u[:, 2] * self.n_actions_2).long().clamp(max=self.n_actions_2 - 1)
         random_action = rot * self.n_actions_1 + pixel
         return torch.where(explore, random_action, greedy_action), ~explore
+
+    def _on_table(self, observation, env):
+        """[N, H * W]: the pixels of every scene that lie on the table (:266-280); all of them where none does."""
+        world = env.pixel_world_device(observation["depth"], self.device)                                # [N,H,W,3]
+        on_table = (world[..., 2] >= env.TABLE_HEIGHT - 0.01).flatten(1)
+        return torch.where(on_table.any(dim=1, keepdim=True), on_table, torch.ones_like(on_table))
 
     def _q_all(self, state, chunk=256):
         """(max Q [N], argmax over the 6*H*W (rotation, pixel) pairs [N]) of every scene: the network runs on `chunk` scenes at a time -- its
@@ -345,6 +452,8 @@ class BatchedGraspAgent:
     # ------------------------------------------------------------------ learning
     def learn(self):
         """One optimiser step (:388-446), see ``Learner.learn``."""
+        if self.objective == "policy":
+            raise RuntimeError("objective='policy' learns within round(): it keeps no transitions")
         self.last_loss = self.learner.learn()
         return self.last_loss
 
@@ -416,13 +525,24 @@ class BatchedGraspAgent:
         obs = self.env.observation_device(self.device)
         raw = {k: v.clone() for k, v in obs.items()} if return_observation else None
         state = self.transform_observation(obs)
-        action, greedy = self.epsilon_greedy(state, obs)
+        if self.objective == "policy":
+            self.begin_round_epsilon()                                                                   # (counts the transitions; nothing explores by epsilon here)
+            mask = self._on_table(obs, self.env)
+            action, logp = self.learner.act(state, self.seed, self.gids, self.rounds_done, mask)
+            greedy = torch.ones_like(action, dtype=torch.bool)
+        else:
+            action, greedy = self.epsilon_greedy(state, obs)
         env_action = self.transform_action(action)
         reward, skipped = self.env.step_device(env_action, obs["depth"], self.device)
         rec = torch.stack([self.gids.int(), env_action[:, 0].int(), env_action[:, 1].int(), reward.int()], dim=1)
         outcomes = sharding.gather_outcomes(rec)                                                         # the round's only collective on the rollout side: 16 B per scene
-        losses, utd = self.learner.push_and_learn(state, action, reward, learn=learn, outcomes=outcomes if self.shared else None,
-                                                  first_scene_id=self.first_scene_id, n_actions_1=self.n_actions_1)   # :551-556
+        if self.objective == "policy":
+            advantage = reward.float() - reward.float().mean()
+            losses = self.learner.update(state, action, logp, advantage, mask) if learn else []
+            utd = len(losses) / self.N
+        else:
+            losses, utd = self.learner.push_and_learn(state, action, reward, learn=learn, outcomes=outcomes if self.shared else None,
+                                                      first_scene_id=self.first_scene_id, n_actions_1=self.n_actions_1)   # :551-556
         return self._end_round(learn, losses, utd, raw, action, reward, skipped, greedy, outcomes)
 
     def _rotation_dict(self, row):

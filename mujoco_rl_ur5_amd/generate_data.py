@@ -43,9 +43,11 @@ def main():
     ap.add_argument("--out", default="Data")
     ap.add_argument("--seed", type=int, default=122)                         # generate_data.py:16
     ap.add_argument("--load-path", default=None, help="checkpoint of the reference's agent (:18, checkpoint['model_state_dict'])")
+    ap.add_argument("--objective", choices=("q", "policy"), default="q", help="epsilon-greedy Q learning (the reference's), or a sampled policy trained on its own rounds")
+    ap.add_argument("--activations", choices=("int8",), default=None, help="keep the network's activations for its backward pass in 8 bits")
     a = ap.parse_args()
     from .agent import BatchedGraspAgent
-    agent = BatchedGraspAgent(n_envs=a.n_envs, seed=a.seed, load_path=a.load_path, mem_size=100)   # :23-29
+    agent = BatchedGraspAgent(n_envs=a.n_envs, seed=a.seed, load_path=a.load_path, mem_size=100, objective=a.objective, activations=a.activations)   # :23-29
     files, counter = generate_data(agent, a.out, a.episodes, a.steps, verbose=True)
     print(f"{len(files)} files in {a.out}; reward counter {counter}")
 
