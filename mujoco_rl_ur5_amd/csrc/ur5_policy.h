@@ -52,16 +52,20 @@ __device__ __forceinline__ float narrow(f32_t, float v) { return v; }
 __device__ __forceinline__ uint16_t narrow(f16_t, float v) { return __builtin_bit_cast(uint16_t, (_Float16)v); }
 __device__ __forceinline__ uint16_t narrow(bf16_t, float v) { return __builtin_bit_cast(uint16_t, (__bf16)v); }   // to nearest, ties to even
 
-__device__ __forceinline__ void load8(f32_t, const float* p, float* v) {
-  const F4 a = *(const F4*)p, b = *(const F4*)(p + 4);
+// 8 values as they lie in memory: what is loaded ahead of its use
+template <typename T> struct Eight { U4 w; };
+template <> struct Eight<f32_t> { F4 a, b; };
+template <typename T> __device__ __forceinline__ Eight<T> fetch8(const typename T::raw* p) { return Eight<T>{*(const U4*)p}; }
+template <> __device__ __forceinline__ Eight<f32_t> fetch8<f32_t>(const float* p) { return Eight<f32_t>{*(const F4*)p, *(const F4*)(p + 4)}; }
+__device__ __forceinline__ void unpack8(const Eight<f32_t>& e, float* v) {
 #pragma unroll
-  for (int i = 0; i < 4; i++) { v[i] = a[i]; v[4 + i] = b[i]; }
+  for (int i = 0; i < 4; i++) { v[i] = e.a[i]; v[4 + i] = e.b[i]; }
 }
-template <typename T> __device__ __forceinline__ void load8(T tag, const uint16_t* p, float* v) {
-  const U4 a = *(const U4*)p;
+template <typename T> __device__ __forceinline__ void unpack8(const Eight<T>& e, float* v) {
 #pragma unroll
-  for (int i = 0; i < 4; i++) { v[2 * i] = widen(tag, (uint16_t)a[i]); v[2 * i + 1] = widen(tag, (uint16_t)(a[i] >> 16)); }
+  for (int i = 0; i < 4; i++) { v[2 * i] = widen(T{}, (uint16_t)e.w[i]); v[2 * i + 1] = widen(T{}, (uint16_t)(e.w[i] >> 16)); }
 }
+template <typename T> __device__ __forceinline__ void load8(T, const typename T::raw* p, float* v) { unpack8(fetch8<T>(p), v); }
 __device__ __forceinline__ void store8(f32_t, float* p, const float* v) {
   F4 a, b;
 #pragma unroll
@@ -75,9 +79,8 @@ template <typename T> __device__ __forceinline__ void store8(T tag, uint16_t* p,
   *(U4*)p = a;
 }
 
-// 8 values from p on, of which the first `left` exist (whole: all)
-template <typename T> __device__ __forceinline__ void take8(const typename T::raw* p, int left, bool whole, float* v) {
-  if (whole) { load8(T{}, p, v); return; }
+// 8 values from p on, of which the first `left` exist
+template <typename T> __device__ __forceinline__ void take8(const typename T::raw* p, int left, float* v) {
 #pragma unroll
   for (int i = 0; i < VEC; i++) v[i] = i < left ? widen(T{}, p[i]) : -INFINITY;
 }
@@ -102,9 +105,10 @@ template <typename T> __device__ __forceinline__ bool action_counts(const Rows& 
   return !(logit<T>(R, row, a) == -INFINITY);
 }
 
-// ---- the 8s of a piece. visit(first action, allowed bits, values that exist, whole) for every 8 pixels of every map of the piece that hold an allowed one.
-// Logits that may not be taken are not read: the allowed 8s of the piece's pixels are listed in LDS once (the maps share them) and dealt to the threads from the list, so that no
-// lane idles where the mask has holes. A table of 42 % of the image: statistics of 513 bf16 rows 123 -> 87 us by not reading the rest.
+// ---- the 8s of a piece. For every 8 pixels of every map of the piece that hold an allowed one: use(first action, allowed bits, fetch(first action)), or
+// part(first action, allowed bits, values that exist) where the mask ends inside the 8; none(piece, 8) for the others, once for all maps.
+// A thread fetches its next 8 before it uses one: what a workgroup does is a chain of latencies. Logits that may not be taken are not read: the allowed 8s of the piece's
+// pixels are listed in LDS once (the maps share them) and dealt to the threads from the list, so that no lane idles where the mask has holes.
 struct Piece { int first, pixels, map0, maps; };   // pixels first .. of maps map0 ..
 __device__ __forceinline__ Piece piece_of(const Rows& R, int piece) {
   const int x = piece % R.pieces_x, y = piece / R.pieces_x;
@@ -113,67 +117,95 @@ __device__ __forceinline__ Piece piece_of(const Rows& R, int piece) {
   P.maps = min(R.maps_per, R.maps - P.map0);
   return P;
 }
-__device__ __forceinline__ uint32_t allowed8(const uint8_t* mask, int left, bool whole) {   // a byte per pixel -> a bit per pixel
+__device__ __forceinline__ uint32_t four(uint32_t bytes) {      // a byte per pixel, non-zero = allowed -> a bit per pixel
+  const uint32_t ones = (((bytes & 0x7f7f7f7fu) + 0x7f7f7f7fu) | bytes) >> 7 & 0x01010101u;
+  return __builtin_amdgcn_udot4(ones, 0x08040201u, 0, false);
+}
+__device__ __forceinline__ uint32_t allowed8(const uint8_t* mask, int left, bool whole) {
   uint64_t b = 0;
   if (whole) b = *(const U8*)mask;
   else for (int i = 0; i < left; i++) b |= (uint64_t)mask[i] << (8 * i);
-  uint32_t bits = 0;
-#pragma unroll
-  for (int i = 0; i < VEC; i++) bits |= (b >> (8 * i) & 0xff) ? 1u << i : 0u;
-  return bits;
+  return four((uint32_t)b) | four((uint32_t)(b >> 32)) << 4;
 }
-template <bool MASK, typename V, typename N> __device__ __forceinline__ void for_piece(const Rows& R, int row, int piece, V visit, N none) {
+template <typename A, typename F, typename U> __device__ __forceinline__ void in_turns(int all, A at, F fetch, U use) {   // items threadIdx.x, + THREADS, .. below all
+  int i = threadIdx.x;
+  if (i >= all) return;
+  auto one = at(i);
+  auto a = fetch(one);
+  for (;;) {
+    const bool more = (i += THREADS) < all;
+    auto other = one;
+    auto b = a;
+    if (more) { other = at(i); b = fetch(other); }
+    use(one, a);
+    if (!more) return;
+    const bool again = (i += THREADS) < all;
+    if (again) { one = at(i); a = fetch(one); }
+    use(other, b);
+    if (!again) return;
+  }
+}
+template <bool MASK, typename F, typename U, typename P8, typename N> __device__ __forceinline__ void for_piece(const Rows& R, int row, int piece, F fetch, U use, P8 part, N none) {
   const Piece P = piece_of(R, piece);
+  struct At { int j; uint32_t allowed; };
+  const auto fetch_at = [&](const At& a) { return fetch(a.j); };
+  const auto use_at = [&](const At& a, const auto& e) { use(a.j, a.allowed, e); };
+  const int tail = P.pixels % VEC, last = P.first + P.pixels - tail;      // the row's or the mask's last, shorter 8
   if (!MASK) {                      // one map: pixel = action
-    const int whole = P.pixels / VEC;
-#pragma unroll 2
-    for (int g = threadIdx.x; g < whole; g += THREADS) visit(P.first + g * VEC, 0xffu, VEC, yes{});
-    const int left = P.pixels % VEC;
-    if (left && threadIdx.x == whole % THREADS) visit(P.first + whole * VEC, (1u << left) - 1, left, no{});
+    in_turns(P.pixels / VEC, [&](int i) { return At{P.first + i * VEC, 0xffu}; }, fetch_at, use_at);
+    if (tail && threadIdx.x == 0) part(last, (1u << tail) - 1, tail);
     return;
   }
   const uint8_t* mask = R.mask + row * R.mask_stride + P.first;
+  if (tail) {                       // a thread per map
+    const uint32_t bits = allowed8(mask + P.pixels - tail, tail, false);
+    if (!bits) { if (threadIdx.x == 0) none(P, P.pixels / VEC); }
+    else for (int m = threadIdx.x; m < P.maps; m += THREADS) part((P.map0 + m) * R.pixels + last, bits, tail);
+  }
   if (R.per == 1 && R.maps_per == 1) {   // a small batch, cut into pieces of an 8 per thread: latency counts, so the logits are asked for together with their mask
-    const int g = threadIdx.x, left = P.pixels - g * VEC, j = P.map0 * R.pixels + P.first + g * VEC;
-    if (left >= VEC) visit(j, allowed8(mask + g * VEC, VEC, true), VEC, yes{});
-    else if (left > 0) visit(j, allowed8(mask + g * VEC, left, false), left, no{});
+    const int g = threadIdx.x, j = P.map0 * R.pixels + P.first + g * VEC;
+    if (g < P.pixels / VEC) {
+      const auto e = fetch(j);
+      use(j, allowed8(mask + g * VEC, VEC, true), e);
+    }
     return;
   }
   __shared__ uint32_t list[MOST_PER_MASKED * THREADS];      // group of 8 << 8 | bits, in the order of the pixels
-  __shared__ int share[MOST_PER_MASKED * THREADS / 64];     // entries of each wavefront of each tile
+  __shared__ int4 share[MOST_PER_MASKED];                   // entries of the four wavefronts of each tile
+  static_assert(THREADS / 64 == 4, "an int4 of wavefronts");
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   uint32_t bits[MOST_PER_MASKED];
   int before[MOST_PER_MASKED];
 #pragma unroll
   for (int t = 0; t < MOST_PER_MASKED; t++) {
-    const int g = t * THREADS + threadIdx.x, left = P.pixels - g * VEC;
-    bits[t] = left >= VEC ? allowed8(mask + g * VEC, VEC, true) : left > 0 ? allowed8(mask + g * VEC, left, false) : 0;
+    if (t >= R.per) break;
+    const int g = t * THREADS + threadIdx.x;
+    const bool in = g < P.pixels / VEC;
+    bits[t] = in ? allowed8(mask + g * VEC, VEC, true) : 0;
     const uint64_t some = __ballot(bits[t] != 0);
-    before[t] = __popcll(some & ((1ull << lane) - 1));
-    if (lane == 0) share[t * (THREADS / 64) + wave] = __popcll(some);
-    if (!bits[t] && left > 0) none(P, g);
+    before[t] = __builtin_amdgcn_mbcnt_hi((uint32_t)(some >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)some, 0));
+    if (lane == 0) ((int*)&share[t])[wave] = __popcll(some);
+    if (in && !bits[t]) none(P, g);
   }
   __syncthreads();
   int n = 0;
 #pragma unroll
-  for (int t = 0; t < MOST_PER_MASKED; t++)
-#pragma unroll
-    for (int w = 0; w < THREADS / 64; w++) {
-      if (w == wave && bits[t]) list[n + before[t]] = (uint32_t)(t * THREADS + threadIdx.x) << 8 | bits[t];
-      n += share[t * (THREADS / 64) + w];
-    }
+  for (int t = 0; t < MOST_PER_MASKED; t++) {
+    if (t >= R.per) break;
+    const int4 w = share[t];
+    const int mine = n + (wave > 0 ? w.x : 0) + (wave > 1 ? w.y : 0) + (wave > 2 ? w.z : 0);
+    if (bits[t]) list[mine + before[t]] = (uint32_t)(t * THREADS + threadIdx.x) << 8 | bits[t];
+    n += w.x + w.y + w.z + w.w;
+  }
   __syncthreads();
-  const int all = n * P.maps;
   const float per = __builtin_amdgcn_rcpf((float)n);
-  for (int i = threadIdx.x; i < all; i += THREADS) {
-    int m = (int)(((float)i + 0.5f) * per), k = i - m * n;             // map and list entry of item i; the estimate is off by at most one
+  in_turns(n * P.maps, [&](int i) {
+    int m = (int)(((float)i + 0.5f) * per), k = i - m * n;               // map and list entry of item i; the estimate is off by at most one
     if (k < 0) { m--; k += n; }
     if (k >= n) { m++; k -= n; }
     const uint32_t e = list[k];
-    const int p = P.first + (e >> 8) * VEC, left = R.pixels - p, j = (P.map0 + m) * R.pixels + p;
-    if (left >= VEC) visit(j, e & 0xff, VEC, yes{});
-    else visit(j, e & 0xff, left, no{});
-  }
+    return At{(P.map0 + m) * R.pixels + P.first + (int)(e >> 8) * VEC, e & 0xff};
+  }, fetch_at, use_at);
 }
 
 // ---- reductions over 64 or 4 neighbouring lanes, in every lane, in a fixed order: lanes of a row of 16 exchange through DPP, the four rows through scalar registers
@@ -290,17 +322,24 @@ __device__ __forceinline__ Sums join_workgroup(const Running& r, bool ref, bool 
 }
 
 // ---- statistics of the pieces of rows
+template <typename T, bool REF> struct Both {       // 8 logits, and the reference's
+  Eight<T> z, q;
+  __device__ __forceinline__ Both(const typename T::raw* z_row, const typename T::raw* q_row, int j) : z(fetch8<T>(z_row + j)) { if (REF) q = fetch8<T>(q_row + j); }
+  __device__ __forceinline__ void get(float* a, float* b) const { unpack8(z, a); if (REF) unpack8(q, b); }
+};
 template <typename T, bool MASK, bool REF, bool ENTROPY> __device__ __forceinline__ Sums piece_sums(const Rows& R, int row, int piece) {
   const auto* z_row = (const typename T::raw*)R.logits + row * R.stride;
   const auto* q_row = REF ? (const typename T::raw*)R.ref + row * R.ref_stride : nullptr;
   Running a = nothing();
-  for_piece<MASK>(R, row, piece, [&](int j, uint32_t allowed, int left, auto whole) {
-    float z[VEC], q[VEC], e[VEC];
-    take8<T>(z_row + j, left, decltype(whole)::value, z);
-    if (REF) take8<T>(q_row + j, left, decltype(whole)::value, q);
+  const auto add = [&](uint32_t allowed, float* z, float* q) {
+    float e[VEC];
     if (MASK) { bar8(allowed, z); if (REF) bar8(allowed, q); }
     add8<REF, ENTROPY>(a, z, q, e);
-  }, [](const Piece&, int) {});
+  };
+  for_piece<MASK>(R, row, piece, [&](int j) { return Both<T, REF>(z_row, q_row, j); },
+    [&](int, uint32_t allowed, const Both<T, REF>& b) { float z[VEC], q[VEC]; b.get(z, q); add(allowed, z, q); },
+    [&](int j, uint32_t allowed, int left) { float z[VEC], q[VEC]; take8<T>(z_row + j, left, z); if (REF) take8<T>(q_row + j, left, q); add(allowed, z, q); },
+    [](const Piece&, int) {});
   return join_workgroup(a, REF, ENTROPY);
 }
 
@@ -394,10 +433,7 @@ template <typename T, bool MASK, bool REF> __global__ void __launch_bounds__(THR
   const int a = (int)action[row];
   const auto* z_row = (const typename T::raw*)R.logits + row * R.stride;
   const auto* q_row = REF ? (const typename T::raw*)R.ref + row * R.ref_stride : nullptr;
-  for_piece<MASK>(R, row, piece, [&](int j, uint32_t allowed, int left, auto whole) {
-    float z[VEC], q[VEC], g[VEC];
-    take8<T>(z_row + j, left, decltype(whole)::value, z);
-    if (REF) take8<T>(q_row + j, left, decltype(whole)::value, q);
+  const auto slope = [&](int j, uint32_t allowed, float* z, const float* q, float* g) {
     if (MASK) bar8(allowed, z);
 #pragma unroll
     for (int i = 0; i < VEC; i++) {
@@ -409,8 +445,16 @@ template <typename T, bool MASK, bool REF> __global__ void __launch_bounds__(THR
     if ((unsigned)(a - j) < VEC)
 #pragma unroll
       for (int i = 0; i < VEC; i++) g[i] += a - j == i ? S.take : 0.f;
-    put8<T>(out + j, left, decltype(whole)::value, g);
-  }, clear);
+  };
+  for_piece<MASK>(R, row, piece, [&](int j) { return Both<T, REF>(z_row, q_row, j); },
+    [&](int j, uint32_t allowed, const Both<T, REF>& b) { float z[VEC], q[VEC], g[VEC]; b.get(z, q); slope(j, allowed, z, q, g); store8(T{}, out + j, g); },
+    [&](int j, uint32_t allowed, int left) {
+      float z[VEC], q[VEC], g[VEC];
+      take8<T>(z_row + j, left, z);
+      if (REF) take8<T>(q_row + j, left, q);
+      slope(j, allowed, z, q, g);
+      put8<T>(out + j, left, false, g);
+    }, clear);
 }
 
 // ---- clipped policy loss. Per row: ratio r = exp(logp - old), L = -min(r A, clip(r, 1 - lo, 1 + hi) A) + kl_coef KL(p || q) - entropy_coef H; the mean over the rows that count.
@@ -559,14 +603,15 @@ template <typename T, bool MASK> __global__ void __launch_bounds__(THREADS) ur5_
   Running a = nothing();
   Best best{-INFINITY, NOBODY};
   bool first = true;
-  for_piece<MASK>(R, row, piece, [&](int j, uint32_t allowed, int left, auto whole) {
-    float z[VEC], e[VEC];
-    take8<T>(z_row + j, left, decltype(whole)::value, z);
+  const auto draw = [&](int j, uint32_t allowed, float* z) {
+    float e[VEC];
     if (MASK) bar8(allowed, z);
     add8<false, false>(a, z, nullptr, e);
     draw8<T>(z_row, key, j, a, z, e, first, &bar, best);
     first = false;
-  }, [](const Piece&, int) {});
+  };
+  for_piece<MASK>(R, row, piece, [&](int j) { return fetch8<T>(z_row + j); }, [&](int j, uint32_t allowed, const Eight<T>& w) { float z[VEC]; unpack8(w, z); draw(j, allowed, z); },
+    [&](int j, uint32_t allowed, int left) { float z[VEC]; take8<T>(z_row + j, left, z); draw(j, allowed, z); }, [](const Piece&, int) {});
   join_best(best, 64);
   if ((threadIdx.x & 63) == 0) wave[threadIdx.x >> 6] = best;
   const Sums sums = join_workgroup(a, false, false);   // (its barrier stands between the wavefronts' bests and their join)
