@@ -92,7 +92,7 @@ class _PointwiseConv(torch.autograd.Function):
     def forward(ctx, x, weight, bias):
         n, c = x.shape[:2]
         w = weight.reshape(weight.shape[0], c)
-        y = torch.matmul(w, x.reshape(n, c, -1))
+        y = torch.matmul(w, x.reshape(n, c, -1).contiguous())
         if bias is not None:
             y = y + bias.view(1, -1, 1)
         kept = pack(x)
@@ -107,7 +107,8 @@ class _PointwiseConv(torch.autograd.Function):
         dx = dw = db = None
         n, cin, cout = ctx.shape[0], ctx.shape[1], weight.shape[0]
         if ctx.needs_input_grad[0]:
-            dx = torch.matmul(weight.reshape(cout, cin).t().contiguous(), dy.reshape(n, cout, -1)).view(ctx.shape)
+            w = weight.reshape(cout, cin).t().contiguous().to(dy.dtype)                      # (under autocast the output, and so dy, has fewer bits than the input)
+            dx = torch.matmul(w, dy.reshape(n, cout, -1).contiguous()).view(ctx.shape).to(ctx.dtype)
         if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
             dw, db = PackedActivation(codes, scales, ctx.shape, ctx.dtype).weight_grad(dy, bias=ctx.has_bias)
             dw = dw.view(weight.shape).to(weight.dtype)
@@ -149,16 +150,17 @@ def active():
 
 
 class saved_activations:
-    """Context manager for a forward pass: floating-point GPU tensors of three or more dimensions (activations; parameters are left alone) that autograd saves inside it are kept as
-    8-bit checkpoints of at least ``min_values`` values and restored when their backward runs. In it, ``qnet``'s pointwise convolutions keep theirs for ``weight_grad`` and its ReLUs which values are positive (``relu``)."""
+    """Context manager for a forward pass: floating-point GPU tensors of three or more dimensions and at least ``min_values`` values that autograd saves inside it are kept as 8-bit
+    checkpoints and restored when their backward runs. Parameters (leaves that want a gradient) and views of them are left alone; a weight that is computed from parameters is an activation here. In it, ``qnet``'s pointwise convolutions keep theirs for ``weight_grad`` and its ReLUs which values are positive (``relu``)."""
 
     def __init__(self, min_values=4096):
         self.min_values = int(min_values)
 
     def _pack(self, t):
-        if not (t.is_cuda and t.dtype in DTYPES and t.dim() >= 3 and t.numel() >= self.min_values) or (t.is_leaf and t.requires_grad):
+        if not (t.is_cuda and t.dtype in DTYPES and t.dim() >= 3 and t.numel() >= self.min_values):
             return t
-        return pack(t)
+        source = t if t._base is None else t._base
+        return t if source.is_leaf and source.requires_grad else pack(t)                     # a parameter, or a view of one
 
     @staticmethod
     def _unpack(t):

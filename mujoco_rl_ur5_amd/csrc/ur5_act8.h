@@ -151,9 +151,9 @@ template <typename T, int A, int B, int WO, int WC> __global__ void __launch_bou
   using R = typename T::raw;
   constexpr int N = Terms<T>::N, TO = 32 * A * WO, TC = 32 * B * WC, COUNT = 64 * WO * WC, ROWS = TO * 8 / COUNT;
   __shared__ U4a shared[2][N][8][TO + 1];                                // [buffer][term][8 pixels][output channel]
-  // workgroups of one range sit on one XCD and run together: they share the range's gradients and codes in its L2
-  const int tiles = W.o_tiles * W.c_tiles, b = blockIdx.x;
-  const int split = (b & 7) + 8 * ((b >> 3) / tiles), tile = (b >> 3) % tiles;
+  // workgroups of one range sit on one XCD and run together: they share the range's gradients and codes in its L2 (less than 8 ranges: one after the other)
+  const int tiles = W.o_tiles * W.c_tiles, b = blockIdx.x, xcds = W.splits & 7 ? 1 : 8;
+  const int split = b % xcds + xcds * (b / xcds / tiles), tile = b / xcds % tiles;
   const int o0 = tile / W.c_tiles * TO, c0 = tile % W.c_tiles * TC;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, half = lane >> 5;
   const int wave_o = wave / WC * 32 * A, wave_c = wave % WC * 32 * B;

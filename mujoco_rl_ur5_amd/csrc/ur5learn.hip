@@ -40,13 +40,18 @@ int no_device(const char* entry, hipError_t e) {
 // thread's fp32 sums stay short (512 terms); images of less than 2048 pixels take as many maps as fill a workgroup. How many pieces a call aims at: more fill the card's 256 CUs
 // (8 workgroups each) more evenly, fewer share what a piece costs before and after its loads. us of the kernel at 2048 / 4096 / 8192 / 16384 pieces wanted:
 // sample (512 fp32 rows) 103 / 106 / 126 / 169, logp (2000 x 40 000 bf16) 45 / 37 / 39 / 49, statistics (513 bf16 rows) 106 / 100 / 94 / 103, gradient 131 / 110 / 102 / 98.
-constexpr int64_t PIECES = 4096, PIECES_LOSS = 8192, PIECES_GRADIENT = 16384, MOST_TURNS = 64;
+// A row of few turns is one piece of the calls that end with it: their second launch costs 3 us more than 5 turns (12 rows of 6 x 40 x 40, us a call: logp 13.6 -> 10.7, sample
+// 13.9 -> 11.8; of 11 turns: logp 13.7 -> 10.7, sample 14.0 -> 17.7).
+struct Aim { int64_t pieces, whole; };
+constexpr Aim SAMPLE{4096, 6}, LOGP{4096, 10}, LOSS{8192, 0}, GRADIENT{16384, 0};
+constexpr int64_t MOST_TURNS = 64;
 int64_t clamp(int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : v > hi ? hi : v; }
-void cut(int64_t rows, int64_t actions, int64_t mask_len, int64_t wanted, Rows* R) {
+void cut(int64_t rows, int64_t actions, int64_t mask_len, const Aim& aim, Rows* R) {
   const int64_t pixels = mask_len ? mask_len : actions, maps = actions / pixels, tiles = (pixels + TILE - 1) / TILE, groups = (pixels + VEC - 1) / VEC;
-  const int64_t turns = clamp(rows * tiles * maps / wanted, 1, MOST_TURNS);
+  const int64_t turns = clamp(rows * tiles * maps / aim.pieces, 1, MOST_TURNS);
   int64_t maps_per = clamp(turns, 1, maps), per = clamp(turns / maps_per, 1, mask_len ? MOST_PER_MASKED : MOST_PER);
   if (groups < THREADS) maps_per = clamp(THREADS / groups * maps_per, 1, maps);
+  if (tiles <= (mask_len ? MOST_PER_MASKED : MOST_PER) && (groups * maps + THREADS - 1) / THREADS <= aim.whole) { per = tiles; maps_per = maps; }
   R->rows = (int)rows; R->actions = (int)actions; R->pixels = (int)pixels; R->maps = (int)maps; R->per = (int)per; R->maps_per = (int)maps_per;
   R->pieces_x = (int)((tiles + per - 1) / per);
   R->pieces = (int)(R->pieces_x * ((maps + maps_per - 1) / maps_per));
@@ -62,22 +67,22 @@ int64_t lay_out(const Rows& R, int64_t terms, void* base, Work* w) {
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 constexpr int64_t MOST = 0x7fffffff;
 
-const char* check_size(int64_t rows, int64_t actions, int64_t mask_len, int64_t pairs, int64_t wanted, Rows* R) {
+const char* check_size(int64_t rows, int64_t actions, int64_t mask_len, int64_t pairs, const Aim& aim, Rows* R) {
   if (rows < 0 || actions < 1) return "rows must be at least 0 and actions at least 1";
   if (actions > MOST - 2 * TILE * MOST_PER || rows > MOST / 64 || pairs > MOST / 64) return "too many rows, pairs (2^25) or actions (2^31 - 65537)";
   if (mask_len < 0 || (mask_len && actions % mask_len)) return "mask_len must divide actions";
-  cut(rows, actions, mask_len, PIECES_GRADIENT, R);
+  cut(rows, actions, mask_len, GRADIENT, R);
   const int64_t most = R->pieces;                    // the finest of the cuts
-  cut(rows, actions, mask_len, wanted, R);
+  cut(rows, actions, mask_len, aim, R);
   if (rows * most > MOST - (rows + THREADS) / THREADS - FIRST) return "too many logits in one call";
   return nullptr;
 }
 // checks what every entry point over rows checks; launches nothing
-const char* check_rows(const ur5_rows* r, int64_t pairs, int64_t wanted, Rows* R, Work* w) {
+const char* check_rows(const ur5_rows* r, int64_t pairs, const Aim& aim, Rows* R, Work* w) {
   if (!r) return "no rows";
   if (r->dtype != UR5_F32 && r->dtype != UR5_F16 && r->dtype != UR5_BF16) return "dtype must be UR5_F32, UR5_F16 or UR5_BF16";
   if (r->mask && (r->mask_len < 1 || r->mask_stride < 0)) return "mask_len must be at least 1 and mask_stride at least 0";
-  if (const char* why = check_size(r->rows, r->actions, r->mask ? r->mask_len : 0, pairs, wanted, R)) return why;
+  if (const char* why = check_size(r->rows, r->actions, r->mask ? r->mask_len : 0, pairs, aim, R)) return why;
   if (r->stride < r->actions && r->rows > 1) return "the row stride is smaller than a row";
   if (r->ref && r->ref_stride < r->actions && r->rows > 1) return "the reference's row stride is smaller than a row";
   if (r->rows && !r->logits) return "no logits";
@@ -125,7 +130,7 @@ void prefer_pairs(const Rows& R, int dtype, hipStream_t s, const Prefer& P, cons
   by_type(dtype, [&](auto t) { ur5_policy_prefer_pairs<decltype(t)><<<P.pairs, THREADS, 0, s>>>(R, P, w.parts, w.slopes, w.term, margin); });
 }
 void gradient(Rows R, int dtype, hipStream_t s, const Terms& t, const int64_t* action, const Work& w, float scale, const float* upstream, void* grad) {
-  cut(R.rows, R.actions, R.mask ? R.pixels : 0, PIECES_GRADIENT, &R);      // it leaves no records
+  cut(R.rows, R.actions, R.mask ? R.pixels : 0, GRADIENT, &R);      // it leaves no records
   by_type(dtype, [&](auto k) { by_flag(R.mask, [&](auto m) { by_flag(R.ref, [&](auto q) {
     ur5_policy_grad<decltype(k), decltype(m)::value, decltype(q)::value><<<FIRST + R.rows * R.pieces, THREADS, 0, s>>>(R, t, action, w.slopes, scale, upstream, grad);
   }); }); });
@@ -139,12 +144,12 @@ extern "C" {
 
 int64_t ur5_policy_work_bytes(int64_t rows, int64_t actions, int64_t mask_len, int64_t pairs) {
   Rows R;
-  return pairs < 0 || check_size(rows, actions, mask_len, pairs, PIECES_LOSS, &R) ? 0 : lay_out(R, pairs, nullptr, nullptr);
+  return pairs < 0 || check_size(rows, actions, mask_len, pairs, LOSS, &R) ? 0 : lay_out(R, pairs, nullptr, nullptr);
 }
 
 int ur5_policy_sample(const ur5_rows* r, uint64_t offset, const int64_t* gids, int64_t* action, float* logp) {
   Rows R; Work w;
-  CHECK(check_rows(r, 0, PIECES, &R, &w));
+  CHECK(check_rows(r, 0, SAMPLE, &R, &w));
   if (!R.rows) return 0;
   if (!gids || !action || !logp) return fail(UR5_ERR_ARG, __func__, "gids, action and logp are needed");
   ON(r->device);
@@ -159,7 +164,7 @@ int ur5_policy_sample(const ur5_rows* r, uint64_t offset, const int64_t* gids, i
 
 int ur5_policy_logp(const ur5_rows* r, const int64_t* action, float* logp, float* entropy) {
   Rows R; Work w;
-  CHECK(check_rows(r, 0, PIECES, &R, &w));
+  CHECK(check_rows(r, 0, LOGP, &R, &w));
   if (!R.rows) return 0;
   if (!action || !logp) return fail(UR5_ERR_ARG, __func__, "action and logp are needed");
   ON(r->device);
@@ -173,7 +178,7 @@ int ur5_policy_logp(const ur5_rows* r, const int64_t* action, float* logp, float
 
 int ur5_policy_clip_loss(const ur5_rows* r, const ur5_clip* c, float* loss, float* logp, float* kl, float* entropy) {
   Rows R; Work w;
-  CHECK(check_rows(r, 0, PIECES_LOSS, &R, &w));
+  CHECK(check_rows(r, 0, LOSS, &R, &w));
   CHECK(check_clip(r, c));
   if (!loss || (R.rows && (!logp || !kl || !entropy))) return fail(UR5_ERR_ARG, __func__, "loss, logp, kl and entropy are needed");
   ON(r->device);
@@ -184,7 +189,7 @@ int ur5_policy_clip_loss(const ur5_rows* r, const ur5_clip* c, float* loss, floa
 }
 int ur5_policy_clip_grad(const ur5_rows* r, const ur5_clip* c, void* grad) {
   Rows R; Work w;
-  CHECK(check_rows(r, 0, PIECES_LOSS, &R, &w));
+  CHECK(check_rows(r, 0, LOSS, &R, &w));
   CHECK(check_clip(r, c));
   if (!R.rows) return 0;
   if (!grad) return fail(UR5_ERR_ARG, __func__, "grad is needed");
@@ -194,7 +199,7 @@ int ur5_policy_clip_grad(const ur5_rows* r, const ur5_clip* c, void* grad) {
 }
 int ur5_policy_clip_loss_grad(const ur5_rows* r, const ur5_clip* c, float* loss, float* logp, float* kl, float* entropy, void* grad) {
   Rows R; Work w;
-  CHECK(check_rows(r, 0, PIECES_LOSS, &R, &w));
+  CHECK(check_rows(r, 0, LOSS, &R, &w));
   CHECK(check_clip(r, c));
   if (!loss || (R.rows && (!logp || !kl || !entropy || !grad))) return fail(UR5_ERR_ARG, __func__, "loss, logp, kl, entropy and grad are needed");
   ON(r->device);
@@ -206,7 +211,7 @@ int ur5_policy_clip_loss_grad(const ur5_rows* r, const ur5_clip* c, float* loss,
 
 int ur5_policy_prefer_loss(const ur5_rows* r, const ur5_prefer* p, float* loss, float* margin) {
   Rows R; Work w;
-  CHECK(check_rows(r, p ? p->pairs : 0, PIECES_LOSS, &R, &w));
+  CHECK(check_rows(r, p ? p->pairs : 0, LOSS, &R, &w));
   CHECK(check_prefer(r, p));
   if (!loss || !margin) return fail(UR5_ERR_ARG, __func__, "loss and margin are needed");
   R.ref = nullptr;
@@ -218,7 +223,7 @@ int ur5_policy_prefer_loss(const ur5_rows* r, const ur5_prefer* p, float* loss, 
 }
 int ur5_policy_prefer_grad(const ur5_rows* r, const ur5_prefer* p, void* grad) {
   Rows R; Work w;
-  CHECK(check_rows(r, p ? p->pairs : 0, PIECES_LOSS, &R, &w));
+  CHECK(check_rows(r, p ? p->pairs : 0, LOSS, &R, &w));
   CHECK(check_prefer(r, p));
   if (!R.rows) return 0;
   if (!grad) return fail(UR5_ERR_ARG, __func__, "grad is needed");
@@ -229,7 +234,7 @@ int ur5_policy_prefer_grad(const ur5_rows* r, const ur5_prefer* p, void* grad) {
 }
 int ur5_policy_prefer_loss_grad(const ur5_rows* r, const ur5_prefer* p, float* loss, float* margin, void* grad) {
   Rows R; Work w;
-  CHECK(check_rows(r, p ? p->pairs : 0, PIECES_LOSS, &R, &w));
+  CHECK(check_rows(r, p ? p->pairs : 0, LOSS, &R, &w));
   CHECK(check_prefer(r, p));
   if (!loss || !margin || (R.rows && !grad)) return fail(UR5_ERR_ARG, __func__, "loss, margin and grad are needed");
   R.ref = nullptr;
@@ -272,7 +277,7 @@ int ur5_act8_unpack(const int8_t* codes, const float* scales, int64_t planes, in
 }
 
 // ---- weight gradient: how the work is split. Tiles of 128 output x 256 input channels (of half the outputs, and of half or a quarter of the inputs where there are no more),
-// and as many ranges of the pixels as give every CU a workgroup (two of the smaller ones), a multiple of 8: one set per XCD.
+// and as many ranges of the pixels as give every CU a workgroup (two of the smaller ones): less than 8, or a multiple of 8, one set per XCD.
 constexpr int64_t WORKGROUPS = 256;
 struct WgradPlan { int to, tc, o_tiles, c_tiles, splits; int64_t part, bytes; };
 static WgradPlan wgrad_plan(int64_t n, int64_t cin, int64_t cout, int64_t size) {
@@ -281,7 +286,7 @@ static WgradPlan wgrad_plan(int64_t n, int64_t cin, int64_t cout, int64_t size) 
   p.o_tiles = (int)((cout + p.to - 1) / p.to); p.c_tiles = (int)((cin + p.tc - 1) / p.tc);
   const int64_t groups = n * ((size + ur5act8::GROUP - 1) / ur5act8::GROUP), tiles = (int64_t)p.o_tiles * p.c_tiles;
   const int64_t s = clamp((WORKGROUPS * (p.to == 64 ? 2 : 1) + tiles - 1) / tiles, 1, groups > 0 ? groups : 1);
-  p.splits = (int)((s + 7) / 8 * 8);
+  p.splits = (int)(s < 8 ? s : (s + 7) / 8 * 8);
   p.part = ((int64_t)p.splits * cin * cout * 4 + 15) / 16 * 16;
   p.bytes = p.part + (int64_t)p.splits * cout * 4;
   return p;

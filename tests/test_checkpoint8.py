@@ -320,3 +320,81 @@ def test_relu_keeps_signs():
     got, = torch.autograd.grad(checkpoint8.relu(x), x, up)
     want, = torch.autograd.grad(torch.relu(x), x, up)
     assert torch.equal(checkpoint8.relu(x), torch.relu(x)) and torch.equal(got, want)
+
+
+@pytest.mark.gpu
+def test_parameters_are_not_packed():
+    """Leaves that want a gradient, and views of them, are saved as they are; the activation between the two layers is packed. The input gradient depends on the weights alone."""
+    torch.manual_seed(2)
+    conv = nn.Conv2d(64, 64, 3, padding=1, bias=False).cuda()
+    line = nn.Parameter(torch.randn(64 * 64, device="cuda"))
+    x = torch.randn(2, 64, 20, 20, device="cuda").requires_grad_()
+    up = torch.randn(2, 64, 20, 20, device="cuda")
+    f = lambda: nn.functional.conv2d(conv(x), line.view(64, 64, 1, 1))  # noqa: E731
+    want, = torch.autograd.grad(f(), x, up)
+    packed = []
+    original = checkpoint8.pack
+    try:
+        checkpoint8.pack = lambda t: packed.append(tuple(t.shape)) or original(t)
+        with checkpoint8.saved_activations():
+            y = f()
+    finally:
+        checkpoint8.pack = original
+    got, = torch.autograd.grad(y, x, up)
+    assert packed == [(2, 64, 20, 20)] and torch.allclose(got, want, rtol=1e-5, atol=1e-5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_pointwise_conv_under_autocast(dtype):
+    g = torch.Generator().manual_seed(5)
+    x = torch.randn(3, 20, 9, 14, generator=g).cuda().requires_grad_()
+    w, b = torch.randn(11, 20, generator=g).cuda().requires_grad_(), torch.randn(11, generator=g).cuda().requires_grad_()
+    up = torch.randn(3, 11, 9, 14, generator=g).cuda()
+    with torch.autocast("cuda", dtype=dtype):
+        y = checkpoint8.pointwise_conv(x, w, b)
+    grads = torch.autograd.grad(y, (x, w, b), up.to(y.dtype))
+    assert all(t.dtype == torch.float32 for t in grads)
+    want = torch.autograd.grad(nn.functional.conv2d(x.double(), w.double()[..., None, None], b.double()), (x, w, b), up.double())
+    # products of two values rounded to the type, and inputs half a checkpoint's step off (1 / 254 of their group's largest): a few per cent of the largest entry is far over both
+    for a, e in zip(grads, want):
+        assert float((a.double() - e).abs().max()) < 0.03 * float(e.abs().max())
+
+
+@pytest.mark.gpu
+def test_weight_gradient_of_many_channels():
+    """More tiles than CUs: less than 8 ranges of the pixels."""
+    g = torch.Generator().manual_seed(8)
+    _check_wgrad(torch.randn(2, 2100, 70, generator=g).cuda(), torch.randn(2, 4200, 70, generator=g).cuda())
+    _check_wgrad(torch.randn(3, 1300, 200, generator=g).cuda(), torch.randn(3, 1100, 200, generator=g).cuda())
+
+
+@pytest.mark.gpu
+def test_checkpoints_in_graphs_and_on_streams():
+    g = torch.Generator().manual_seed(9)
+    xs = [torch.randn(3, 70, 300, generator=g).cuda() for _ in range(3)]
+    ds = [torch.randn(3, 65, 300, generator=g).cuda() for _ in range(3)]
+    both = lambda x, d: (lambda k: (k.unpack(),) + k.weight_grad(d))(checkpoint8.pack(x))  # noqa: E731
+    want = [both(x, d) for x, d in zip(xs, ds)]
+    x, d = xs[0].clone(), ds[0].clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = both(x, d)
+    for k in (0, 1, 2, 1, 0):
+        x.copy_(xs[k])
+        d.copy_(ds[k])
+        graph.replay()
+        eager = both(xs[k], ds[k])
+        torch.cuda.synchronize()
+        for a, b, c in zip(out, want[k], eager):
+            assert torch.equal(a, b) and torch.equal(c, b)
+    s, t = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        torch.cuda._sleep(10_000_000)
+        late = both(xs[1].clone(), ds[1].clone())
+    with torch.cuda.stream(t):
+        other = both(xs[2], ds[2])
+    torch.cuda.synchronize()
+    for a, b in zip(late + other, want[1] + want[2]):
+        assert torch.equal(a, b)
