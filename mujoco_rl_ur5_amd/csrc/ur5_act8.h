@@ -7,11 +7,12 @@ namespace ur5act8 {
 using ur5policy::load8; using ur5policy::store8; using ur5policy::widen; using ur5policy::narrow; using ur5policy::lanes_sum;
 using ur5policy::f32_t; using ur5policy::f16_t; using ur5policy::bf16_t; using ur5policy::yes; using ur5policy::no;
 
-constexpr int GROUP = 64, THREADS = 256, LANES = 8;   // 8 lanes of 8 neighbouring values per group
+constexpr int GROUP = 64, THREADS = 256;
 constexpr float ZERO_BELOW = 1e-30f;
 constexpr float MOST_SCALE = 0x1.020406p+121f;            // the largest fp32 s with a finite 127 s: a group of fp32's largest values stays finite
 
-// ---- pack: reads each value once, writes a byte and 1/16 of a scale's byte for it; bound by the reads.
+// ---- pack and unpack move 4 (2) + 1.06 bytes per value and are bound by them: 164 M fp32 values, one MI355X, 130 + 122 us, 6.6 TB/s (with lanes of 8 values, plain accesses:
+// 168 + 150).
 // code = the integer nearest to x / s, exactly: the quotient by a reciprocal is right to 1e-4, so the code is floor or floor + 1 of it, and the sign of
 // fma(-(floor + 1/2), s, x) -- one rounding, never through zero -- says which.
 __device__ __forceinline__ int nearest_code(float x, float s, float per) {
@@ -19,40 +20,81 @@ __device__ __forceinline__ int nearest_code(float x, float s, float per) {
   const int c = (int)f;
   return c + (over > 0.f || (over == 0.f && (c & 1)));
 }
+// A lane holds as many neighbouring values as a 16-byte load brings, so that a wavefront's load or store is one run of memory; each thread has two groups under way.
+template <typename T> struct Lane {
+  static constexpr int PER = 16 / sizeof(typename T::raw), LANES = GROUP / PER, GROUPS = 2 * THREADS / LANES;   // values per lane, lanes per group, groups per workgroup
+};
+__device__ __forceinline__ void take(f32_t, const float* p, float* v) {
+  const ur5policy::F4 a = __builtin_nontemporal_load((const ur5policy::F4*)p);     // read once
+#pragma unroll
+  for (int i = 0; i < 4; i++) v[i] = a[i];
+}
+template <typename T> __device__ __forceinline__ void take(T tag, const uint16_t* p, float* v) { ur5policy::unpack8(ur5policy::fetch8_last<T>(p), v); }
+template <typename Past> __device__ __forceinline__ void put(f32_t, float* p, const float* v, Past past) {
+  ur5policy::F4 a;
+#pragma unroll
+  for (int i = 0; i < 4; i++) a[i] = v[i];
+  ur5policy::put((ur5policy::F4*)p, a, past);
+}
+template <typename T, typename Past> __device__ __forceinline__ void put(T tag, uint16_t* p, const float* v, Past past) { store8(tag, p, v, past); }
+
 template <typename T> __global__ void __launch_bounds__(THREADS) ur5_act8_pack(const typename T::raw* x, unsigned groups, unsigned total, long long size, int8_t* codes, float* scales) {
-  const unsigned g = blockIdx.x * (THREADS / LANES) + threadIdx.x / LANES, lane = threadIdx.x % LANES;
-  if (g >= total) return;                                     // all 8 lanes of a group leave together
-  const unsigned plane = g / groups, at = (g - plane * groups) * GROUP + lane * 8;
-  const auto* p = x + plane * size + at;
-  float v[8];
-  if (at + 8 <= size) load8(T{}, p, v);
-  else for (int i = 0; i < 8; i++) v[i] = at + i < size ? widen(T{}, p[i]) : 0.f;
-  uint32_t most = 0;                                          // magnitudes compare as integers, a NaN above everything
+  using L = Lane<T>;
+  const unsigned lane = threadIdx.x % L::LANES;
+  float v[2][L::PER];
 #pragma unroll
-  for (int i = 0; i < 8; i++) most = max(most, __float_as_uint(v[i]) & 0x7fffffffu);
-  for (int o = LANES / 2; o; o >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, o));
-  const float amax = __uint_as_float(most);
-  const bool finite = most < 0x7f800000u, some = finite && amax >= ZERO_BELOW;
-  const float s = some ? fminf(amax / 127.f, MOST_SCALE) : finite ? 0.f : NAN, per = some ? __builtin_amdgcn_rcpf(s) : 0.f;
-  uint64_t c = 0;
+  for (int k = 0; k < 2; k++) {
+    const unsigned g = blockIdx.x * L::GROUPS + k * (L::GROUPS / 2) + threadIdx.x / L::LANES, plane = g / groups, at = (g - plane * groups) * GROUP + lane * L::PER;
+    const auto* p = x + plane * size + at;
+    if (g < total && at + L::PER <= size) take(T{}, p, v[k]);
+    else for (int i = 0; i < L::PER; i++) v[k][i] = g < total && at + i < size ? widen(T{}, p[i]) : 0.f;
+  }
 #pragma unroll
-  for (int i = 0; i < 8; i++) c |= (uint64_t)(uint8_t)(some ? nearest_code(v[i], s, per) : 0) << (8 * i);
-  *(uint64_t*)(codes + (size_t)g * GROUP + lane * 8) = c;
-  if (lane == 0) scales[g] = s;
+  for (int k = 0; k < 2; k++) {
+    const unsigned g = blockIdx.x * L::GROUPS + k * (L::GROUPS / 2) + threadIdx.x / L::LANES;
+    if (g >= total) return;                                   // all lanes of a group leave together
+    uint32_t most = 0;                                        // magnitudes compare as integers, a NaN above everything
+#pragma unroll
+    for (int i = 0; i < L::PER; i++) most = max(most, __float_as_uint(v[k][i]) & 0x7fffffffu);
+    for (int o = L::LANES / 2; o; o >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, o));
+    const float amax = __uint_as_float(most);
+    const bool finite = most < 0x7f800000u, some = finite && amax >= ZERO_BELOW;
+    const float s = some ? fminf(amax / 127.f, MOST_SCALE) : finite ? 0.f : NAN, per = some ? __builtin_amdgcn_rcpf(s) : 0.f;
+    uint32_t c[L::PER / 4] = {};
+#pragma unroll
+    for (int i = 0; i < L::PER; i++) c[i / 4] |= (uint32_t)(uint8_t)(some ? nearest_code(v[k][i], s, per) : 0) << (8 * (i % 4));
+    int8_t* to = codes + (size_t)g * GROUP + lane * L::PER;
+    if (L::PER == 4) *(uint32_t*)to = c[0];
+    else *(uint2*)to = uint2{c[0], c[L::PER / 4 - 1]};
+    if (lane == 0) scales[g] = s;
+  }
 }
 
-template <typename T> __global__ void __launch_bounds__(THREADS) ur5_act8_unpack(const int8_t* codes, const float* scales, unsigned groups, unsigned total, long long size, typename T::raw* x) {
-  const unsigned g = blockIdx.x * (THREADS / LANES) + threadIdx.x / LANES, lane = threadIdx.x % LANES;
-  if (g >= total) return;
-  const unsigned plane = g / groups, at = (g - plane * groups) * GROUP + lane * 8;
-  const uint64_t c = *(const uint64_t*)(codes + (size_t)g * GROUP + lane * 8);
-  const float s = scales[g];
-  float v[8];
+template <typename T, typename Past> __global__ void __launch_bounds__(THREADS) ur5_act8_unpack(const int8_t* codes, const float* scales, unsigned groups, unsigned total, long long size, typename T::raw* x) {
+  using L = Lane<T>;
+  const unsigned lane = threadIdx.x % L::LANES;
+  uint2 c[2];
+  float s[2];
 #pragma unroll
-  for (int i = 0; i < 8; i++) v[i] = (float)(int8_t)(c >> (8 * i)) * s;
-  auto* p = x + plane * size + at;
-  if (at + 8 <= size) store8(T{}, p, v);
-  else for (int i = 0; i < 8; i++) if (at + i < size) p[i] = narrow(T{}, v[i]);
+  for (int k = 0; k < 2; k++) {
+    const unsigned g = min(blockIdx.x * L::GROUPS + k * (L::GROUPS / 2) + threadIdx.x / (unsigned)L::LANES, total - 1);
+    const int8_t* from = codes + (size_t)g * GROUP + lane * L::PER;
+    if (L::PER == 4) c[k].x = *(const uint32_t*)from;
+    else c[k] = *(const uint2*)from;
+    s[k] = scales[g];
+  }
+#pragma unroll
+  for (int k = 0; k < 2; k++) {
+    const unsigned g = blockIdx.x * L::GROUPS + k * (L::GROUPS / 2) + threadIdx.x / L::LANES;
+    if (g >= total) return;
+    const unsigned plane = g / groups, at = (g - plane * groups) * GROUP + lane * L::PER;
+    float v[L::PER];
+#pragma unroll
+    for (int i = 0; i < L::PER; i++) v[i] = (float)(int8_t)((i < 4 ? c[k].x : c[k].y) >> (8 * (i % 4))) * s[k];
+    auto* p = x + plane * size + at;
+    if (at + L::PER <= size) put(T{}, p, v, Past{});
+    else for (int i = 0; i < L::PER; i++) if (at + i < size) p[i] = narrow(T{}, v[i]);
+  }
 }
 
 // ---- weight gradient: dw[o][c] = sum over (image, pixel) of dy[o] x[c], a matrix product whose long axis is the pixels (both operands have them neighbouring).

@@ -52,11 +52,23 @@ __device__ __forceinline__ float narrow(f32_t, float v) { return v; }
 __device__ __forceinline__ uint16_t narrow(f16_t, float v) { return __builtin_bit_cast(uint16_t, (_Float16)v); }
 __device__ __forceinline__ uint16_t narrow(bf16_t, float v) { return __builtin_bit_cast(uint16_t, (__bf16)v); }   // to nearest, ties to even
 
+// Non-temporal accesses. Logits at their last use need not stay in the caches. What is written goes past them (`past`) only in calls over more memory than the 256 MB cache
+// holds: its reader would not find it there anyway, and it would push out what this kernel still reads; a small result stays for its reader. (The gradient of 513 bf16 rows
+// with plain stores 194 us a call, past the caches 171, with last reads too 161.) A lane's 8 fp32 logits are two loads of half a sector each: their line has to stay until the
+// second (323 fp32 rows: 117 us, with such reads 127).
+constexpr int64_t CACHE_BYTES = 256ll << 20;
+__device__ __forceinline__ void put(F4* p, F4 v, yes) { __builtin_nontemporal_store(v, p); }
+__device__ __forceinline__ void put(F4* p, F4 v, no) { *p = v; }
+__device__ __forceinline__ void put(U4* p, U4 v, yes) { __builtin_nontemporal_store(v, p); }
+__device__ __forceinline__ void put(U4* p, U4 v, no) { *p = v; }
+
 // 8 values as they lie in memory: what is loaded ahead of its use
 template <typename T> struct Eight { U4 w; };
 template <> struct Eight<f32_t> { F4 a, b; };
 template <typename T> __device__ __forceinline__ Eight<T> fetch8(const typename T::raw* p) { return Eight<T>{*(const U4*)p}; }
 template <> __device__ __forceinline__ Eight<f32_t> fetch8<f32_t>(const float* p) { return Eight<f32_t>{*(const F4*)p, *(const F4*)(p + 4)}; }
+template <typename T> __device__ __forceinline__ Eight<T> fetch8_last(const typename T::raw* p) { return Eight<T>{__builtin_nontemporal_load((const U4*)p)}; }
+template <> __device__ __forceinline__ Eight<f32_t> fetch8_last<f32_t>(const float* p) { return fetch8<f32_t>(p); }
 __device__ __forceinline__ void unpack8(const Eight<f32_t>& e, float* v) {
 #pragma unroll
   for (int i = 0; i < 4; i++) { v[i] = e.a[i]; v[4 + i] = e.b[i]; }
@@ -66,17 +78,18 @@ template <typename T> __device__ __forceinline__ void unpack8(const Eight<T>& e,
   for (int i = 0; i < 4; i++) { v[2 * i] = widen(T{}, (uint16_t)e.w[i]); v[2 * i + 1] = widen(T{}, (uint16_t)(e.w[i] >> 16)); }
 }
 template <typename T> __device__ __forceinline__ void load8(T, const typename T::raw* p, float* v) { unpack8(fetch8<T>(p), v); }
-__device__ __forceinline__ void store8(f32_t, float* p, const float* v) {
+template <typename Past> __device__ __forceinline__ void store8(f32_t, float* p, const float* v, Past past) {
   F4 a, b;
 #pragma unroll
   for (int i = 0; i < 4; i++) { a[i] = v[i]; b[i] = v[4 + i]; }
-  *(F4*)p = a; *(F4*)(p + 4) = b;
+  put((F4*)p, a, past);
+  put((F4*)(p + 4), b, past);
 }
-template <typename T> __device__ __forceinline__ void store8(T tag, uint16_t* p, const float* v) {
+template <typename T, typename Past> __device__ __forceinline__ void store8(T tag, uint16_t* p, const float* v, Past past) {
   U4 a;
 #pragma unroll
   for (int i = 0; i < 4; i++) a[i] = (uint32_t)narrow(tag, v[2 * i]) | (uint32_t)narrow(tag, v[2 * i + 1]) << 16;
-  *(U4*)p = a;
+  put((U4*)p, a, past);
 }
 
 // 8 values from p on, of which the first `left` exist
@@ -84,8 +97,8 @@ template <typename T> __device__ __forceinline__ void take8(const typename T::ra
 #pragma unroll
   for (int i = 0; i < VEC; i++) v[i] = i < left ? widen(T{}, p[i]) : -INFINITY;
 }
-template <typename T> __device__ __forceinline__ void put8(typename T::raw* p, int left, bool whole, const float* v) {
-  if (whole) { store8(T{}, p, v); return; }
+template <typename T, typename Past> __device__ __forceinline__ void put8(typename T::raw* p, int left, bool whole, const float* v, Past past) {
+  if (whole) { store8(T{}, p, v, past); return; }
 #pragma unroll
   for (int i = 0; i < VEC; i++) if (i < left) p[i] = narrow(T{}, v[i]);
 }
@@ -324,7 +337,8 @@ __device__ __forceinline__ Sums join_workgroup(const Running& r, bool ref, bool 
 // ---- statistics of the pieces of rows
 template <typename T, bool REF> struct Both {       // 8 logits, and the reference's
   Eight<T> z, q;
-  __device__ __forceinline__ Both(const typename T::raw* z_row, const typename T::raw* q_row, int j) : z(fetch8<T>(z_row + j)) { if (REF) q = fetch8<T>(q_row + j); }
+  __device__ __forceinline__ Both(const typename T::raw* z_row, const typename T::raw* q_row, int j, no) : z(fetch8<T>(z_row + j)) { if (REF) q = fetch8<T>(q_row + j); }
+  __device__ __forceinline__ Both(const typename T::raw* z_row, const typename T::raw* q_row, int j, yes) : z(fetch8_last<T>(z_row + j)) { if (REF) q = fetch8_last<T>(q_row + j); }
   __device__ __forceinline__ void get(float* a, float* b) const { unpack8(z, a); if (REF) unpack8(q, b); }
 };
 template <typename T, bool MASK, bool REF, bool ENTROPY> __device__ __forceinline__ Sums piece_sums(const Rows& R, int row, int piece) {
@@ -336,7 +350,7 @@ template <typename T, bool MASK, bool REF, bool ENTROPY> __device__ __forceinlin
     if (MASK) { bar8(allowed, z); if (REF) bar8(allowed, q); }
     add8<REF, ENTROPY>(a, z, q, e);
   };
-  for_piece<MASK>(R, row, piece, [&](int j) { return Both<T, REF>(z_row, q_row, j); },
+  for_piece<MASK>(R, row, piece, [&](int j) { return Both<T, REF>(z_row, q_row, j, no{}); },
     [&](int, uint32_t allowed, const Both<T, REF>& b) { float z[VEC], q[VEC]; b.get(z, q); add(allowed, z, q); },
     [&](int j, uint32_t allowed, int left) { float z[VEC], q[VEC]; take8<T>(z_row + j, left, z); if (REF) take8<T>(q_row + j, left, q); add(allowed, z, q); },
     [](const Piece&, int) {});
@@ -409,7 +423,8 @@ __device__ __forceinline__ void add_terms(const Terms& t) {
 // (a translation unit of its own kind: also launched alone, by a forward pass without a gradient)
 static __global__ void __launch_bounds__(THREADS) ur5_policy_loss(Terms t) { add_terms(t); }
 constexpr int FIRST = 8;             // workgroups before the pieces, as in the statistics; the first of them writes the loss if t.loss
-template <typename T, bool MASK, bool REF> __global__ void __launch_bounds__(THREADS) ur5_policy_grad(Rows R, Terms t, const int64_t* action, const Slope* slopes, float scale, const float* upstream, void* grad) {
+template <typename T, bool MASK, bool REF, typename Past> __global__ void __launch_bounds__(THREADS) ur5_policy_grad(Rows R, Terms t, const int64_t* action, const Slope* slopes, float scale, const float* upstream, void* grad) {
+  constexpr Past past;
   const int block = (int)blockIdx.x - FIRST;
   if (block < 0) {
     if (t.loss && blockIdx.x == 0) add_terms(t);
@@ -421,7 +436,7 @@ template <typename T, bool MASK, bool REF> __global__ void __launch_bounds__(THR
   const float zero[VEC] = {};
   const auto clear = [&](const Piece& P, int g) {          // 8 pixels of all maps of the piece
     const int p = P.first + g * VEC, left = R.pixels - p;
-    for (int m = 0; m < P.maps; m++) put8<T>(out + (P.map0 + m) * R.pixels + p, left, left >= VEC, zero);
+    for (int m = 0; m < P.maps; m++) put8<T>(out + (P.map0 + m) * R.pixels + p, left, left >= VEC, zero, past);
   };
   if (!S.on) {                                             // zeros; the logits are not read
     const Piece P = piece_of(R, piece);
@@ -446,14 +461,14 @@ template <typename T, bool MASK, bool REF> __global__ void __launch_bounds__(THR
 #pragma unroll
       for (int i = 0; i < VEC; i++) g[i] += a - j == i ? S.take : 0.f;
   };
-  for_piece<MASK>(R, row, piece, [&](int j) { return Both<T, REF>(z_row, q_row, j); },
-    [&](int j, uint32_t allowed, const Both<T, REF>& b) { float z[VEC], q[VEC], g[VEC]; b.get(z, q); slope(j, allowed, z, q, g); store8(T{}, out + j, g); },
+  for_piece<MASK>(R, row, piece, [&](int j) { return Both<T, REF>(z_row, q_row, j, yes{}); },
+    [&](int j, uint32_t allowed, const Both<T, REF>& b) { float z[VEC], q[VEC], g[VEC]; b.get(z, q); slope(j, allowed, z, q, g); store8(T{}, out + j, g, past); },
     [&](int j, uint32_t allowed, int left) {
       float z[VEC], q[VEC], g[VEC];
       take8<T>(z_row + j, left, z);
       if (REF) take8<T>(q_row + j, left, q);
       slope(j, allowed, z, q, g);
-      put8<T>(out + j, left, false, g);
+      put8<T>(out + j, left, false, g, past);
     }, clear);
 }
 

@@ -131,9 +131,10 @@ void prefer_pairs(const Rows& R, int dtype, hipStream_t s, const Prefer& P, cons
 }
 void gradient(Rows R, int dtype, hipStream_t s, const Terms& t, const int64_t* action, const Work& w, float scale, const float* upstream, void* grad) {
   cut(R.rows, R.actions, R.mask ? R.pixels : 0, GRADIENT, &R);      // it leaves no records
-  by_type(dtype, [&](auto k) { by_flag(R.mask, [&](auto m) { by_flag(R.ref, [&](auto q) {
-    ur5_policy_grad<decltype(k), decltype(m)::value, decltype(q)::value><<<FIRST + R.rows * R.pieces, THREADS, 0, s>>>(R, t, action, w.slopes, scale, upstream, grad);
-  }); }); });
+  const bool past = (int64_t)R.rows * R.actions * (dtype == UR5_F32 ? 4 : 2) * (R.ref ? 3 : 2) > CACHE_BYTES;
+  by_type(dtype, [&](auto k) { by_flag(R.mask, [&](auto m) { by_flag(R.ref, [&](auto q) { by_flag(past, [&](auto p) {
+    ur5_policy_grad<decltype(k), decltype(m)::value, decltype(q)::value, decltype(p)><<<FIRST + R.rows * R.pieces, THREADS, 0, s>>>(R, t, action, w.slopes, scale, upstream, grad);
+  }); }); }); });
 }
 }  // namespace
 
@@ -256,9 +257,10 @@ int ur5_act8_pack(const void* x, int dtype, int64_t planes, int64_t size, int8_t
   if (!planes) return 0;
   if (!x || !codes || !scales || !aligned16(codes)) return fail(UR5_ERR_ARG, __func__, "x, codes (16-byte aligned) and scales are needed");
   ON(device);
-  const unsigned groups = (unsigned)((size + ur5act8::GROUP - 1) / ur5act8::GROUP), total = (unsigned)(planes * groups), per = ur5act8::THREADS / ur5act8::LANES;
+  const unsigned groups = (unsigned)((size + ur5act8::GROUP - 1) / ur5act8::GROUP), total = (unsigned)(planes * groups);
   by_type(dtype, [&](auto t) {
     using T = decltype(t);
+    constexpr unsigned per = ur5act8::Lane<T>::GROUPS;
     ur5act8::ur5_act8_pack<T><<<(total + per - 1) / per, ur5act8::THREADS, 0, (hipStream_t)stream>>>((const typename T::raw*)x, groups, total, size, codes, scales);
   });
   return launched(__func__);
@@ -268,10 +270,13 @@ int ur5_act8_unpack(const int8_t* codes, const float* scales, int64_t planes, in
   if (!planes) return 0;
   if (!x || !codes || !scales || !aligned16(codes)) return fail(UR5_ERR_ARG, __func__, "x, codes (16-byte aligned) and scales are needed");
   ON(device);
-  const unsigned groups = (unsigned)((size + ur5act8::GROUP - 1) / ur5act8::GROUP), total = (unsigned)(planes * groups), per = ur5act8::THREADS / ur5act8::LANES;
+  const unsigned groups = (unsigned)((size + ur5act8::GROUP - 1) / ur5act8::GROUP), total = (unsigned)(planes * groups);
   by_type(dtype, [&](auto t) {
     using T = decltype(t);
-    ur5act8::ur5_act8_unpack<T><<<(total + per - 1) / per, ur5act8::THREADS, 0, (hipStream_t)stream>>>(codes, scales, groups, total, size, (typename T::raw*)x);
+    constexpr unsigned per = ur5act8::Lane<T>::GROUPS;
+    by_flag(planes * size * (int64_t)(sizeof(typename T::raw) + 1) > CACHE_BYTES, [&](auto p) {
+      ur5act8::ur5_act8_unpack<T, decltype(p)><<<(total + per - 1) / per, ur5act8::THREADS, 0, (hipStream_t)stream>>>(codes, scales, groups, total, size, (typename T::raw*)x);
+    });
   });
   return launched(__func__);
 }
