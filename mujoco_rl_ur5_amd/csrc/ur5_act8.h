@@ -11,8 +11,8 @@ constexpr int GROUP = 64, THREADS = 256;
 constexpr float ZERO_BELOW = 1e-30f;
 constexpr float MOST_SCALE = 0x1.020406p+121f;            // the largest fp32 s with a finite 127 s: a group of fp32's largest values stays finite
 
-// ---- pack and unpack move 4 (2) + 1.06 bytes per value and are bound by them: 164 M fp32 values, one MI355X, 130 + 122 us, 6.6 TB/s (with lanes of 8 values, plain accesses:
-// 168 + 150).
+// ---- pack and unpack move 4 (2) + 1.06 bytes per value and are bound by them: 164 M fp32 values, one MI355X, 133 + 113 us, 6.3 and 7.4 TB/s (with 8 fp32 values per lane,
+// so that a wavefront's 16-byte loads skip every second 16 bytes, and plain accesses: 168 + 150).
 // code = the integer nearest to x / s, exactly: the quotient by a reciprocal is right to 1e-4, so the code is floor or floor + 1 of it, and the sign of
 // fma(-(floor + 1/2), s, x) -- one rounding, never through zero -- says which.
 __device__ __forceinline__ int nearest_code(float x, float s, float per) {
@@ -38,46 +38,81 @@ template <typename Past> __device__ __forceinline__ void put(f32_t, float* p, co
 }
 template <typename T, typename Past> __device__ __forceinline__ void put(T tag, uint16_t* p, const float* v, Past past) { store8(tag, p, v, past); }
 
+// where this thread's two groups lie: group, first value of the lane, and how many of the lane's values exist (0: no such group)
+struct Where { unsigned g; long long at; int left; };
+template <typename T> __device__ __forceinline__ void locate(unsigned groups, unsigned total, long long size, Where* w) {
+  using L = Lane<T>;
+  const unsigned lane = threadIdx.x % L::LANES, g = blockIdx.x * L::GROUPS + threadIdx.x / L::LANES;
+  if (size == (long long)groups * GROUP) {                    // planes of whole groups lie like one
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+      w[k].g = g + k * (L::GROUPS / 2);
+      w[k].at = (long long)w[k].g * GROUP + lane * L::PER;
+      w[k].left = w[k].g < total ? L::PER : 0;
+    }
+    return;
+  }
+  unsigned plane = g / groups, at = g - plane * groups;
+#pragma unroll
+  for (int k = 0; k < 2; k++) {
+    w[k].g = g + k * (L::GROUPS / 2);
+    if (k) for (at += L::GROUPS / 2; at >= groups; at -= groups) plane++;
+    const long long first = (long long)at * GROUP + lane * L::PER;
+    w[k].at = plane * size + first;
+    w[k].left = w[k].g < total ? (int)min((long long)L::PER, max(0ll, size - first)) : 0;
+  }
+}
+// the largest of the lanes of a group, in all of them
+template <int LANES> __device__ __forceinline__ uint32_t group_max(uint32_t v) {
+  using ur5policy::dpp;
+  v = max(v, (uint32_t)dpp<0xB1>((int)v));
+  v = max(v, (uint32_t)dpp<0x4E>((int)v));
+  v = max(v, (uint32_t)dpp<0x141>((int)v));
+  return LANES == 16 ? max(v, (uint32_t)dpp<0x140>((int)v)) : v;
+}
 template <typename T> __global__ void __launch_bounds__(THREADS) ur5_act8_pack(const typename T::raw* x, unsigned groups, unsigned total, long long size, int8_t* codes, float* scales) {
   using L = Lane<T>;
   const unsigned lane = threadIdx.x % L::LANES;
+  Where w[2];
+  locate<T>(groups, total, size, w);
   float v[2][L::PER];
 #pragma unroll
   for (int k = 0; k < 2; k++) {
-    const unsigned g = blockIdx.x * L::GROUPS + k * (L::GROUPS / 2) + threadIdx.x / L::LANES, plane = g / groups, at = (g - plane * groups) * GROUP + lane * L::PER;
-    const auto* p = x + plane * size + at;
-    if (g < total && at + L::PER <= size) take(T{}, p, v[k]);
-    else for (int i = 0; i < L::PER; i++) v[k][i] = g < total && at + i < size ? widen(T{}, p[i]) : 0.f;
+    if (w[k].left == L::PER) take(T{}, x + w[k].at, v[k]);
+    else for (int i = 0; i < L::PER; i++) v[k][i] = i < w[k].left ? widen(T{}, x[w[k].at + i]) : 0.f;
   }
 #pragma unroll
   for (int k = 0; k < 2; k++) {
-    const unsigned g = blockIdx.x * L::GROUPS + k * (L::GROUPS / 2) + threadIdx.x / L::LANES;
-    if (g >= total) return;                                   // all lanes of a group leave together
     uint32_t most = 0;                                        // magnitudes compare as integers, a NaN above everything
 #pragma unroll
     for (int i = 0; i < L::PER; i++) most = max(most, __float_as_uint(v[k][i]) & 0x7fffffffu);
-    for (int o = L::LANES / 2; o; o >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, o));
+    most = group_max<L::LANES>(most);
     const float amax = __uint_as_float(most);
     const bool finite = most < 0x7f800000u, some = finite && amax >= ZERO_BELOW;
     const float s = some ? fminf(amax / 127.f, MOST_SCALE) : finite ? 0.f : NAN, per = some ? __builtin_amdgcn_rcpf(s) : 0.f;
+    if (w[k].g >= total) return;                              // all lanes of a group leave together
     uint32_t c[L::PER / 4] = {};
+    if (some) {
 #pragma unroll
-    for (int i = 0; i < L::PER; i++) c[i / 4] |= (uint32_t)(uint8_t)(some ? nearest_code(v[k][i], s, per) : 0) << (8 * (i % 4));
-    int8_t* to = codes + (size_t)g * GROUP + lane * L::PER;
+      for (int i = 0; i < L::PER; i++) c[i / 4] |= (uint32_t)(uint8_t)nearest_code(v[k][i], s, per) << (8 * (i % 4));
+    }
+    int8_t* to = codes + (size_t)w[k].g * GROUP + lane * L::PER;
     if (L::PER == 4) *(uint32_t*)to = c[0];
     else *(uint2*)to = uint2{c[0], c[L::PER / 4 - 1]};
-    if (lane == 0) scales[g] = s;
+    if (lane == 0) scales[w[k].g] = s;
   }
 }
 
 template <typename T, typename Past> __global__ void __launch_bounds__(THREADS) ur5_act8_unpack(const int8_t* codes, const float* scales, unsigned groups, unsigned total, long long size, typename T::raw* x) {
   using L = Lane<T>;
   const unsigned lane = threadIdx.x % L::LANES;
+  Where w[2];
+  locate<T>(groups, total, size, w);
   uint2 c[2];
   float s[2];
 #pragma unroll
   for (int k = 0; k < 2; k++) {
-    const unsigned g = min(blockIdx.x * L::GROUPS + k * (L::GROUPS / 2) + threadIdx.x / (unsigned)L::LANES, total - 1);
+    const unsigned g = min(w[k].g, total - 1);
     const int8_t* from = codes + (size_t)g * GROUP + lane * L::PER;
     if (L::PER == 4) c[k].x = *(const uint32_t*)from;
     else c[k] = *(const uint2*)from;
@@ -85,15 +120,12 @@ template <typename T, typename Past> __global__ void __launch_bounds__(THREADS) 
   }
 #pragma unroll
   for (int k = 0; k < 2; k++) {
-    const unsigned g = blockIdx.x * L::GROUPS + k * (L::GROUPS / 2) + threadIdx.x / L::LANES;
-    if (g >= total) return;
-    const unsigned plane = g / groups, at = (g - plane * groups) * GROUP + lane * L::PER;
     float v[L::PER];
 #pragma unroll
     for (int i = 0; i < L::PER; i++) v[i] = (float)(int8_t)((i < 4 ? c[k].x : c[k].y) >> (8 * (i % 4))) * s[k];
-    auto* p = x + plane * size + at;
-    if (at + L::PER <= size) put(T{}, p, v, Past{});
-    else for (int i = 0; i < L::PER; i++) if (at + i < size) p[i] = narrow(T{}, v[i]);
+    auto* p = x + w[k].at;
+    if (w[k].left == L::PER) put(T{}, p, v, Past{});
+    else for (int i = 0; i < L::PER; i++) if (i < w[k].left) p[i] = narrow(T{}, v[i]);
   }
 }
 
