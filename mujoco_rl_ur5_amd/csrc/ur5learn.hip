@@ -39,11 +39,12 @@ int no_device(const char* entry, hipError_t e) {
 // ---- how rows are cut. Pieces grow from one turn of 256 threads first over the maps, which share a list of allowed pixels, then along the pixels, up to 64 turns, so that a
 // thread's fp32 sums stay short (512 terms); images of less than 2048 pixels take as many maps as fill a workgroup. How many pieces a call aims at: more fill the card's 256 CUs
 // (8 workgroups each) more evenly, fewer share what a piece costs before and after its loads. us of the kernel at 2048 / 4096 / 8192 / 16384 pieces wanted:
-// sample (512 fp32 rows) 103 / 106 / 126 / 169, logp (2000 x 40 000 bf16) 45 / 37 / 39 / 49, statistics (513 bf16 rows) 106 / 100 / 94 / 103, gradient 131 / 110 / 102 / 98.
-// A row of few turns is one piece of the calls that end with it: their second launch costs 3 us more than 5 turns (12 rows of 6 x 40 x 40, us a call: logp 13.6 -> 10.7, sample
+// sample (512 fp32 rows) 103 / 101 / 114 / 157, logp (2000 x 40 000 bf16) 45 / 36 / 38 / 47, statistics (513 bf16 rows) 70 / 66 / 75 / 99, gradient 123 / 113 / 103 / 90, at
+// 24576 89, at 32768 123 (259 fp32 rows: 78, 73, 75).
+// A row of few turns is one piece of the calls that end with it: their second launch costs 3 us more than 5 turns (12 rows of 6 x 40 x 40, us a call: logp 14.4 -> 11.6, sample
 // 13.9 -> 11.8; of 11 turns: logp 13.7 -> 10.7, sample 14.0 -> 17.7).
 struct Aim { int64_t pieces, whole; };
-constexpr Aim SAMPLE{4096, 6}, LOGP{4096, 10}, LOSS{8192, 0}, GRADIENT{16384, 0};
+constexpr Aim SAMPLE{4096, 6}, LOGP{4096, 10}, LOSS{4096, 0}, GRADIENT{24576, 0};
 constexpr int64_t MOST_TURNS = 64;
 int64_t clamp(int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : v > hi ? hi : v; }
 void cut(int64_t rows, int64_t actions, int64_t mask_len, const Aim& aim, Rows* R) {
@@ -282,7 +283,9 @@ int ur5_act8_unpack(const int8_t* codes, const float* scales, int64_t planes, in
 }
 
 // ---- weight gradient: how the work is split. Tiles of 128 output x 256 input channels (of half the outputs, and of half or a quarter of the inputs where there are no more),
-// and as many ranges of the pixels as give every CU a workgroup (two of the smaller ones): less than 8, or a multiple of 8, one set per XCD.
+// and as many ranges of the pixels as give every CU a workgroup (two of the smaller ones): less than 8, or a multiple of 8, one set per XCD. A larger tile reads and converts
+// each operand less often: 256 -> 512 channels 183 us with 128 x 256, 229 with 128 x 128, 233 with 64 x 256. One that reaches past the channels multiplies for nothing: 64 -> 128
+// channels 22 us with 128 x 64, 36 with 128 x 256.
 constexpr int64_t WORKGROUPS = 256;
 struct WgradPlan { int to, tc, o_tiles, c_tiles, splits; int64_t part, bytes; };
 static WgradPlan wgrad_plan(int64_t n, int64_t cin, int64_t cout, int64_t size) {
