@@ -9,7 +9,8 @@
  * Rows of logits: `rows` rows of `actions` logits (dtype UR5_F32 / UR5_F16 / UR5_BF16), neighbouring in memory within a row, `stride` elements from row to row. mask (NULL:
  * everything is allowed): one byte per pixel, non-zero = allowed, mask_len bytes per row (a divisor of actions: action j uses byte j % mask_len), mask_stride bytes from
  * row to row (0: one mask for all). Logits (and reference logits) of actions that are not allowed may hold anything. A logit of -inf is an action of probability 0;
- * NaN or +inf in an allowed place make the row's results NaN. A row COUNTS if its action lies in [0, actions), is allowed and has a logit above -inf. */
+ * NaN or +inf in an allowed place make the row's results NaN. A row COUNTS if its action lies in [0, actions), is allowed and has a logit above -inf. Less than 2^24 rows and
+ * pairs, and rows of which a call makes less than 2^24 workgroups. */
 #ifndef UR5LEARN_H
 #define UR5LEARN_H
 #include "ur5sim.h"
@@ -49,7 +50,7 @@ typedef struct ur5_clip {
   const float* upstream;         /* another one, on the device; NULL: 1 */
 } ur5_clip;
 /* loss[1] = mean over the rows that count of -min(r A, clip(r) A) + kl_coef KL(row || ref) - entropy_coef H(row), r = exp(logp - old_logp); logp, kl, entropy [rows] (0 in rows
-   that do not count). No counting row: 0. */
+   that do not count). No counting row: 0. KL is +inf where the reference gives probability 0 to an action whose own is above 0 in 32 bits; without a kl_coef it is only reported. */
 int ur5_policy_clip_loss(const ur5_rows* r, const ur5_clip* c, float* loss, float* logp, float* kl, float* entropy);
 /* grad [rows][actions] (dense, dtype of the logits) of the loss times grad_scale times *upstream, from the workspace that clip_loss left; rows that do not count get 0. */
 int ur5_policy_clip_grad(const ur5_rows* r, const ur5_clip* c, void* grad);

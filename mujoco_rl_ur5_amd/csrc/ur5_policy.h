@@ -265,6 +265,9 @@ __device__ __forceinline__ double noisy_score(float z, uint64_t key, int j) {
 }
 __device__ __forceinline__ bool better(double s, int i, double than, int at) { return s > than || (s == than && i < at); }
 
+// a sum times the factor of a new maximum: a KL sum that met a reference of probability 0 is infinite, and stays out where its share of the row vanishes
+template <typename S> __device__ __forceinline__ S scaled(S sum, S f) { return f > 0 ? sum * f : f; }
+
 // running sums of one thread: fp32, over at most a few hundred terms
 struct Running { float m, s, t, k, mq, sq; };
 __device__ __forceinline__ Running nothing() { return Running{LOWEST, 0, 0, 0, LOWEST, 0}; }
@@ -277,7 +280,7 @@ template <bool REF, bool ENTROPY> __device__ __forceinline__ void add8(Running& 
     const float f = shrink(a.m, m);
     if (ENTROPY) a.t = f * (a.t + a.s * fmaxf(a.m - m, -1e30f));   // an empty sum meets LOWEST - m: kept finite
     a.s *= f;
-    if (REF) a.k *= f;
+    if (REF) a.k = scaled(a.k, f);
     a.m = m;
   }
   if (REF && mq > a.mq) { a.sq *= shrink(a.mq, mq); a.mq = mq; }
@@ -286,9 +289,9 @@ template <bool REF, bool ENTROPY> __device__ __forceinline__ void add8(Running& 
     const float d = z[i] - a.m;
     e[i] = fall(d);
     a.s += e[i];
-    if (ENTROPY) a.t += e[i] * fmaxf(d, -1e4f);                   // e is 0 long before -1e4 (and before -1e30 below): 0 * -inf does not arise
+    if (ENTROPY) a.t += e[i] * fmaxf(d, -1e4f);                   // e is 0 long before -1e4: 0 * -inf does not arise
     if (REF) {
-      a.k += e[i] * fmaxf(z[i] - q[i], -1e30f);
+      a.k += e[i] * (e[i] > 0 ? z[i] - q[i] : 0.f);               // what is not allowed or too unlikely for 32 bits adds nothing, whatever q holds
       a.sq += fall(q[i] - a.mq);
     }
   }
@@ -303,7 +306,7 @@ template <int WIDTH> __device__ __forceinline__ void join_lanes(Sums& a, bool re
   if (entropy) a.t = lanes_sum<WIDTH>(f * moved(a.s, a.t, a.m, m));
   a.s = lanes_sum<WIDTH>(a.s * f);
   if (ref) {
-    a.k = lanes_sum<WIDTH>(a.k * f);
+    a.k = lanes_sum<WIDTH>(scaled(a.k, f));
     const float mq = lanes_max<WIDTH>(a.mq);
     a.sq = lanes_sum<WIDTH>(a.sq * exp((double)a.mq - mq));
     a.mq = mq;
@@ -317,7 +320,7 @@ __device__ __forceinline__ Sums join_wave(const Running& r, bool ref, bool entro
   a.s = lanes_sum((double)(r.s * f));
   if (entropy) a.t = lanes_sum((double)(f * (r.t + r.s * fmaxf(r.m - a.m, -1e30f))));
   if (ref) {
-    a.k = lanes_sum((double)(r.k * f));
+    a.k = lanes_sum((double)scaled(r.k, f));
     a.mq = lanes_max(r.mq);
     a.sq = lanes_sum((double)(r.sq * shrink(r.mq, a.mq)));
   }
@@ -366,10 +369,13 @@ struct Slope { float m, rs, c0, kl, gap, entropy, level, take; int on; };   // o
 struct Span { const int64_t* ends; int last; };   // the preference loss: rows outside [ends[0], ends[last]) belong to no episode and do not count; ends == null: all rows
 __device__ __forceinline__ bool in_span(const Span& s, int row) { return !s.ends || (row >= s.ends[0] && row < s.ends[s.last]); }
 // The pieces come after `front` workgroups (a multiple of 8, so that pieces keep their XCDs from kernel to kernel) that write which rows count, a thread each.
-template <typename T, bool MASK, bool REF> __global__ void __launch_bounds__(THREADS) ur5_policy_stats(Rows R, Span span, int front, const int64_t* action, Part* parts, Slope* slopes) {
+template <typename T, bool MASK, bool REF> __global__ void __launch_bounds__(THREADS) ur5_policy_stats(Rows R, Span span, int front, const int64_t* action, Part* parts, Slope* slopes, int* counts) {
   if ((int)blockIdx.x < front) {
     const int row = blockIdx.x * THREADS + threadIdx.x;
-    if (row < R.rows) slopes[row] = Slope{0, 0, 0, 0, 0, 0, 0, 0, in_span(span, row) && action_counts<T>(R, row, action[row])};
+    const bool on = row < R.rows && in_span(span, row) && action_counts<T>(R, row, action[row]);
+    if (row < R.rows) slopes[row] = Slope{0, 0, 0, 0, 0, 0, 0, 0, on};
+    const int n = __syncthreads_count(on);
+    if (threadIdx.x == 0 && row < R.rows) counts[blockIdx.x] = n;
     return;
   }
   const int block = (int)blockIdx.x - front, row = block / R.pieces, piece = block % R.pieces;
@@ -388,7 +394,7 @@ __device__ __forceinline__ Sums join_row(const Part* parts, int pieces, bool ref
     a.t = f * moved(a.s, a.t, a.m, m) + g * moved(p.s, p.t, p.m, m);
     a.s = f * a.s + g * p.s;
     if (ref) {
-      a.k = f * a.k + g * p.k;
+      a.k = scaled(a.k, f) + scaled(p.k, g);
       a.sq = a.sq * exp((double)a.mq - mq) + p.sq * exp((double)p.mq - mq);
     }
     a.m = m; a.mq = mq;
@@ -408,19 +414,13 @@ template <typename S> __device__ __forceinline__ S workgroup_sum(S v) {
   for (int i = 1; i < WAVES; i++) v += wave[i];
   return v;
 }
-__device__ __forceinline__ int counting_rows(const Slope* slopes, int rows) {
-  int n = 0;
-  for (int i = threadIdx.x; i < rows; i += THREADS) n += slopes[i].on;
-  return workgroup_sum(n);
-}
-// loss = sum of n terms / what they are a mean over (the rows that count, or `over`)
-struct Terms { const double* term; int n, over; const Slope* slopes; int rows; float* loss; };
+// loss = sum of n terms / what they are a mean over: *counting (the rows that count), or n without it
+struct Terms { const double* term; int n; const int* counting; float* loss; };
 __device__ __forceinline__ void add_terms(const Terms& t) {
   double sum = 0;
   for (int i = threadIdx.x; i < t.n; i += THREADS) sum += t.term[i];
   sum = workgroup_sum(sum);
-  const int over = t.over ? t.over : max(1, counting_rows(t.slopes, t.rows));
-  if (threadIdx.x == 0) *t.loss = (float)(sum / over);
+  if (threadIdx.x == 0) *t.loss = (float)(sum / max(1, t.counting ? *t.counting : t.n));
 }
 // (a forward pass without a gradient)
 static __global__ void __launch_bounds__(THREADS) ur5_policy_loss(Terms t) { add_terms(t); }
@@ -445,7 +445,7 @@ template <typename T, bool MASK, bool REF, typename Past> __global__ void __laun
     for (int g = threadIdx.x; g * VEC < P.pixels; g += THREADS) clear(P, g);
     return;
   }
-  const float factor = scale * (upstream ? *upstream : 1.f);
+  const float factor = scale * (upstream ? *upstream : 1.f) / (t.counting ? max(1, *t.counting) : 1);
   S.rs *= factor; S.take *= factor;
   const int a = (int)action[row];
   const auto* z_row = (const typename T::raw*)R.logits + row * R.stride;
@@ -477,8 +477,14 @@ template <typename T, bool MASK, bool REF, typename Past> __global__ void __laun
 // ---- clipped policy loss. Per row: ratio r = exp(logp - old), L = -min(r A, clip(r, 1 - lo, 1 + hi) A) + kl_coef KL(p || q) - entropy_coef H; the mean over the rows that count.
 struct Clip { const int64_t* action; const float* old_logp; const float* advantage; float lo, hi, kl_coef, entropy_coef; };
 // a wavefront per row. Normalisers in 64 bits: KL = k / s - (lse - lse_q) is a small difference of large numbers.
-template <typename T, bool REF> __global__ void __launch_bounds__(THREADS) ur5_policy_clip_rows(Rows R, Clip C, const Part* parts, Slope* slopes, double* term, float* logp, float* kl, float* entropy) {
-  const int n = counting_rows(slopes, R.rows), row = blockIdx.x * WAVES + (threadIdx.x >> 6);
+template <typename T, bool REF> __global__ void __launch_bounds__(THREADS) ur5_policy_clip_rows(Rows R, Clip C, const Part* parts, Slope* slopes, const int* counts, int* counting, double* term, float* logp, float* kl, float* entropy) {
+  if (blockIdx.x == 0) {
+    int n = 0;
+    for (int i = threadIdx.x; i < (R.rows + THREADS - 1) / THREADS; i += THREADS) n += counts[i];
+    n = workgroup_sum(n);
+    if (threadIdx.x == 0) *counting = n;
+  }
+  const int row = blockIdx.x * WAVES + (threadIdx.x >> 6);
   if (row >= R.rows) return;
   const bool on = slopes[row].on, writes = (threadIdx.x & 63) == 0;
   if (!on) {
@@ -492,8 +498,8 @@ template <typename T, bool REF> __global__ void __launch_bounds__(THREADS) ur5_p
   const float ratio = expf(lp - C.old_logp[row]), free = ratio * adv, held = fminf(fmaxf(ratio, 1 - C.lo), 1 + C.hi) * adv;
   const float take = held < free ? 0.f : -adv * ratio;   // the clipped branch has no slope; NaN stays
   logp[row] = lp; kl[row] = k; entropy[row] = h;
-  term[row] = -(double)(held < free ? held : free) + (REF ? (double)C.kl_coef * k : 0.0) - (double)C.entropy_coef * h;
-  slopes[row] = Slope{a.m, (float)(1 / (a.s * n)), -take, C.kl_coef, (float)(shift + k), C.entropy_coef, (float)(ls - h), take / n, 1};
+  term[row] = -(double)(held < free ? held : free) + (REF && C.kl_coef > 0 ? (double)C.kl_coef * k : 0.0) - (double)C.entropy_coef * h;   // (an infinite KL that has no weight is only reported)
+  slopes[row] = Slope{a.m, (float)(1 / a.s), -take, C.kl_coef, (float)(shift + k), C.entropy_coef, (float)(ls - h), take, 1};
 }
 
 // ---- preference loss. Episodes are runs of rows: episode k holds the rows offsets[k] .. offsets[k + 1]. S_k = sum over its counting rows of logp - ref_logp,

@@ -57,25 +57,27 @@ void cut(int64_t rows, int64_t actions, int64_t mask_len, const Aim& aim, Rows* 
   R->pieces_x = (int)((tiles + per - 1) / per);
   R->pieces = (int)(R->pieces_x * ((maps + maps_per - 1) / maps_per));
 }
-// workspace: records | slopes | terms of the loss (one per row; one per pair where there are more pairs than rows)
-struct Work { Part* parts; Slope* slopes; double* term; };
+// workspace: records | slopes | terms of the loss (one per row; one per pair where there are more pairs than rows) | rows that count, of all and of every 256
+struct Work { Part* parts; Slope* slopes; double* term; int* counting; int* counts; };
 int64_t lay_out(const Rows& R, int64_t terms, void* base, Work* w) {
   char* p = (char*)base;
-  const int64_t n = R.rows, parts = n * R.pieces * (int64_t)sizeof(Part), slopes = (n * (int64_t)sizeof(Slope) + 15) / 16 * 16;
-  if (w) *w = Work{(Part*)p, (Slope*)(p + parts), (double*)(p + parts + slopes)};
-  return parts + slopes + (terms > n ? terms : n) * 8;
+  const int64_t n = R.rows, parts = n * R.pieces * (int64_t)sizeof(Part), slopes = (n * (int64_t)sizeof(Slope) + 15) / 16 * 16, sums = (terms > n ? terms : n) * 8;
+  int* counting = (int*)(p + parts + slopes + sums);
+  if (w) *w = Work{(Part*)p, (Slope*)(p + parts), (double*)(p + parts + slopes), counting, counting + 1};
+  return parts + slopes + sums + (1 + (n + THREADS - 1) / THREADS) * 4;
 }
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 constexpr int64_t MOST = 0x7fffffff;
+constexpr int64_t MOST_LAUNCHED = (1 << 24) - 1;     // workgroups of 256 threads: a launch holds less than 2^32 threads
 
 const char* check_size(int64_t rows, int64_t actions, int64_t mask_len, int64_t pairs, const Aim& aim, Rows* R) {
   if (rows < 0 || actions < 1) return "rows must be at least 0 and actions at least 1";
-  if (actions > MOST - 2 * TILE * MOST_PER || rows > MOST / 64 || pairs > MOST / 64) return "too many rows, pairs (2^25) or actions (2^31 - 65537)";
+  if (actions > MOST - 2 * TILE * MOST_PER || rows > MOST_LAUNCHED || pairs > MOST_LAUNCHED) return "too many rows, pairs (2^24 - 1) or actions (2^31 - 65537)";
   if (mask_len < 0 || (mask_len && actions % mask_len)) return "mask_len must divide actions";
   cut(rows, actions, mask_len, GRADIENT, R);
   const int64_t most = R->pieces;                    // the finest of the cuts
   cut(rows, actions, mask_len, aim, R);
-  if (rows * most > MOST - (rows + THREADS) / THREADS - FIRST) return "too many logits in one call";
+  if (rows * most > MOST_LAUNCHED - rows / THREADS - 2 * FIRST) return "too many logits in one call";
   return nullptr;
 }
 // checks what every entry point over rows checks; launches nothing
@@ -116,14 +118,14 @@ void stats(const Rows& R, int dtype, hipStream_t s, const Span& span, const int6
   if (!R.rows) return;
   const int front = (R.rows + 8 * THREADS - 1) / (8 * THREADS) * 8;
   by_type(dtype, [&](auto t) { by_flag(R.mask, [&](auto m) { by_flag(R.ref, [&](auto q) {
-    ur5_policy_stats<decltype(t), decltype(m)::value, decltype(q)::value><<<front + R.rows * R.pieces, THREADS, 0, s>>>(R, span, front, action, w.parts, w.slopes);
+    ur5_policy_stats<decltype(t), decltype(m)::value, decltype(q)::value><<<front + R.rows * R.pieces, THREADS, 0, s>>>(R, span, front, action, w.parts, w.slopes, w.counts);
   }); }); });
 }
 // the rows of the clipped loss, or the pairs of the preference loss: slopes and terms
 void clip_rows(const Rows& R, int dtype, hipStream_t s, const Clip& C, const Work& w, float* logp, float* kl, float* entropy) {
   stats(R, dtype, s, Span{}, C.action, w);
   if (R.rows) by_type(dtype, [&](auto t) { by_flag(R.ref, [&](auto q) {
-    ur5_policy_clip_rows<decltype(t), decltype(q)::value><<<(R.rows + WAVES - 1) / WAVES, THREADS, 0, s>>>(R, C, w.parts, w.slopes, w.term, logp, kl, entropy);
+    ur5_policy_clip_rows<decltype(t), decltype(q)::value><<<(R.rows + WAVES - 1) / WAVES, THREADS, 0, s>>>(R, C, w.parts, w.slopes, w.counts, w.counting, w.term, logp, kl, entropy);
   }); });
 }
 void prefer_pairs(const Rows& R, int dtype, hipStream_t s, const Prefer& P, const Work& w, float* margin) {
@@ -136,6 +138,12 @@ void gradient(Rows R, int dtype, hipStream_t s, const Terms& t, const int64_t* a
   by_type(dtype, [&](auto k) { by_flag(R.mask, [&](auto m) { by_flag(R.ref, [&](auto q) { by_flag(past, [&](auto p) {
     ur5_policy_grad<decltype(k), decltype(m)::value, decltype(q)::value, decltype(p)><<<FIRST + R.rows * R.pieces, THREADS, 0, s>>>(R, t, action, w.slopes, scale, upstream, grad);
   }); }); }); });
+}
+Terms clip_terms(const Rows& R, const Work& w, float* loss) { return Terms{w.term, R.rows, R.rows ? w.counting : nullptr, loss}; }
+// the gradient of the clipped loss; the reference has no part in it without a KL term
+void clip_gradient(Rows R, const ur5_rows* r, const ur5_clip* c, const Terms& t, const Work& w, void* grad) {
+  if (!(c->kl_coef > 0)) R.ref = nullptr;
+  gradient(R, r->dtype, (hipStream_t)r->stream, t, c->action, w, c->grad_scale, c->upstream, grad);
 }
 }  // namespace
 
@@ -186,7 +194,7 @@ int ur5_policy_clip_loss(const ur5_rows* r, const ur5_clip* c, float* loss, floa
   ON(r->device);
   const hipStream_t s = (hipStream_t)r->stream;
   clip_rows(R, r->dtype, s, clip_of(c), w, logp, kl, entropy);
-  ur5_policy_loss<<<1, THREADS, 0, s>>>(Terms{w.term, R.rows, 0, w.slopes, R.rows, loss});
+  ur5_policy_loss<<<1, THREADS, 0, s>>>(clip_terms(R, w, loss));
   return launched(__func__);
 }
 int ur5_policy_clip_grad(const ur5_rows* r, const ur5_clip* c, void* grad) {
@@ -196,7 +204,7 @@ int ur5_policy_clip_grad(const ur5_rows* r, const ur5_clip* c, void* grad) {
   if (!R.rows) return 0;
   if (!grad) return fail(UR5_ERR_ARG, __func__, "grad is needed");
   ON(r->device);
-  gradient(R, r->dtype, (hipStream_t)r->stream, Terms{}, c->action, w, c->grad_scale, c->upstream, grad);
+  clip_gradient(R, r, c, clip_terms(R, w, nullptr), w, grad);
   return launched(__func__);
 }
 int ur5_policy_clip_loss_grad(const ur5_rows* r, const ur5_clip* c, float* loss, float* logp, float* kl, float* entropy, void* grad) {
@@ -207,7 +215,7 @@ int ur5_policy_clip_loss_grad(const ur5_rows* r, const ur5_clip* c, float* loss,
   ON(r->device);
   const hipStream_t s = (hipStream_t)r->stream;
   clip_rows(R, r->dtype, s, clip_of(c), w, logp, kl, entropy);
-  gradient(R, r->dtype, s, Terms{w.term, R.rows, 0, w.slopes, R.rows, loss}, c->action, w, c->grad_scale, c->upstream, grad);
+  clip_gradient(R, r, c, clip_terms(R, w, loss), w, grad);
   return launched(__func__);
 }
 
@@ -220,7 +228,7 @@ int ur5_policy_prefer_loss(const ur5_rows* r, const ur5_prefer* p, float* loss, 
   ON(r->device);
   const hipStream_t s = (hipStream_t)r->stream;
   prefer_pairs(R, r->dtype, s, prefer_of(p), w, margin);
-  ur5_policy_loss<<<1, THREADS, 0, s>>>(Terms{w.term, (int)p->pairs, (int)p->pairs, w.slopes, R.rows, loss});
+  ur5_policy_loss<<<1, THREADS, 0, s>>>(Terms{w.term, (int)p->pairs, nullptr, loss});
   return launched(__func__);
 }
 int ur5_policy_prefer_grad(const ur5_rows* r, const ur5_prefer* p, void* grad) {
@@ -243,14 +251,14 @@ int ur5_policy_prefer_loss_grad(const ur5_rows* r, const ur5_prefer* p, float* l
   ON(r->device);
   const hipStream_t s = (hipStream_t)r->stream;
   prefer_pairs(R, r->dtype, s, prefer_of(p), w, margin);
-  gradient(R, r->dtype, s, Terms{w.term, (int)p->pairs, (int)p->pairs, w.slopes, R.rows, loss}, p->action, w, p->grad_scale, p->upstream, grad);
+  gradient(R, r->dtype, s, Terms{w.term, (int)p->pairs, nullptr, loss}, p->action, w, p->grad_scale, p->upstream, grad);
   return launched(__func__);
 }
 
 // ---- 8-bit checkpoints
 static const char* check_planes(int dtype, int64_t planes, int64_t size) {
   if (dtype != UR5_F32 && dtype != UR5_F16 && dtype != UR5_BF16) return "dtype must be UR5_F32, UR5_F16 or UR5_BF16";
-  if (planes < 0 || size < 1 || size > MOST - ur5act8::GROUP || planes > MOST || planes * ((size + ur5act8::GROUP - 1) / ur5act8::GROUP) > MOST) return "planes must be at least 0, a plane of 1 .. 2^31 - 65 values, and all groups below 2^31";
+  if (planes < 0 || size < 1 || size > MOST - ur5act8::GROUP || planes > MOST || planes * ((size + ur5act8::GROUP - 1) / ur5act8::GROUP) > MOST_LAUNCHED * ur5act8::Lane<f32_t>::GROUPS) return "planes must be at least 0, a plane of 1 .. 2^31 - 65 values, and all groups below 2^29 - 31";
   return nullptr;
 }
 int ur5_act8_pack(const void* x, int dtype, int64_t planes, int64_t size, int8_t* codes, float* scales, int device, void* stream) {

@@ -231,7 +231,7 @@ def clipped_policy_loss(logits, action, old_logp, advantage, mask=None, ref_logi
         -min(r A, clip(r, 1 - low, 1 + high) A) + kl_coef KL(row || ref row) - entropy_coef H(row),      r = exp(logp - old_logp)
 
     action int64 [N] (-1: the row does not count), old_logp / advantage A float [N] (constants); ``ref_logits`` like the logits: the KL is exact, over all allowed actions (+inf where
-    the reference gives probability 0 to an action of positive probability). ``clip``: one number or (low, high). logp, kl, entropy: float32 [N], no gradient, 0 in rows that do not
+    the reference gives probability 0 to an action whose own is above 0 in 32 bits; without a kl_coef it is only reported). ``clip``: one number or (low, high). logp, kl, entropy: float32 [N], no gradient, 0 in rows that do not
     count (kl is 0 without ref_logits)."""
     return PolicyLoss(*_ClippedPolicyLoss.apply(logits, _Clip(logits, action, old_logp, advantage, mask, ref_logits, clip, kl_coef, entropy_coef)))
 

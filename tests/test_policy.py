@@ -78,6 +78,17 @@ def test_entry_points_refuse_bad_numbers_and_missing_outputs():
     assert all(lib.ur5_policy_work_bytes(*bad) == 0 for bad in ((-1, 5, 0, 0), (5, 0, 0, 0), (5, 6, 4, 0), (5, 6, -1, 0), (5, 6, 0, -1)))
 
 
+def test_sizes_past_one_launch_are_refused():
+    """A launch holds less than 2^32 threads, and a row (a pair) takes a workgroup of 256 at least."""
+    lib = native.load()
+    assert lib.ur5_policy_work_bytes(16_000_000, 6, 0, 0) > 0
+    for rows, pairs in (((1 << 24) - 1, 0), (1 << 24, 0), (1, 1 << 24)):
+        assert lib.ur5_policy_work_bytes(rows, 6, 0, pairs) == 0
+    big = _good_rows()
+    big.rows = 1 << 24
+    assert lib.ur5_policy_logp(C.byref(big), 4096, 4096, None) == -1 and b"too many" in lib.ur5_last_error()
+
+
 def test_no_gpu_is_an_error():
     if torch.cuda.is_available():
         pytest.skip("a GPU is visible here")
@@ -336,6 +347,42 @@ def test_nan_and_infinity_in_allowed_places_show():
 
 
 # ------------------------------------------------------------------ preference loss
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_reference_that_rules_actions_out(dtype):
+    """Its KL is infinite where the policy may take such an action: reported, and without weight in neither the loss nor the gradient. An action whose probability is 0 in 32 bits
+    adds nothing, whatever the reference says of it."""
+    shape, kind = (7, 2, 6, 11), "random"
+    z, mask, ok, a, counts, old, adv, ref = _clip_case(shape, dtype, kind, True, seed=21)
+    numbers = dict(clip=0.2, entropy_coef=0.1)
+    hard = ref.clone()
+    hard[..., ::3] = -math.inf
+    terms, grad = policy.clipped_policy_grad(z, a, old, adv, mask, hard, **numbers)
+    assert (terms.kl[counts] == math.inf).any()
+    _check_clip(terms._replace(kl=torch.zeros_like(terms.kl)), grad, _plain_clip(z, ok, a, counts, old, adv, None, **numbers), dtype, numbers)
+    leaf = z.clone().requires_grad_()
+    loss = policy.clipped_policy_loss(leaf, a, old, adv, mask, hard, **numbers).loss
+    loss.backward()
+    assert torch.equal(loss.detach(), terms.loss) and torch.equal(leaf.grad, grad)
+    far = z.clone()
+    far[..., ::3] = -32768                                          # (its exp is 0 in 64 bits, too)
+    a = torch.where((a % 11) % 3 == 0, -1, a)
+    numbers = dict(clip=0.2, kl_coef=0.3)
+    want = policy.clipped_policy_grad(far, a, old, adv, mask, far, **numbers), policy.clipped_policy_grad(far, a, old, adv, mask, torch.where(far == -32768, -math.inf, far), **numbers)
+    for x, y in zip((*want[0][0], want[0][1]), (*want[1][0], want[1][1])):
+        assert torch.isfinite(x).all() and torch.equal(x, y)
+
+
+@pytest.mark.gpu
+def test_many_short_rows():
+    """More rows than one workgroup counts, in parts that end inside it."""
+    for n, shape, kind in ((257, (2, 1, 3), "random"), (70_001, (1, 1, 5), "none"), (20_000, (2, 2, 2), "random")):
+        z, mask, ok, a, counts, old, adv, ref = _clip_case((n,) + shape, torch.float32, kind, True, seed=n)
+        numbers = dict(clip=0.2, kl_coef=0.5, entropy_coef=0.01)
+        got, grad = policy.clipped_policy_grad(z, a, old, adv, mask, ref, **numbers)
+        _check_clip(got, grad, _plain_clip(z, ok, a, counts, old, adv, ref, **numbers), torch.float32, numbers)
+
+
 def _plain_prefer(z, ok, a, counts, ref_logp, offsets, beta, eps):
     P = Plain(z, ok)
     ratio = torch.where(counts, _at(P.logp, a) - ref_logp.double(), 0.0)
