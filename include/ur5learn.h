@@ -77,7 +77,7 @@ int ur5_policy_prefer_loss_grad(const ur5_rows* r, const ur5_prefer* p, float* l
 int ur5_act8_pack(const void* x, int dtype, int64_t planes, int64_t size, int8_t* codes, float* scales, int device, void* stream);
 int ur5_act8_unpack(const int8_t* codes, const float* scales, int64_t planes, int64_t size, void* x, int dtype, int device, void* stream);
 /* weight gradient of a pointwise (1 x 1) convolution from its checkpointed input: codes / scales of x [n][cin][size], dy [n][cout][size] (dense, dtype) ->
-   dw [cout][cin] = sum over images and pixels of dy x, db [cout] = sum of dy (NULL: not wanted), both fp32. work: ur5_act8_wgrad_work_bytes(...) bytes, 16-byte aligned. */
+   dw [cout][cin] = sum over images and pixels of dy x, db [cout] = sum of dy (NULL: not wanted), both fp32; an infinity in dy makes its row of dw NaN. work: ur5_act8_wgrad_work_bytes(...) bytes, 16-byte aligned. */
 int64_t ur5_act8_wgrad_work_bytes(int64_t n, int64_t cin, int64_t cout, int64_t size);
 int ur5_act8_wgrad(const int8_t* codes, const float* scales, const void* dy, int dtype, int64_t n, int64_t cin, int64_t cout, int64_t size, float* dw, float* db,
                    void* work, int64_t work_bytes, int device, void* stream);

@@ -50,7 +50,7 @@ class PackedActivation:
 
     def weight_grad(self, dy, bias=True):
         """For a pointwise convolution y[n, o] = sum_c w[o, c] x[n, c] + b[o] of the packed x [N, C, ...]: (dw float32 [O, C], db float32 [O]) from dy [N, O, ...] -- sums over images
-        and pixels, the same every time. bias=False: (dw, None)."""
+        and pixels, the same every time; an infinity in dy gives NaN. bias=False: (dw, None)."""
         _float_gpu(dy, "dy")
         shape = self.shape
         if len(shape) < 3 or shape[1] == 0 or dy.dim() != len(shape) or dy.shape[0] != shape[0] or dy.shape[2:] != shape[2:] or dy.get_device() != self.codes.get_device():
@@ -92,7 +92,7 @@ class _PointwiseConv(torch.autograd.Function):
     def forward(ctx, x, weight, bias):
         n, c = x.shape[:2]
         w = weight.reshape(weight.shape[0], c)
-        y = torch.matmul(w, x.reshape(n, c, -1).contiguous())
+        y = torch.matmul(w, x.flatten(2).contiguous())
         if bias is not None:
             y = y + bias.view(1, -1, 1)
         kept = pack(x)
@@ -105,10 +105,10 @@ class _PointwiseConv(torch.autograd.Function):
     def backward(ctx, dy):
         codes, scales, weight = ctx.saved_tensors
         dx = dw = db = None
-        n, cin, cout = ctx.shape[0], ctx.shape[1], weight.shape[0]
+        cin, cout = ctx.shape[1], weight.shape[0]
         if ctx.needs_input_grad[0]:
             w = weight.reshape(cout, cin).t().contiguous().to(dy.dtype)                      # (under autocast the output, and so dy, has fewer bits than the input)
-            dx = torch.matmul(w, dy.reshape(n, cout, -1).contiguous()).view(ctx.shape).to(ctx.dtype)
+            dx = torch.matmul(w, dy.flatten(2).contiguous()).view(ctx.shape).to(ctx.dtype)
         if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
             dw, db = PackedActivation(codes, scales, ctx.shape, ctx.dtype).weight_grad(dy, bias=ctx.has_bias)
             dw = dw.view(weight.shape).to(weight.dtype)
@@ -129,13 +129,13 @@ class _Relu(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x):
         y = torch.relu(x)
-        ctx.save_for_backward(y > 0)
+        ctx.save_for_backward(y <= 0)                        # (not of a NaN: its gradient passes)
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        return dy * ctx.saved_tensors[0]
+        return dy.masked_fill(ctx.saved_tensors[0], 0)       # whatever dy holds there
 
 
 def relu(x):
@@ -149,9 +149,19 @@ def active():
     return getattr(_active, "depth", 0) > 0
 
 
+def _is_parameter(t):
+    """A parameter, a view of one, or its copy in another type (what autocast hands to a layer)."""
+    source = t if t._base is None else t._base
+    if isinstance(source, torch.nn.Parameter) or (source.is_leaf and source.requires_grad):
+        return True
+    made = source.grad_fn
+    return made is not None and made.name() == "ToCopyBackward0" and made.next_functions[0][0].name() == "torch::autograd::AccumulateGrad"
+
+
 class saved_activations:
     """Context manager for a forward pass: floating-point GPU tensors of three or more dimensions and at least ``min_values`` values that autograd saves inside it are kept as 8-bit
-    checkpoints and restored when their backward runs. Parameters (leaves that want a gradient) and views of them are left alone; a weight that is computed from parameters is an activation here. In it, ``qnet``'s pointwise convolutions keep theirs for ``weight_grad`` and its ReLUs which values are positive (``relu``)."""
+    checkpoints and restored when their backward runs. Parameters (leaves that want a gradient, frozen nn.Parameters), views of them and
+    autocast's copies of the former are left alone; a weight that is computed from parameters is an activation here. In it, ``qnet``'s pointwise convolutions keep theirs for ``weight_grad`` and its ReLUs which values are positive (``relu``)."""
 
     def __init__(self, min_values=4096):
         self.min_values = int(min_values)
@@ -159,8 +169,7 @@ class saved_activations:
     def _pack(self, t):
         if not (t.is_cuda and t.dtype in DTYPES and t.dim() >= 3 and t.numel() >= self.min_values):
             return t
-        source = t if t._base is None else t._base
-        return t if source.is_leaf and source.requires_grad else pack(t)                     # a parameter, or a view of one
+        return t if _is_parameter(t) else pack(t)
 
     @staticmethod
     def _unpack(t):

@@ -19,6 +19,7 @@ def test_entry_points_refuse_bad_arguments():
         a = {**ok, **change}
         assert lib.ur5_act8_pack(a["x"], a["dtype"], a["planes"], a["size"], a["codes"], a["scales"], 0, None) == -1, change
         assert lib.ur5_act8_unpack(a["codes"], a["scales"], a["planes"], a["size"], a["x"], a["dtype"], 0, None) == -1 and lib.ur5_last_error().startswith(b"ur5_act8_unpack"), change
+    assert lib.ur5_act8_pack(4096, 0, 1 << 20, 64 * 600, 4096, 4096, 0, None) == -1                          # more groups than one launch takes
     need = lib.ur5_act8_wgrad_work_bytes(2, 3, 5, 100)
     assert need > 0 and lib.ur5_act8_wgrad_work_bytes(2, 0, 5, 100) == 0 and lib.ur5_act8_wgrad_work_bytes(2, 1 << 17, 5, 100) == 0
     ok = dict(codes=4096, scales=4096, dy=4096, dtype=0, n=2, cin=3, cout=5, size=100, dw=4096, db=4096, work=4096, bytes=need)
@@ -342,6 +343,47 @@ def test_parameters_are_not_packed():
         checkpoint8.pack = original
     got, = torch.autograd.grad(y, x, up)
     assert packed == [(2, 64, 20, 20)] and torch.allclose(got, want, rtol=1e-5, atol=1e-5)
+
+
+@pytest.mark.gpu
+def test_frozen_and_cast_parameters_are_not_packed():
+    """A frozen layer's weights, and autocast's copies of trained ones: what they are multiplied with in the backward pass is what the forward pass used."""
+    torch.manual_seed(3)
+    frozen, trained = nn.Conv2d(64, 64, 3, padding=1, bias=False).cuda().requires_grad_(False), nn.Conv2d(64, 64, 3, padding=1, bias=False).cuda()
+    context, seen = checkpoint8.saved_activations(), []
+    context._unpack = lambda t: t
+    pack = context._pack
+    context._pack = lambda t: seen.append((tuple(t.shape), t.dtype, pack(t))) or t
+    x = torch.randn(2, 64, 20, 20, device="cuda").requires_grad_()
+    with context:
+        frozen(x)
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            trained(x)
+    weights = [(d, p) for shape, d, p in seen if shape == (64, 64, 3, 3)]
+    assert {d for d, _ in weights} == {torch.float32, torch.bfloat16} and all(isinstance(p, torch.Tensor) for _, p in weights)
+    assert not any(isinstance(p, checkpoint8.PackedActivation) for _, _, p in seen)                          # x is a leaf that wants a gradient, too
+    del seen[:]
+    with context:
+        h = frozen(x)
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            trained(h)
+    assert [d for shape, d, p in seen if isinstance(p, checkpoint8.PackedActivation)] == [torch.bfloat16]    # the second layer's input, as it went in
+
+
+@pytest.mark.gpu
+def test_pointwise_conv_of_an_empty_batch():
+    x, w, b = torch.empty(0, 5, 3, 4).cuda().requires_grad_(), torch.randn(7, 5).cuda().requires_grad_(), torch.randn(7).cuda().requires_grad_()
+    y = checkpoint8.pointwise_conv(x, w, b)
+    dx, dw, db = torch.autograd.grad(y.sum(), (x, w, b))
+    assert y.shape == (0, 7, 3, 4) and dx.shape == x.shape and torch.equal(dw, torch.zeros_like(w)) and torch.equal(db, torch.zeros_like(b))
+
+
+def test_relu_passes_what_the_plain_one_passes():
+    x = torch.tensor([-1.0, 0.0, 2.0, math.nan, -math.inf, math.inf], requires_grad=True)
+    for up in (torch.full((6,), 3.0), torch.full((6,), math.inf), torch.full((6,), math.nan)):
+        got, = torch.autograd.grad(checkpoint8.relu(x), x, up)
+        want, = torch.autograd.grad(torch.relu(x), x, up)
+        assert torch.equal(torch.nan_to_num(got, nan=7.0), torch.nan_to_num(want, nan=7.0))
 
 
 @pytest.mark.gpu
