@@ -167,6 +167,11 @@ def action_log_probs(logits, action, mask=None):
     return logp, entropy
 
 
+def _gradient_of(logits):
+    """Room for a dense gradient (empty_like costs the host half of what a shape does)."""
+    return torch.empty_like(logits) if logits.is_contiguous() else torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+
+
 # ------------------------------------------------------------------ clipped policy loss
 class _Clip:
     """Checked arguments of a clipped loss."""
@@ -241,7 +246,7 @@ def clipped_policy_grad(logits, action, old_logp, advantage, mask=None, ref_logi
     ``logits.backward(grad)``. float16 logits want a ``grad_scale``: the entries are about p / N."""
     c = _Clip(logits, action, old_logp, advantage, mask, ref_logits, clip, kl_coef, entropy_coef)
     loss, logp, kl, entropy = c.outputs()
-    grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    grad = _gradient_of(logits)
     work = _work(c.z, c.mask)
     _check(_library().ur5_policy_clip_loss_grad(_rows(c.z, c.mask, c.ref, work), c.pack(float(grad_scale)), loss.data_ptr(), logp.data_ptr(), kl.data_ptr(), entropy.data_ptr(),
                                                 grad.data_ptr()), "ur5_policy_clip_loss_grad")
@@ -308,7 +313,7 @@ def preference_grad(logits, action, ref_logp, offsets, mask=None, beta=0.1, labe
     """(``PreferenceLoss``, its gradient times ``grad_scale`` with respect to the logits) without an autograd graph: for ``logits.backward(grad)``."""
     p = _Prefer(logits, action, ref_logp, offsets, mask, beta, label_smoothing)
     loss, margin = p.outputs()
-    grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    grad = _gradient_of(logits)
     work = _work(p.z, p.mask, p.pairs)
     _check(_library().ur5_policy_prefer_loss_grad(_rows(p.z, p.mask, None, work), p.pack(float(grad_scale)), loss.data_ptr(), margin.data_ptr(), grad.data_ptr()),
            "ur5_policy_prefer_loss_grad")
