@@ -575,38 +575,56 @@ __device__ __forceinline__ void join_best(Best& b, int width) {
     if (better(s, i, b.score, b.at)) { b.score = s; b.at = i; }
   }
 }
-// 1 - u of 8 neighbouring draws, rounded down to 32 bits
+// 1 - u of 8 neighbouring draws in units of 2^-32, off by at most 1 from what it is rounded down (the finaliser's last shift, left out, may flip the lowest bit)
 __device__ __forceinline__ void missing8(uint64_t key, int j, uint32_t* w) {
   uint64_t c = key + (uint64_t)(j + 1) * GOLD;
 #pragma unroll
   for (int i = 0; i < VEC; i++, c += GOLD) {
     uint64_t x = (c ^ (c >> 30)) * 0xBF58476D1CE4E5B9ull;
     x = (x ^ (x >> 27)) * 0x94D049BB133111EBull;
-    const uint32_t hi = (uint32_t)(x >> 32);
-    w[i] = ~(hi ^ (hi >> 31));
+    w[i] = ~(uint32_t)(x >> 32);
   }
 }
-template <typename T> __device__ __forceinline__ void draw8(const typename T::raw* row, uint64_t key, int j, const Running& a, const float* z, const float* e, bool first, int* bar, Best& best) {
+// What the workgroup has found: the bar, and the actions that passed it, whose scores are computed together at the end (64 bits of two logarithms cost 250 instructions, for one
+// lane as for all). Where more pass -- logits so large that the margin covers many -- the rest are scored as they come.
+constexpr int LISTED = 64;
+struct Found { int bar, listed; int at[LISTED]; };
+template <typename T> __device__ __forceinline__ void score(const typename T::raw* row, uint64_t key, int at, Best& best) {
+  const float v = widen(T{}, row[at]);
+  const double s = noisy_score(v, key, at);
+  if (v > -INFINITY && better(s, at, best.score, best.at)) best = Best{s, at};
+}
+// a score from below in 32 bits: E <= (1 - u) / u
+__device__ __forceinline__ float at_least(float z, uint32_t w) { return z - 0.693147181f * __log2f(((float)w + 2.f) * __builtin_amdgcn_rcpf((float)~w)); }
+template <typename T> __device__ __forceinline__ void draw8(const typename T::raw* row, uint64_t key, int j, const Running& a, uint32_t allowed, const float* z, const float* e, bool first, Found& found, Best& best) {
   uint32_t w[VEC];
   missing8(key, j, w);
-  if (first) {   // no score yet: a bound from below, E <= (1 - u) / u, one fast logarithm per action
+  if (first) {   // no score yet
     float low = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < VEC; i++) low = fmaxf(low, z[i] - 0.693147181f * __log2f(((float)w[i] + 1.f) * __builtin_amdgcn_rcpf((float)~w[i])));
-    atomicMax(bar, ordered(below(low)));
+    for (int i = 0; i < VEC; i++) low = fmaxf(low, at_least(z[i], w[i]));
+    atomicMax(&found.bar, ordered(below(low)));
   }
-  const float reach = fminf(__builtin_amdgcn_exp2f((a.m - unordered(__hip_atomic_load(bar, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP))) * LOG2E), 1e30f) * (1.0001f * 4294967296.f);
-  uint32_t near = 0;
+  const float reach = fminf(__builtin_amdgcn_exp2f((a.m - unordered(__hip_atomic_load(&found.bar, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP))) * LOG2E), 1e30f) * (1.0001f * 4294967296.f);
+  bool some = false;                                           // of all lanes, on the scalar side; which one it was is asked only where there is one
 #pragma unroll
-  for (int i = 0; i < VEC; i++) near |= (e[i] > 0 && (float)w[i] <= e[i] * reach) ? 1u << i : 0u;
-  while (near) {
+  for (int i = 0; i < VEC; i++) some |= (float)w[i] <= fmaf(e[i], reach, 1.f);
+  if (!some) return;
+  uint32_t near = 0;
+  float low = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < VEC; i++) {
+    const bool passes = (allowed >> i & 1) && (float)w[i] <= fmaf(e[i], reach, 1.f);
+    near |= passes ? 1u << i : 0u;
+    low = passes ? fmaxf(low, at_least(z[i], w[i])) : low;
+  }
+  if (!near) return;
+  if (!first) atomicMax(&found.bar, ordered(below(low)));
+  int to = atomicAdd(&found.listed, __popc(near));
+  for (; near; near &= near - 1, to++) {
     const int at = j + __ffs(near) - 1;
-    near &= near - 1;
-    const double s = noisy_score(widen(T{}, row[at]), key, at);
-    if (better(s, at, best.score, best.at)) {
-      best = Best{s, at};
-      atomicMax(bar, ordered(below(s)));
-    }
+    if (to < LISTED) found.at[to] = at;
+    else score<T>(row, key, at, best);
   }
 }
 // the drawn action (-1: nothing may be taken, log-probability 0) and its log-probability
@@ -619,9 +637,9 @@ constexpr int NOBODY = 0x7fffffff;
 template <typename T, bool MASK> __global__ void __launch_bounds__(THREADS) ur5_policy_sample(Rows R, uint64_t offset, const int64_t* gids, Draw* draws, int64_t* action, float* logp) {
   const int row = blockIdx.x / R.pieces, piece = blockIdx.x % R.pieces;
   const uint64_t key = mix64((uint64_t)gids[row] * GOLD + offset);
-  __shared__ int bar;
+  __shared__ Found found;
   __shared__ Best wave[WAVES];
-  if (threadIdx.x == 0) bar = ordered(-INFINITY);
+  if (threadIdx.x == 0) { found.bar = ordered(-INFINITY); found.listed = 0; }
   __syncthreads();
   const auto* z_row = (const typename T::raw*)R.logits + row * R.stride;
   Running a = nothing();
@@ -631,16 +649,22 @@ template <typename T, bool MASK> __global__ void __launch_bounds__(THREADS) ur5_
     float e[VEC];
     if (MASK) bar8(allowed, z);
     add8<false, false>(a, z, nullptr, e);
-    draw8<T>(z_row, key, j, a, z, e, first, &bar, best);
+    draw8<T>(z_row, key, j, a, allowed, z, e, first, found, best);
     first = false;
   };
   for_piece<MASK>(R, row, piece, [&](int j) { return fetch8<T>(z_row + j); }, [&](int j, uint32_t allowed, const Eight<T>& w) { float z[VEC]; unpack8(w, z); draw(j, allowed, z); },
     [&](int j, uint32_t allowed, int left) { float z[VEC]; take8<T>(z_row + j, left, z); draw(j, allowed, z); }, [](const Piece&, int) {});
+  const Sums sums = join_workgroup(a, false, false);   // (its barrier stands between the list and its readers)
+  const int listed = found.listed;
+  if (listed > LISTED) {                               // the others' bests, too
+    join_best(best, 64);
+    if ((threadIdx.x & 63) == 0) wave[threadIdx.x >> 6] = best;
+    __syncthreads();
+    best = wave[threadIdx.x & (WAVES - 1)];
+  }
+  if (threadIdx.x >= 64) return;
+  if ((int)threadIdx.x < listed) score<T>(z_row, key, found.at[threadIdx.x], best);
   join_best(best, 64);
-  if ((threadIdx.x & 63) == 0) wave[threadIdx.x >> 6] = best;
-  const Sums sums = join_workgroup(a, false, false);   // (its barrier stands between the wavefronts' bests and their join)
-  best = wave[threadIdx.x & (WAVES - 1)];
-  join_best(best, WAVES);
   if (threadIdx.x) return;
   if (R.pieces == 1) write_draw<T>(R, row, sums.m, sums.s, best, action, logp);
   else draws[blockIdx.x] = Draw{best.score, sums.s, sums.m, best.at};
