@@ -560,9 +560,10 @@ template <typename T> __global__ void __launch_bounds__(THREADS) ur5_policy_logp
 
 // ---- sampling. argmax_j z_j - log(-log u_j) is a draw from softmax(z). Two logarithms in 64 bits per action would cost more than reading it, and nearly every action
 // is far from winning: with E = -log u >= 1 - u, action j can only reach score `bar` if 1 - u_j <= exp(z_j - bar) -- one product and one comparison on the exp that the
-// softmax's sum needs anyway. `bar` is the best score any thread of the workgroup has seen (less a margin over every rounding below), so about one action per
-// piece passes and is scored in 64 bits; equal scores go to the lower action, so the result does not depend on who was first.
-// What is left per action is the hash: three products of 64 bits, which is what bounds it (512 masked fp32 rows of 6 x 200 x 200: 100 us, log-probability and entropy of the same rows 51).
+// softmax's sum needs anyway. `bar` is the best score any thread of the workgroup has seen (less a margin over every rounding below), so a few actions per
+// piece pass and are scored in 64 bits; equal scores go to the lower action, so the result does not depend on who was first.
+// What is left per action is the hash: two products of 64 bits, six of the slow integer instructions, which is what bounds it (512 masked fp32 rows of 6 x 200 x 200: 88 us,
+// log-probability and entropy of the same rows 51).
 __device__ __forceinline__ int ordered(float v) { const int b = __float_as_int(v); return b ^ ((b >> 31) & 0x7fffffff); }
 __device__ __forceinline__ float unordered(int o) { return __int_as_float(o ^ ((o >> 31) & 0x7fffffff)); }
 __device__ __forceinline__ float below(double score) { return (float)score - (1e-4f + 1e-6f * fabsf((float)score)); }

@@ -39,7 +39,7 @@ int no_device(const char* entry, hipError_t e) {
 // ---- how rows are cut. Pieces grow from one turn of 256 threads first over the maps, which share a list of allowed pixels, then along the pixels, up to 64 turns, so that a
 // thread's fp32 sums stay short (512 terms); images of less than 2048 pixels take as many maps as fill a workgroup. How many pieces a call aims at: more fill the card's 256 CUs
 // (8 workgroups each) more evenly, fewer share what a piece costs before and after its loads. us of the kernel at 2048 / 4096 / 8192 / 16384 pieces wanted:
-// sample (512 fp32 rows) 103 / 101 / 114 / 157, logp (2000 x 40 000 bf16) 45 / 36 / 38 / 47, statistics (513 bf16 rows) 70 / 66 / 75 / 99, gradient 123 / 113 / 103 / 90, at
+// sample (512 fp32 rows) 96 / 88 / 102 / 138, logp (2000 x 40 000 bf16) 45 / 36 / 38 / 47, statistics (513 bf16 rows) 70 / 66 / 75 / 99, gradient 123 / 113 / 103 / 90, at
 // 24576 89, at 32768 123 (259 fp32 rows: 78, 73, 75).
 // A row of few turns is one piece of the calls that end with it: their second launch costs 3 us more than 5 turns (12 rows of 6 x 40 x 40, us a call: logp 14.4 -> 11.6, sample
 // 13.9 -> 11.8; of 11 turns: logp 13.7 -> 10.7, sample 14.0 -> 17.7).
