@@ -208,6 +208,20 @@ def test_sampled_actions_are_the_noisy_argmax(shape, dtype, kind):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,large", [(torch.float32, 1e8), (torch.float32, -3e5), (torch.bfloat16, 1e8), (torch.float16, 6e4)])
+def test_sampling_of_large_logits(dtype, large):
+    """Logits whose spacing is coarser than the noise: many actions stay in the running to the end, and 64 bits decide between them."""
+    z, mask, ok = _inputs((3, 2, 70, 97), dtype, "random", seed=31)
+    z = (z.double() + large).to(dtype)
+    gids = torch.arange(3).cuda() + 5
+    action, logp = policy.sample_actions(z, 4, gids, 2, mask)
+    u = sharding.scene_uniform(4, gids, 2, policy.SAMPLE_STREAM, ok.shape[1], dtype=torch.float64).clamp(min=2.0 ** -54)
+    P = Plain(z, ok)
+    assert torch.equal(action, torch.where(P.some, (P.z - torch.log(-torch.log(u))).argmax(1), -1))
+    _close(logp, torch.where(P.some, _at(P.logp, action), 0.0), SUM, "logp")
+
+
+@pytest.mark.gpu
 def test_a_scene_draws_the_same_however_the_scenes_are_split():
     z, mask, ok = _inputs((9, 6, 40, 40), torch.float32, "random", seed=4)
     gids = torch.randperm(9, generator=torch.Generator().manual_seed(1)).cuda() + 100
