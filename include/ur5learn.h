@@ -54,7 +54,7 @@ typedef struct ur5_clip {
 int ur5_policy_clip_loss(const ur5_rows* r, const ur5_clip* c, float* loss, float* logp, float* kl, float* entropy);
 /* grad [rows][actions] (dense, dtype of the logits) of the loss times grad_scale times *upstream, from the workspace that clip_loss left; rows that do not count get 0. */
 int ur5_policy_clip_grad(const ur5_rows* r, const ur5_clip* c, void* grad);
-/* both at once, in three launches. */
+/* both at once, in two (few rows) or three launches. */
 int ur5_policy_clip_loss_grad(const ur5_rows* r, const ur5_clip* c, float* loss, float* logp, float* kl, float* entropy, void* grad);
 
 typedef struct ur5_prefer {

@@ -362,7 +362,7 @@ template <typename T, bool MASK, bool REF, bool ENTROPY> __device__ __forceinlin
 
 // ---- what both losses have in common. Per row, dL/dz_j = p_j (c0 + kl (z_j - q_j - gap) + entropy (z_j - m - level)) + [j = action] take; p_j = exp(z_j - m) rs.
 // Three launches: statistics of the pieces -- a Slope per row and a term per row or pair of the loss -- the gradient, of which the first workgroup adds the terms up.
-// (Joining a row's records in every workgroup of the gradient instead saves a launch and costs each of them 3 us of double arithmetic before its first load.)
+// (Joining a row's records in every workgroup of the gradient saves a launch and costs each of them 3 us of double arithmetic before its first load: ur5_policy_clip_few.)
 // Bound by memory where rows are many -- 513 masked bf16 rows of 6 x 200 x 200 with their reference: 71 + 7 + 89 us; the mask's runs end inside 128-byte lines, 288 MB are
 // fetched for 199 MB of allowed logits --, by the latency of three small launches where they are few (12 fp32 rows: 8 + 5 + 7 us).
 struct Slope { float m, rs, c0, kl, gap, entropy, level, take; int on; };   // on: the row counts; anything else is unset where it does not
@@ -424,16 +424,8 @@ __device__ __forceinline__ void add_terms(const Terms& t) {
 }
 // (a forward pass without a gradient)
 static __global__ void __launch_bounds__(THREADS) ur5_policy_loss(Terms t) { add_terms(t); }
-constexpr int FIRST = 8;             // workgroups before the pieces, as in the statistics; the first of them writes the loss if t.loss
-template <typename T, bool MASK, bool REF, typename Past> __global__ void __launch_bounds__(THREADS) ur5_policy_grad(Rows R, Terms t, const int64_t* action, const Slope* slopes, float scale, const float* upstream, void* grad) {
-  constexpr Past past;
-  const int block = (int)blockIdx.x - FIRST;
-  if (block < 0) {
-    if (t.loss && blockIdx.x == 0) add_terms(t);
-    return;
-  }
-  const int row = R.rows - 1 - block / R.pieces, piece = block % R.pieces;   // the rows that the statistics read last, and the 256 MB memory-side cache may hold, come first (259 fp32 rows: 80.0 us in their order, 78.7 in this; 513 bf16 rows: 91.6 and 90.3)
-  Slope S = slopes[row];
+// the gradient of a piece of a row; factor: of the whole gradient
+template <typename T, bool MASK, bool REF, typename Past> __device__ __forceinline__ void grad_piece(const Rows& R, int row, int piece, Slope S, float factor, int a, void* grad, Past past) {
   typename T::raw* out = (typename T::raw*)grad + (long long)row * R.actions;
   const float zero[VEC] = {};
   const auto clear = [&](const Piece& P, int g) {          // 8 pixels of all maps of the piece
@@ -445,9 +437,7 @@ template <typename T, bool MASK, bool REF, typename Past> __global__ void __laun
     for (int g = threadIdx.x; g * VEC < P.pixels; g += THREADS) clear(P, g);
     return;
   }
-  const float factor = scale * (upstream ? *upstream : 1.f) / (t.counting ? max(1, *t.counting) : 1);
   S.rs *= factor; S.take *= factor;
-  const int a = (int)action[row];
   const auto* z_row = (const typename T::raw*)R.logits + row * R.stride;
   const auto* q_row = REF ? (const typename T::raw*)R.ref + row * R.ref_stride : nullptr;
   const auto slope = [&](int j, uint32_t allowed, float* z, const float* q, float* g) {
@@ -473,34 +463,77 @@ template <typename T, bool MASK, bool REF, typename Past> __global__ void __laun
       put8<T>(out + j, left, false, g, past);
     }, clear);
 }
+__device__ __forceinline__ float grad_factor(float scale, const float* upstream, const int* counting) { return scale * (upstream ? *upstream : 1.f) / (counting ? max(1, *counting) : 1); }
+constexpr int FIRST = 8;             // workgroups before the pieces, as in the statistics; the first of them writes the loss if t.loss
+template <typename T, bool MASK, bool REF, typename Past> __global__ void __launch_bounds__(THREADS) ur5_policy_grad(Rows R, Terms t, const int64_t* action, const Slope* slopes, float scale, const float* upstream, void* grad) {
+  constexpr Past past;
+  const int block = (int)blockIdx.x - FIRST;
+  if (block < 0) {
+    if (t.loss && blockIdx.x == 0) add_terms(t);
+    return;
+  }
+  const int row = R.rows - 1 - block / R.pieces, piece = block % R.pieces;   // the rows that the statistics read last, and the 256 MB memory-side cache may hold, come first (259 fp32 rows: 80.0 us in their order, 78.7 in this; 513 bf16 rows: 91.6 and 90.3)
+  grad_piece<T, MASK, REF>(R, row, piece, slopes[row], grad_factor(scale, upstream, t.counting), (int)action[row], grad, past);
+}
 
 // ---- clipped policy loss. Per row: ratio r = exp(logp - old), L = -min(r A, clip(r, 1 - lo, 1 + hi) A) + kl_coef KL(p || q) - entropy_coef H; the mean over the rows that count.
 struct Clip { const int64_t* action; const float* old_logp; const float* advantage; float lo, hi, kl_coef, entropy_coef; };
-// a wavefront per row. Normalisers in 64 bits: KL = k / s - (lse - lse_q) is a small difference of large numbers.
-template <typename T, bool REF> __global__ void __launch_bounds__(THREADS) ur5_policy_clip_rows(Rows R, Clip C, const Part* parts, Slope* slopes, const int* counts, int* counting, double* term, float* logp, float* kl, float* entropy) {
-  if (blockIdx.x == 0) {
-    int n = 0;
-    for (int i = threadIdx.x; i < (R.rows + THREADS - 1) / THREADS; i += THREADS) n += counts[i];
-    n = workgroup_sum(n);
-    if (threadIdx.x == 0) *counting = n;
-  }
-  const int row = blockIdx.x * WAVES + (threadIdx.x >> 6);
-  if (row >= R.rows) return;
-  const bool on = slopes[row].on, writes = (threadIdx.x & 63) == 0;
-  if (!on) {
-    if (writes) { term[row] = 0; logp[row] = kl[row] = entropy[row] = 0; }
-    return;
-  }
-  const Sums a = join_row(parts + (size_t)row * R.pieces, R.pieces, REF);
-  if (!writes) return;
+// The end of a row that counts, by a wavefront, in every lane. Normalisers in 64 bits: KL = k / s - (lse - lse_q) is a small difference of large numbers.
+struct ClipRow { Slope slope; double term; float logp, kl, entropy; };
+template <typename T, bool REF> __device__ __forceinline__ ClipRow clip_row(const Rows& R, const Clip& C, const Part* parts, int pieces, int row) {
+  const Sums a = join_row(parts + (size_t)row * pieces, pieces, REF);
   const double ls = log(a.s), shift = REF ? (double)a.m - a.mq + ls - log(a.sq) : 0;
   const float adv = C.advantage[row], lp = (float)((double)logit<T>(R, row, C.action[row]) - a.m - ls), k = REF ? (float)(a.k / a.s - shift) : 0.f, h = (float)(ls - a.t / a.s);
   const float ratio = expf(lp - C.old_logp[row]), free = ratio * adv, held = fminf(fmaxf(ratio, 1 - C.lo), 1 + C.hi) * adv;
   const float take = held < free ? 0.f : -adv * ratio;   // the clipped branch has no slope; NaN stays
-  logp[row] = lp; kl[row] = k; entropy[row] = h;
-  term[row] = -(double)(held < free ? held : free) + (REF && C.kl_coef > 0 ? (double)C.kl_coef * k : 0.0) - (double)C.entropy_coef * h;   // (an infinite KL that has no weight is only reported)
-  slopes[row] = Slope{a.m, (float)(1 / a.s), -take, C.kl_coef, (float)(shift + k), C.entropy_coef, (float)(ls - h), take, 1};
+  const double term = -(double)(held < free ? held : free) + (REF && C.kl_coef > 0 ? (double)C.kl_coef * k : 0.0) - (double)C.entropy_coef * h;   // (an infinite KL that has no weight is only reported)
+  return ClipRow{Slope{a.m, (float)(1 / a.s), -take, C.kl_coef, (float)(shift + k), C.entropy_coef, (float)(ls - h), take, 1}, term, lp, k, h};
 }
+struct ClipOut { float* logp; float* kl; float* entropy; };
+__device__ __forceinline__ int rows_that_count(const int* counts, int rows) {   // by the workgroup
+  int n = 0;
+  for (int i = threadIdx.x; i < (rows + THREADS - 1) / THREADS; i += THREADS) n += counts[i];
+  return workgroup_sum(n);
+}
+template <typename T, bool REF> __global__ void __launch_bounds__(THREADS) ur5_policy_clip_rows(Rows R, Clip C, const Part* parts, Slope* slopes, const int* counts, int* counting, double* term, ClipOut out) {
+  if (blockIdx.x == 0) {
+    const int n = rows_that_count(counts, R.rows);
+    if (threadIdx.x == 0) *counting = n;
+  }
+  const int row = blockIdx.x * WAVES + (threadIdx.x >> 6);   // a wavefront per row
+  if (row >= R.rows) return;
+  ClipRow end{};
+  if (slopes[row].on) end = clip_row<T, REF>(R, C, parts, R.pieces, row);
+  if (threadIdx.x & 63) return;
+  term[row] = end.term; out.logp[row] = end.logp; out.kl[row] = end.kl; out.entropy[row] = end.entropy;
+  if (end.slope.on) slopes[row] = end.slope;
+}
+// Few rows: the gradient ends them by itself, every workgroup its own (its wavefronts all the same), the first one all of them for the loss: two launches instead of three.
+// `pieces`: the statistics' of a row. The first workgroup's wavefronts take the rows in turns, some 2.5 us each, while the others write the gradient: at most FEW rows, or as many
+// fewer as a lane has records of one. A call on fp32 rows with their reference, two launches against three: 12 of 6 x 200 x 200 (120 records) 22.1 us, 23.9; 16 of them 24.6, 24.0;
+// 24 of 131 x 93 21.5, 24.6; 48 of them 28.6, 24.5.
+constexpr int FEW = 24;
+template <typename T, bool MASK, bool REF> __global__ void __launch_bounds__(THREADS) ur5_policy_clip_few(Rows R, int pieces, Clip C, const Part* parts, const Slope* slopes, const int* counts, float* loss, ClipOut out, float scale,
+                                                                                                          const float* upstream, void* grad) {
+  const int block = (int)blockIdx.x - FIRST;
+  if (block < 0) {
+    if (blockIdx.x) return;
+    __shared__ double term[FEW];
+    for (int row = threadIdx.x >> 6; row < R.rows; row += WAVES) {
+      ClipRow end{};
+      if (slopes[row].on) end = clip_row<T, REF>(R, C, parts, pieces, row);
+      if ((threadIdx.x & 63) == 0) { term[row] = end.term; out.logp[row] = end.logp; out.kl[row] = end.kl; out.entropy[row] = end.entropy; }
+    }
+    __syncthreads();
+    add_terms(Terms{term, R.rows, counts, loss});          // (so few rows are one part of the counts)
+    return;
+  }
+  const int row = R.rows - 1 - block / R.pieces, piece = block % R.pieces;
+  Slope S{};
+  if (slopes[row].on) S = clip_row<T, REF>(R, C, parts, pieces, row).slope;
+  grad_piece<T, MASK, REF>(R, row, piece, S, grad_factor(scale, upstream, counts), (int)C.action[row], grad, no{});
+}
+static_assert(FEW <= THREADS, "one part of the counts");
 
 // ---- preference loss. Episodes are runs of rows: episode k holds the rows offsets[k] .. offsets[k + 1]. S_k = sum over its counting rows of logp - ref_logp,
 // margin_i = beta (S_2i - S_2i+1), loss = mean over pairs of (1 - eps) softplus(-margin) + eps softplus(margin).

@@ -122,20 +122,21 @@ void stats(const Rows& R, int dtype, hipStream_t s, const Span& span, const int6
   }); }); });
 }
 // the rows of the clipped loss, or the pairs of the preference loss: slopes and terms
-void clip_rows(const Rows& R, int dtype, hipStream_t s, const Clip& C, const Work& w, float* logp, float* kl, float* entropy) {
+void clip_rows(const Rows& R, int dtype, hipStream_t s, const Clip& C, const Work& w, const ClipOut& out) {
   stats(R, dtype, s, Span{}, C.action, w);
   if (R.rows) by_type(dtype, [&](auto t) { by_flag(R.ref, [&](auto q) {
-    ur5_policy_clip_rows<decltype(t), decltype(q)::value><<<(R.rows + WAVES - 1) / WAVES, THREADS, 0, s>>>(R, C, w.parts, w.slopes, w.counts, w.counting, w.term, logp, kl, entropy);
+    ur5_policy_clip_rows<decltype(t), decltype(q)::value><<<(R.rows + WAVES - 1) / WAVES, THREADS, 0, s>>>(R, C, w.parts, w.slopes, w.counts, w.counting, w.term, out);
   }); });
 }
 void prefer_pairs(const Rows& R, int dtype, hipStream_t s, const Prefer& P, const Work& w, float* margin) {
   stats(R, dtype, s, Span{P.offsets, 2 * P.pairs}, P.action, w);
   by_type(dtype, [&](auto t) { ur5_policy_prefer_pairs<decltype(t)><<<P.pairs, THREADS, 0, s>>>(R, P, w.parts, w.slopes, w.term, margin); });
 }
+// a call over more memory than the caches hold
+bool past_caches(const Rows& R, int dtype) { return (int64_t)R.rows * R.actions * (dtype == UR5_F32 ? 4 : 2) * (R.ref ? 3 : 2) > CACHE_BYTES; }
 void gradient(Rows R, int dtype, hipStream_t s, const Terms& t, const int64_t* action, const Work& w, float scale, const float* upstream, void* grad) {
   cut(R.rows, R.actions, R.mask ? R.pixels : 0, GRADIENT, &R);      // it leaves no records
-  const bool past = (int64_t)R.rows * R.actions * (dtype == UR5_F32 ? 4 : 2) * (R.ref ? 3 : 2) > CACHE_BYTES;
-  by_type(dtype, [&](auto k) { by_flag(R.mask, [&](auto m) { by_flag(R.ref, [&](auto q) { by_flag(past, [&](auto p) {
+  by_type(dtype, [&](auto k) { by_flag(R.mask, [&](auto m) { by_flag(R.ref, [&](auto q) { by_flag(past_caches(R, dtype), [&](auto p) {
     ur5_policy_grad<decltype(k), decltype(m)::value, decltype(q)::value, decltype(p)><<<FIRST + R.rows * R.pieces, THREADS, 0, s>>>(R, t, action, w.slopes, scale, upstream, grad);
   }); }); }); });
 }
@@ -193,7 +194,7 @@ int ur5_policy_clip_loss(const ur5_rows* r, const ur5_clip* c, float* loss, floa
   if (!loss || (R.rows && (!logp || !kl || !entropy))) return fail(UR5_ERR_ARG, __func__, "loss, logp, kl and entropy are needed");
   ON(r->device);
   const hipStream_t s = (hipStream_t)r->stream;
-  clip_rows(R, r->dtype, s, clip_of(c), w, logp, kl, entropy);
+  clip_rows(R, r->dtype, s, clip_of(c), w, ClipOut{logp, kl, entropy});
   ur5_policy_loss<<<1, THREADS, 0, s>>>(clip_terms(R, w, loss));
   return launched(__func__);
 }
@@ -214,7 +215,18 @@ int ur5_policy_clip_loss_grad(const ur5_rows* r, const ur5_clip* c, float* loss,
   if (!loss || (R.rows && (!logp || !kl || !entropy || !grad))) return fail(UR5_ERR_ARG, __func__, "loss, logp, kl, entropy and grad are needed");
   ON(r->device);
   const hipStream_t s = (hipStream_t)r->stream;
-  clip_rows(R, r->dtype, s, clip_of(c), w, logp, kl, entropy);
+  const ClipOut out{logp, kl, entropy};
+  if (R.rows && R.rows * (((int64_t)R.pieces + 63) / 64) <= FEW && (!R.ref || c->kl_coef > 0) && !past_caches(R, r->dtype)) {
+    const Clip C = clip_of(c);
+    const int pieces = R.pieces;
+    stats(R, r->dtype, s, Span{}, C.action, w);
+    cut(R.rows, R.actions, R.mask ? R.pixels : 0, GRADIENT, &R);
+    by_type(r->dtype, [&](auto t) { by_flag(R.mask, [&](auto m) { by_flag(R.ref, [&](auto q) {
+      ur5_policy_clip_few<decltype(t), decltype(m)::value, decltype(q)::value><<<FIRST + R.rows * R.pieces, THREADS, 0, s>>>(R, pieces, C, w.parts, w.slopes, w.counts, loss, out, c->grad_scale, c->upstream, grad);
+    }); }); });
+    return launched(__func__);
+  }
+  clip_rows(R, r->dtype, s, clip_of(c), w, out);
   clip_gradient(R, r, c, clip_terms(R, w, loss), w, grad);
   return launched(__func__);
 }

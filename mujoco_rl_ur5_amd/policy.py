@@ -242,7 +242,7 @@ def clipped_policy_loss(logits, action, old_logp, advantage, mask=None, ref_logi
 
 
 def clipped_policy_grad(logits, action, old_logp, advantage, mask=None, ref_logits=None, clip=0.2, kl_coef=0.0, entropy_coef=0.0, grad_scale=1.0):
-    """(``PolicyLoss``, its gradient times ``grad_scale`` with respect to the logits, in their shape and type) in three launches, without an autograd graph: for
+    """(``PolicyLoss``, its gradient times ``grad_scale`` with respect to the logits, in their shape and type) in two or three launches, without an autograd graph: for
     ``logits.backward(grad)``. float16 logits want a ``grad_scale``: the entries are about p / N."""
     c = _Clip(logits, action, old_logp, advantage, mask, ref_logits, clip, kl_coef, entropy_coef)
     loss, logp, kl, entropy = c.outputs()

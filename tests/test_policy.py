@@ -388,6 +388,21 @@ def test_a_reference_that_rules_actions_out(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(24, 1, 9, 11), (25, 1, 9, 11), (12, 3, 200, 200), (13, 6, 200, 200), (9, 6, 200, 200)])
+def test_both_sides_of_the_rule_for_few_rows(shape, dtype):
+    """Few rows are ended by the gradient itself, more by a launch of their own: same definition, and the same bits as the form that takes the gradient later."""
+    z, mask, ok, a, counts, old, adv, ref = _clip_case(shape, dtype, "random", True, seed=shape[0])
+    numbers, scale = dict(clip=0.2, kl_coef=0.5, entropy_coef=0.01), 64.0 if dtype == torch.float16 else 1.0
+    got, grad = policy.clipped_policy_grad(z, a, old, adv, mask, ref, grad_scale=scale, **numbers)
+    _check_clip(got, grad, _plain_clip(z, ok, a, counts, old, adv, ref, **numbers), dtype, numbers, scale)
+    leaf = z.clone().requires_grad_()
+    terms = policy.clipped_policy_loss(leaf, a, old, adv, mask, ref, **numbers)
+    (terms.loss * scale).backward()
+    assert all(torch.equal(x.detach(), y) for x, y in zip(terms, got)) and torch.equal(leaf.grad, grad)
+
+
+@pytest.mark.gpu
 def test_many_short_rows():
     """More rows than one workgroup counts, in parts that end inside it."""
     for n, shape, kind in ((257, (2, 1, 3), "random"), (70_001, (1, 1, 5), "none"), (20_000, (2, 2, 2), "random")):
