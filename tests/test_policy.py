@@ -481,9 +481,10 @@ def _call_inputs(shape=(5, 3, 20, 23), dtype=torch.float32, seed=8):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows", [5, 31])
 @pytest.mark.parametrize("dtype", TYPES)
-def test_strided_and_misaligned_rows_give_the_same_bits(dtype):
-    args = _call_inputs(dtype=dtype)
+def test_strided_and_misaligned_rows_give_the_same_bits(dtype, rows):
+    args = _call_inputs((rows, 3, 20, 23), dtype=dtype)
     want = _all_calls(*args)
     n, width = args[0].shape[0], args[0][0].numel()
 
@@ -560,8 +561,9 @@ def test_refusals_of_tensors():
 
 
 @pytest.mark.gpu
-def test_side_streams_and_two_calls_at_once():
-    args, other = _call_inputs((12, 6, 40, 40)), _call_inputs((7, 6, 40, 40), seed=15)
+@pytest.mark.parametrize("rows,others", [(12, 7), (37, 60)])
+def test_side_streams_and_two_calls_at_once(rows, others):
+    args, other = _call_inputs((rows, 6, 40, 40)), _call_inputs((others, 6, 40, 40), seed=15)
     want, want2 = _all_calls(*args), _all_calls(*other)
     torch.cuda.synchronize()
     s, t = torch.cuda.Stream(), torch.cuda.Stream()
@@ -577,9 +579,10 @@ def test_side_streams_and_two_calls_at_once():
 
 
 @pytest.mark.gpu
-def test_captured_graphs_replay():
+@pytest.mark.parametrize("first,second", [((5, 3, 20, 23), (9, 6, 40, 40)), ((300, 1, 20, 23), (40, 6, 40, 40))])
+def test_captured_graphs_replay(first, second):
     """Two graphs of the same calls on other sizes, replayed in turn with new inputs and eager work in between; every replay equals the eager result."""
-    sets = [(_call_inputs((5, 3, 20, 23), seed=s), _call_inputs((9, 6, 40, 40), seed=s + 50)) for s in (21, 22, 23)]
+    sets = [(_call_inputs(first, seed=s), _call_inputs(second, seed=s + 50)) for s in (21, 22, 23)]
     held = [[x.clone() for x in part] for part in sets[0]]
     for part in held:
         _all_calls(*part)
@@ -629,8 +632,9 @@ def test_backward_in_a_graph_and_twice():
 
 
 @pytest.mark.gpu
-def test_results_do_not_change_from_run_to_run():
-    args = _call_inputs((40, 6, 60, 61))
+@pytest.mark.parametrize("shape", [(40, 6, 60, 61), (8, 6, 60, 61)])
+def test_results_do_not_change_from_run_to_run(shape):
+    args = _call_inputs(shape)
     want = _all_calls(*args)
     for _ in range(5):
         for x, y in zip(_all_calls(*args), want):
