@@ -76,6 +76,10 @@ int ur5_policy_prefer_loss_grad(const ur5_rows* r, const ur5_prefer* p, float* l
    A group whose largest magnitude is below 1e-30 is 0; one that holds an infinity or a NaN stands for NaN throughout. Codes behind a plane's end are 0. */
 int ur5_act8_pack(const void* x, int dtype, int64_t planes, int64_t size, int8_t* codes, float* scales, int device, void* stream);
 int ur5_act8_unpack(const int8_t* codes, const float* scales, int64_t planes, int64_t size, void* x, int dtype, int device, void* stream);
+/* ReLU that leaves a bit per value for its backward pass: y = x <= 0 ? 0 : x (a NaN stays) of `count` neighbouring values, dx = dy where x passed (not x <= 0), 0 elsewhere whatever dy
+   holds. bits: ceil(count / 512) * 64 bytes, 8-byte aligned, to be read by ur5_act8_relu_grad of the same count and dtype only. Inputs and outputs may not overlap. */
+int ur5_act8_relu(const void* x, int dtype, int64_t count, void* y, uint64_t* bits, int device, void* stream);
+int ur5_act8_relu_grad(const void* dy, int dtype, const uint64_t* bits, int64_t count, void* dx, int device, void* stream);
 /* weight gradient of a pointwise (1 x 1) convolution from its checkpointed input: codes / scales of x [n][cin][size], dy [n][cout][size] (dense, dtype) ->
    dw [cout][cin] = sum over images and pixels of dy x, db [cout] = sum of dy (NULL: not wanted), both fp32; an infinity in dy makes its row of dw NaN. work: ur5_act8_wgrad_work_bytes(...) bytes, 16-byte aligned. */
 int64_t ur5_act8_wgrad_work_bytes(int64_t n, int64_t cin, int64_t cout, int64_t size);

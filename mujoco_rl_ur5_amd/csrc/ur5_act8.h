@@ -129,6 +129,65 @@ template <typename T, typename Past> __global__ void __launch_bounds__(THREADS) 
   }
 }
 
+// ---- ReLU whose backward pass needs a bit per value: 64 neighbouring lanes hold 64 PER values, word i of theirs has a bit per lane, for value i of each. Bound by memory: 2 x 4 (2)
+// + 1/8 bytes per value in both directions (41 M fp32 values, one MI355X: 53 us each way, 6.3 TB/s).
+template <typename T> struct Run { long long at; int left; long long word; };   // this thread's values: the first, how many exist, and the first word of its wavefront
+template <typename T> __device__ __forceinline__ Run<T> run_of(int k, long long count) {
+  const long long wave = ((long long)blockIdx.x * 2 + k) * (THREADS / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  constexpr int PER = Lane<T>::PER;
+  const long long at = (wave * 64 + (threadIdx.x & 63)) * PER;
+  return Run<T>{at, (int)min((long long)PER, max(0ll, count - at)), wave * 64 * PER < count ? wave * PER : -1};
+}
+template <typename T> __device__ __forceinline__ void take_some(const typename T::raw* p, int left, float* v) {
+  if (left == Lane<T>::PER) take(T{}, p, v);
+  else for (int i = 0; i < Lane<T>::PER; i++) v[i] = i < left ? widen(T{}, p[i]) : 0.f;
+}
+template <typename T, typename Past> __device__ __forceinline__ void put_some(typename T::raw* p, int left, const float* v, Past past) {
+  if (left == Lane<T>::PER) put(T{}, p, v, past);
+  else for (int i = 0; i < Lane<T>::PER; i++) if (i < left) p[i] = narrow(T{}, v[i]);
+}
+template <typename T, typename Past> __global__ void __launch_bounds__(THREADS) ur5_act8_relu(const typename T::raw* x, long long count, typename T::raw* y, uint64_t* bits) {
+  constexpr int PER = Lane<T>::PER;
+  float v[2][PER];
+#pragma unroll
+  for (int k = 0; k < 2; k++) {
+    const Run<T> r = run_of<T>(k, count);
+    take_some<T>(x + r.at, r.left, v[k]);
+  }
+#pragma unroll
+  for (int k = 0; k < 2; k++) {
+    const Run<T> r = run_of<T>(k, count);
+    if (r.word < 0) return;                                   // (a wavefront together)
+    uint64_t mine = 0;
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+      const bool passes = !(v[k][i] <= 0.f);                  // a NaN passes
+      const uint64_t word = __ballot(passes);
+      if ((threadIdx.x & 63) == i) mine = word;
+      v[k][i] = passes ? v[k][i] : 0.f;
+    }
+    put_some<T>(y + r.at, r.left, v[k], Past{});
+    if ((threadIdx.x & 63) < PER) bits[r.word + (threadIdx.x & 63)] = mine;
+  }
+}
+template <typename T, typename Past> __global__ void __launch_bounds__(THREADS) ur5_act8_relu_grad(const typename T::raw* dy, const uint64_t* bits, long long count, typename T::raw* dx) {
+  constexpr int PER = Lane<T>::PER;
+  float v[2][PER];
+#pragma unroll
+  for (int k = 0; k < 2; k++) {
+    const Run<T> r = run_of<T>(k, count);
+    take_some<T>(dy + r.at, r.left, v[k]);
+  }
+#pragma unroll
+  for (int k = 0; k < 2; k++) {
+    const Run<T> r = run_of<T>(k, count);
+    if (r.word < 0) return;
+#pragma unroll
+    for (int i = 0; i < PER; i++) v[k][i] = bits[r.word + i] >> (threadIdx.x & 63) & 1 ? v[k][i] : 0.f;
+    put_some<T>(dx + r.at, r.left, v[k], Past{});
+  }
+}
+
 // ---- weight gradient: dw[o][c] = sum over (image, pixel) of dy[o] x[c], a matrix product whose long axis is the pixels (both operands have them neighbouring).
 // Codes are small integers, exact in 16-bit floats, and a group's scale is a factor of 64 pixels of one input channel: v_mfma_f32_32x32x16 runs over the 64 pixels on
 // plain codes, and its 32 x 32 result is multiplied by the scales once -- a lane holds one column (one input channel) of it, so the scale is one register.

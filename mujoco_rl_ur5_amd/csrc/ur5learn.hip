@@ -302,6 +302,39 @@ int ur5_act8_unpack(const int8_t* codes, const float* scales, int64_t planes, in
   return launched(__func__);
 }
 
+static const char* check_relu(int dtype, int64_t count) {
+  if (dtype != UR5_F32 && dtype != UR5_F16 && dtype != UR5_BF16) return "dtype must be UR5_F32, UR5_F16 or UR5_BF16";
+  if (count < 0 || count > MOST_LAUNCHED * 2 * ur5act8::THREADS * ur5act8::Lane<f32_t>::PER) return "count must be at least 0 and below 2^35 - 2047";
+  return nullptr;
+}
+static unsigned relu_grid(int64_t count, int per) { return (unsigned)((count + 2 * ur5act8::THREADS * per - 1) / (2 * ur5act8::THREADS * per)); }
+int ur5_act8_relu(const void* x, int dtype, int64_t count, void* y, uint64_t* bits, int device, void* stream) {
+  CHECK(check_relu(dtype, count));
+  if (!count) return 0;
+  if (!x || !y || !bits || ((uintptr_t)bits & 7)) return fail(UR5_ERR_ARG, __func__, "x, y and bits (8-byte aligned) are needed");
+  ON(device);
+  by_type(dtype, [&](auto t) {
+    using T = decltype(t);
+    by_flag(count * 2 * (int64_t)sizeof(typename T::raw) > CACHE_BYTES, [&](auto p) {
+      ur5act8::ur5_act8_relu<T, decltype(p)><<<relu_grid(count, ur5act8::Lane<T>::PER), ur5act8::THREADS, 0, (hipStream_t)stream>>>((const typename T::raw*)x, count, (typename T::raw*)y, bits);
+    });
+  });
+  return launched(__func__);
+}
+int ur5_act8_relu_grad(const void* dy, int dtype, const uint64_t* bits, int64_t count, void* dx, int device, void* stream) {
+  CHECK(check_relu(dtype, count));
+  if (!count) return 0;
+  if (!dy || !dx || !bits || ((uintptr_t)bits & 7)) return fail(UR5_ERR_ARG, __func__, "dy, dx and bits (8-byte aligned) are needed");
+  ON(device);
+  by_type(dtype, [&](auto t) {
+    using T = decltype(t);
+    by_flag(count * 2 * (int64_t)sizeof(typename T::raw) > CACHE_BYTES, [&](auto p) {
+      ur5act8::ur5_act8_relu_grad<T, decltype(p)><<<relu_grid(count, ur5act8::Lane<T>::PER), ur5act8::THREADS, 0, (hipStream_t)stream>>>((const typename T::raw*)dy, bits, count, (typename T::raw*)dx);
+    });
+  });
+  return launched(__func__);
+}
+
 // ---- weight gradient: how the work is split. Tiles of 128 output x 256 input channels (of half the outputs, and of half or a quarter of the inputs where there are no more),
 // and as many ranges of the pixels as give every CU a workgroup (two of the smaller ones): less than 8, or a multiple of 8, one set per XCD. A larger tile reads and converts
 // each operand less often: 256 -> 512 channels 183 us with 128 x 256, 229 with 128 x 128, 233 with 64 x 256. One that reaches past the channels multiplies for nothing: 64 -> 128

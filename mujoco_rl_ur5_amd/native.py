@@ -24,7 +24,7 @@ EXPORTS = ["ur5_last_error", "ur5_create", "ur5_destroy", "ur5_num_envs", "ur5_n
 TEST_EXPORTS = ["ur5_forward_debug", "ur5_set_step_cap_dev", "ur5_model_uploads"]   # include/ur5sim_test.h: introspection for tests/ and tools/, not part of the boundary
 
 LEARN_EXPORTS = ["ur5_policy_work_bytes", "ur5_policy_sample", "ur5_policy_logp", "ur5_policy_clip_loss", "ur5_policy_clip_grad", "ur5_policy_clip_loss_grad",
-                 "ur5_policy_prefer_loss", "ur5_policy_prefer_grad", "ur5_policy_prefer_loss_grad", "ur5_act8_pack", "ur5_act8_unpack", "ur5_act8_wgrad_work_bytes", "ur5_act8_wgrad"]   # include/ur5learn.h
+                 "ur5_policy_prefer_loss", "ur5_policy_prefer_grad", "ur5_policy_prefer_loss_grad", "ur5_act8_pack", "ur5_act8_unpack", "ur5_act8_relu", "ur5_act8_relu_grad", "ur5_act8_wgrad_work_bytes", "ur5_act8_wgrad"]   # include/ur5learn.h
 
 
 class Config(C.Structure):
@@ -126,6 +126,8 @@ def load(path=None):
         L.ur5_policy_prefer_loss_grad.argtypes = [rows, vp, vp, vp, vp]
         L.ur5_act8_pack.argtypes = [vp, i32, i64, i64, vp, vp, i32, vp]
         L.ur5_act8_unpack.argtypes = [vp, vp, i64, i64, vp, i32, i32, vp]
+        L.ur5_act8_relu.argtypes = [vp, i32, i64, vp, vp, i32, vp]
+        L.ur5_act8_relu_grad.argtypes = [vp, i32, vp, i64, vp, i32, vp]
         L.ur5_act8_wgrad_work_bytes.argtypes, L.ur5_act8_wgrad_work_bytes.restype = [i64] * 4, i64
         L.ur5_act8_wgrad.argtypes = [vp, vp, vp, i32, i64, i64, i64, i64, vp, vp, vp, i64, i32, vp]
     _libs[path] = L

@@ -20,6 +20,10 @@ def test_entry_points_refuse_bad_arguments():
         assert lib.ur5_act8_pack(a["x"], a["dtype"], a["planes"], a["size"], a["codes"], a["scales"], 0, None) == -1, change
         assert lib.ur5_act8_unpack(a["codes"], a["scales"], a["planes"], a["size"], a["x"], a["dtype"], 0, None) == -1 and lib.ur5_last_error().startswith(b"ur5_act8_unpack"), change
     assert lib.ur5_act8_pack(4096, 0, 1 << 20, 64 * 600, 4096, 4096, 0, None) == -1                          # more groups than one launch takes
+    for change in (dict(x=None), dict(dtype=3), dict(size=-1), dict(size=1 << 36), dict(codes=None), dict(codes=4100), dict(scales=None)):
+        a = {**ok, **change}
+        assert lib.ur5_act8_relu(a["x"], a["dtype"], a["size"], a["scales"], a["codes"], 0, None) == -1, change
+        assert lib.ur5_act8_relu_grad(a["x"], a["dtype"], a["codes"], a["size"], a["scales"], 0, None) == -1 and lib.ur5_last_error().startswith(b"ur5_act8_relu_grad"), change
     need = lib.ur5_act8_wgrad_work_bytes(2, 3, 5, 100)
     assert need > 0 and lib.ur5_act8_wgrad_work_bytes(2, 0, 5, 100) == 0 and lib.ur5_act8_wgrad_work_bytes(2, 1 << 17, 5, 100) == 0
     ok = dict(codes=4096, scales=4096, dy=4096, dtype=0, n=2, cin=3, cout=5, size=100, dw=4096, db=4096, work=4096, bytes=need)
@@ -31,7 +35,7 @@ def test_entry_points_refuse_bad_arguments():
 
 def test_no_cpu_fallback():
     x = torch.zeros(2, 3, 8)
-    for call in (lambda: checkpoint8.pack(x), lambda: checkpoint8.pointwise_conv(x, torch.zeros(4, 3))):
+    for call in (lambda: checkpoint8.pack(x), lambda: checkpoint8.pointwise_conv(x, torch.zeros(4, 3)), lambda: checkpoint8.relu(x)):
         with pytest.raises(ValueError, match="no CPU fallback"):
             call()
 
@@ -378,12 +382,68 @@ def test_pointwise_conv_of_an_empty_batch():
     assert y.shape == (0, 7, 3, 4) and dx.shape == x.shape and torch.equal(dw, torch.zeros_like(w)) and torch.equal(db, torch.zeros_like(b))
 
 
-def test_relu_passes_what_the_plain_one_passes():
-    x = torch.tensor([-1.0, 0.0, 2.0, math.nan, -math.inf, math.inf], requires_grad=True)
-    for up in (torch.full((6,), 3.0), torch.full((6,), math.inf), torch.full((6,), math.nan)):
-        got, = torch.autograd.grad(checkpoint8.relu(x), x, up)
-        want, = torch.autograd.grad(torch.relu(x), x, up)
-        assert torch.equal(torch.nan_to_num(got, nan=7.0), torch.nan_to_num(want, nan=7.0))
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("count", [1, 3, 7, 8, 255, 256, 257, 511, 512, 513, 1024, 1025, 2047, 2049, 4100, 70001])
+def test_relu_is_the_plain_one(count, dtype):
+    """Value for value, whatever x and dy hold, from an address that is a multiple of the element only, and nothing behind the last value is touched."""
+    g = torch.Generator().manual_seed(count)
+    special = torch.tensor([0.0, -0.0, math.nan, math.inf, -math.inf, torch.finfo(dtype).smallest_normal / 4, -torch.finfo(dtype).smallest_normal / 4, torch.finfo(dtype).max])
+    mixed = lambda: torch.where(torch.rand(count, generator=g) < 0.2, special[torch.randint(0, 8, (count,), generator=g)], torch.randn(count, generator=g))  # noqa: E731
+    x, dy = mixed().to(dtype).cuda(), mixed().to(dtype).cuda()
+    leaf = x.clone().requires_grad_()
+    want = torch.relu(leaf)
+    want_dx, = torch.autograd.grad(want, leaf, dy)
+    same = lambda a, b: torch.equal(torch.nan_to_num(a.float(), nan=7.0, posinf=8.0, neginf=9.0), torch.nan_to_num(b.float(), nan=7.0, posinf=8.0, neginf=9.0)) and bool((a.isnan() == b.isnan()).all())  # noqa: E731
+    for move in (0, 1):
+        held = torch.zeros(count + 2, dtype=dtype, device="cuda")
+        held[move:move + count] = x
+        part = held[move:move + count].requires_grad_()
+        y = checkpoint8.relu(part)
+        dx, = torch.autograd.grad(y, part, dy)
+        assert same(y.detach(), want.detach()) and same(dx, want_dx)
+    lib, index = native.load(), x.get_device()
+    out, bits = torch.full((count + 3,), 5.0, dtype=dtype, device="cuda"), torch.full((-(-count // 512) * 8 + 2,), 77, dtype=torch.int64, device="cuda")
+    code = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}[dtype]
+    assert lib.ur5_act8_relu(x.data_ptr(), code, count, out.data_ptr(), bits.data_ptr(), index, None) == 0
+    assert lib.ur5_act8_relu_grad(dy.data_ptr(), code, bits.data_ptr(), count, out.data_ptr(), index, None) == 0
+    torch.cuda.synchronize()
+    assert same(out[:count], want_dx) and (out[count:] == 5).all() and (bits[-2:] == 77).all()
+
+
+@pytest.mark.gpu
+def test_relu_formats_streams_and_graphs():
+    g = torch.Generator().manual_seed(12)
+    x, dy = torch.randn(3, 20, 9, 11, generator=g).cuda(), torch.randn(3, 20, 9, 11, generator=g).cuda()
+    want, want_dx = torch.relu(x), dy * (x > 0)
+    for form in (torch.contiguous_format, torch.channels_last):
+        for dy_form in (torch.contiguous_format, torch.channels_last):
+            leaf = x.contiguous(memory_format=form).requires_grad_()
+            y = checkpoint8.relu(leaf)
+            dx, = torch.autograd.grad(y, leaf, dy.contiguous(memory_format=dy_form))
+            assert torch.equal(y.detach(), want) and torch.equal(dx, want_dx) and y.is_contiguous(memory_format=form)
+    leaf = x.transpose(1, 3).requires_grad_()
+    dx, = torch.autograd.grad(checkpoint8.relu(leaf), leaf, dy.transpose(1, 3))
+    assert torch.equal(dx, want_dx.transpose(1, 3))
+    empty = torch.empty(0, 3).cuda().requires_grad_()
+    assert torch.autograd.grad(checkpoint8.relu(empty).sum(), empty)[0].shape == (0, 3)
+    late = torch.cuda.Stream()
+    with torch.cuda.stream(late):
+        torch.cuda._sleep(5_000_000)
+        moved = checkpoint8.relu(x.clone())
+    torch.cuda.synchronize()
+    assert torch.equal(moved, want)
+    held, graph = x.clone(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = checkpoint8.relu(held)
+    for k in range(3):
+        held.copy_(torch.randn(x.shape, generator=g))
+        graph.replay()
+        other = torch.relu(held)
+        torch.cuda.synchronize()
+        assert torch.equal(out, other)
+    with pytest.raises(TypeError):
+        checkpoint8.relu(x.double())
 
 
 @pytest.mark.gpu
