@@ -25,27 +25,41 @@ def _float_gpu(t, what):
         raise TypeError(f"{what} must be float32, float16 or bfloat16, not {t.dtype}")
 
 
-def _planes(shape):
-    """Planes of a tensor: groups never reach over a plane's end. [N, C, ...] has N C planes, a matrix its rows, a vector is one plane."""
-    if len(shape) > 2:
-        return shape[0] * shape[1]
-    return shape[0] if len(shape) == 2 else 1
+def _layout(shape):
+    """(planes, values of a plane, groups of a plane) of a tensor: groups never reach over a plane's end. [N, C, ...] has N C planes, a matrix its rows, a vector is one plane. A tensor
+    without values has no groups."""
+    planes = shape[0] * shape[1] if len(shape) > 2 else shape[0] if len(shape) == 2 else 1
+    count = shape.numel()
+    size = count // planes if planes else 0
+    return planes, size, -(-size // GROUP)
 
 
 class PackedActivation:
-    """Codes int8 [planes, groups, 64], scales float32 [planes, groups], and the shape and type that ``unpack`` restores."""
-    __slots__ = ("codes", "scales", "shape", "dtype")
+    """A checkpoint: ``codes`` int8 [planes, groups, 64], ``scales`` float32 [planes, groups], and the ``shape`` and ``dtype`` that ``unpack`` restores. Codes and, behind them, scales lie
+    in one tensor of bytes, ``data``: on a small activation a call takes as long as its allocations."""
+    __slots__ = ("data", "shape", "dtype", "planes", "size", "groups")
 
-    def __init__(self, codes, scales, shape, dtype):
-        self.codes, self.scales, self.shape, self.dtype = codes, scales, shape, dtype
+    def __init__(self, data, shape, dtype):
+        self.data, self.shape, self.dtype = data, shape, dtype
+        self.planes, self.size, self.groups = _layout(shape)
+
+    @property
+    def codes(self):
+        return self.data[:self.planes * self.groups * GROUP].view(torch.int8).view(self.planes, self.groups, GROUP)
+
+    @property
+    def scales(self):
+        return self.data[self.planes * self.groups * GROUP:].view(torch.float32).view(self.planes, self.groups)
+
+    def _pointers(self):
+        at = self.data.data_ptr()
+        return at, at + self.planes * self.groups * GROUP
 
     def unpack(self):
-        x = torch.empty(self.shape, dtype=self.dtype, device=self.codes.device)
-        count = x.numel()
-        if count:
-            planes, index = self.codes.shape[0], x.get_device()
-            _check(_library().ur5_act8_unpack(self.codes.data_ptr(), self.scales.data_ptr(), planes, count // planes, x.data_ptr(), DTYPES[self.dtype], index, _raw_stream(index)),
-                   "ur5_act8_unpack")
+        x = self.data.new_empty(self.shape, dtype=self.dtype)
+        if self.planes * self.groups:
+            index = x.get_device()
+            _check(_library().ur5_act8_unpack(*self._pointers(), self.planes, self.size, x.data_ptr(), DTYPES[self.dtype], index, _raw_stream(index)), "ur5_act8_unpack")
         return x
 
     def weight_grad(self, dy, bias=True):
@@ -53,17 +67,17 @@ class PackedActivation:
         and pixels, the same every time; an infinity in dy gives NaN. bias=False: (dw, None)."""
         _float_gpu(dy, "dy")
         shape = self.shape
-        if len(shape) < 3 or shape[1] == 0 or dy.dim() != len(shape) or dy.shape[0] != shape[0] or dy.shape[2:] != shape[2:] or dy.get_device() != self.codes.get_device():
-            raise ValueError(f"dy must be [N, O, ...] like the packed {tuple(shape)} on {self.codes.device}, not {tuple(dy.shape)} on {dy.device}")
+        if len(shape) < 3 or shape[1] == 0 or dy.dim() != len(shape) or dy.shape[0] != shape[0] or dy.shape[2:] != shape[2:] or dy.get_device() != self.data.get_device():
+            raise ValueError(f"dy must be [N, O, ...] like the packed {tuple(shape)} on {self.data.device}, not {tuple(dy.shape)} on {dy.device}")
         n, cin, cout = shape[0], shape[1], dy.shape[1]
         dw = torch.empty((cout, cin), dtype=torch.float32, device=dy.device)
         db = torch.empty(cout, dtype=torch.float32, device=dy.device) if bias else None
         if dy.numel() == 0:
             return dw.zero_(), db.zero_() if bias else None
         dy = dy.detach().contiguous()
-        size, index, lib = dy.numel() // (n * cout), dy.get_device(), _library()
+        size, index, lib = self.size, dy.get_device(), _library()
         work = torch.empty(max(1, lib.ur5_act8_wgrad_work_bytes(n, cin, cout, size)), dtype=torch.uint8, device=dy.device)
-        _check(lib.ur5_act8_wgrad(self.codes.data_ptr(), self.scales.data_ptr(), dy.data_ptr(), DTYPES[dy.dtype], n, cin, cout, size, dw.data_ptr(), db.data_ptr() if bias else None,
+        _check(lib.ur5_act8_wgrad(*self._pointers(), dy.data_ptr(), DTYPES[dy.dtype], n, cin, cout, size, dw.data_ptr(), db.data_ptr() if bias else None,
                                   work.data_ptr(), work.numel(), index, _raw_stream(index)), "ur5_act8_wgrad")
         return dw, db
 
@@ -75,16 +89,12 @@ def pack(x):
     shape = x.shape
     if not shape:
         raise ValueError("a scalar has no activations to pack")
-    count = x.numel()
-    planes = _planes(shape)
-    size = count // planes if planes else 0
-    groups = -(-size // GROUP)
-    codes = torch.empty((planes, groups, GROUP), dtype=torch.int8, device=x.device)
-    scales = torch.empty((planes, groups), dtype=torch.float32, device=x.device)
-    if count:
-        src, index = x.contiguous(), x.get_device()
-        _check(_library().ur5_act8_pack(src.data_ptr(), DTYPES[x.dtype], planes, size, codes.data_ptr(), scales.data_ptr(), index, _raw_stream(index)), "ur5_act8_pack")
-    return PackedActivation(codes, scales, shape, x.dtype)
+    planes, size, groups = _layout(shape)
+    data = torch.empty(planes * groups * (GROUP + 4), dtype=torch.uint8, device=x.device)
+    if planes * groups:
+        src, index, at = x.contiguous(), x.get_device(), data.data_ptr()
+        _check(_library().ur5_act8_pack(src.data_ptr(), DTYPES[x.dtype], planes, size, at, at + planes * groups * GROUP, index, _raw_stream(index)), "ur5_act8_pack")
+    return PackedActivation(data, shape, x.dtype)
 
 
 class _PointwiseConv(torch.autograd.Function):
@@ -95,22 +105,21 @@ class _PointwiseConv(torch.autograd.Function):
         y = torch.matmul(w, x.flatten(2).contiguous())
         if bias is not None:
             y = y + bias.view(1, -1, 1)
-        kept = pack(x)
-        ctx.save_for_backward(kept.codes, kept.scales, weight)
+        ctx.save_for_backward(pack(x).data, weight)
         ctx.shape, ctx.dtype, ctx.has_bias = x.shape, x.dtype, bias is not None
         return y.view(n, w.shape[0], *x.shape[2:])
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        codes, scales, weight = ctx.saved_tensors
+        data, weight = ctx.saved_tensors
         dx = dw = db = None
         cin, cout = ctx.shape[1], weight.shape[0]
         if ctx.needs_input_grad[0]:
             w = weight.reshape(cout, cin).t().contiguous().to(dy.dtype)                      # (under autocast the output, and so dy, has fewer bits than the input)
             dx = torch.matmul(w, dy.flatten(2).contiguous()).view(ctx.shape).to(ctx.dtype)
         if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
-            dw, db = PackedActivation(codes, scales, ctx.shape, ctx.dtype).weight_grad(dy, bias=ctx.has_bias)
+            dw, db = PackedActivation(data, ctx.shape, ctx.dtype).weight_grad(dy, bias=ctx.has_bias)
             dw = dw.view(weight.shape).to(weight.dtype)
             db = db.to(weight.dtype) if ctx.has_bias else None
         return dx, dw, db

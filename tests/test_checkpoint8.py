@@ -266,6 +266,9 @@ def _gradients(net, x, weight, context):
 class _PlainPacked(checkpoint8.PackedActivation):
     """The checkpoint by the plain definition."""
 
+    def __init__(self, codes, scales, shape, dtype):
+        super().__init__(torch.cat((codes.contiguous().view(torch.uint8).flatten(), scales.float().contiguous().view(torch.uint8).flatten())), shape, dtype)
+
     def unpack(self):
         size = math.prod(self.shape[min(2, len(self.shape) - 1):])
         return (self.codes.double() * self.scales[..., None].double()).reshape(self.codes.shape[0], -1)[:, :size].float().to(self.dtype).reshape(self.shape)
