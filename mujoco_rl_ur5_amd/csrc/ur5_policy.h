@@ -117,7 +117,7 @@ template <typename T> __device__ __forceinline__ bool action_counts(const Rows& 
 }
 
 // ---- the 8s of a piece. For every 8 pixels of every map of the piece that hold an allowed one: use(first action, allowed bits, fetch(first action)), or
-// part(first action, allowed bits, values that exist) where the mask ends inside the 8; none(piece, 8) for the others, once for all maps.
+// part(first action, allowed bits, values that exist) where the mask ends inside the 8; with NONE, none(piece, 8, map, step) for the others: every step-th map from that one on.
 // A thread fetches its next 8 before it uses one: what a workgroup does is a chain of latencies. Logits that may not be taken are not read: the allowed 8s of the piece's
 // pixels are listed in LDS once (the maps share them) and dealt to the threads from the list, so that no lane idles where the mask has holes.
 struct Piece { int first, pixels, map0, maps; };   // pixels first .. of maps map0 ..
@@ -156,7 +156,7 @@ template <typename A, typename F, typename U> __device__ __forceinline__ void in
     if (!again) return;
   }
 }
-template <bool MASK, typename F, typename U, typename P8, typename N> __device__ __forceinline__ void for_piece(const Rows& R, int row, int piece, F fetch, U use, P8 part, N none) {
+template <bool MASK, bool NONE, typename F, typename U, typename P8, typename N> __device__ __forceinline__ void for_piece(const Rows& R, int row, int piece, F fetch, U use, P8 part, N none) {
   const Piece P = piece_of(R, piece);
   struct At { int j; uint32_t allowed; };
   const auto fetch_at = [&](const At& a) { return fetch(a.j); };
@@ -170,7 +170,7 @@ template <bool MASK, typename F, typename U, typename P8, typename N> __device__
   const uint8_t* mask = R.mask + row * R.mask_stride + P.first;
   if (tail) {                       // a thread per map
     const uint32_t bits = allowed8(mask + P.pixels - tail, tail, false);
-    if (!bits) { if (threadIdx.x == 0) none(P, P.pixels / VEC); }
+    if (!bits) { if (NONE) none(P, P.pixels / VEC, threadIdx.x, THREADS); }
     else for (int m = threadIdx.x; m < P.maps; m += THREADS) part((P.map0 + m) * R.pixels + last, bits, tail);
   }
   // A small batch, cut into pieces of an 8 per thread: latency counts, so the logits are asked for together with their mask (17 masked f16 rows of 131 x 93, statistics and
@@ -186,6 +186,7 @@ template <bool MASK, typename F, typename U, typename P8, typename N> __device__
   __shared__ uint32_t list[MOST_PER_MASKED * THREADS];      // group of 8 << 8 | bits, in the order of the pixels
   __shared__ int4 share[MOST_PER_MASKED];                   // entries of the four wavefronts of each tile
   static_assert(THREADS / 64 == 4, "an int4 of wavefronts");
+  const bool narrow = P.pixels / VEC < THREADS;             // few 8s of many maps: all threads share each
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   uint32_t bits[MOST_PER_MASKED];
   int before[MOST_PER_MASKED];
@@ -198,8 +199,11 @@ template <bool MASK, typename F, typename U, typename P8, typename N> __device__
     const uint64_t some = __ballot(bits[t] != 0);
     before[t] = __builtin_amdgcn_mbcnt_hi((uint32_t)(some >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)some, 0));
     if (lane == 0) ((int*)&share[t])[wave] = __popcll(some);
-    if (in && !bits[t]) none(P, g);
+    if (NONE && in && !bits[t] && !narrow) none(P, g, 0, 1);
   }
+  if (NONE && narrow)
+    for (int i = threadIdx.x, groups = P.pixels / VEC; i < groups * P.maps; i += THREADS)
+      if (!allowed8(mask + i % groups * VEC, VEC, true)) none(P, i % groups, i / groups, P.maps);
   __syncthreads();
   int n = 0;
 #pragma unroll
@@ -353,10 +357,10 @@ template <typename T, bool MASK, bool REF, bool ENTROPY> __device__ __forceinlin
     if (MASK) { bar8(allowed, z); if (REF) bar8(allowed, q); }
     add8<REF, ENTROPY>(a, z, q, e);
   };
-  for_piece<MASK>(R, row, piece, [&](int j) { return Both<T, REF>(z_row, q_row, j, no{}); },
+  for_piece<MASK, false>(R, row, piece, [&](int j) { return Both<T, REF>(z_row, q_row, j, no{}); },
     [&](int, uint32_t allowed, const Both<T, REF>& b) { float z[VEC], q[VEC]; b.get(z, q); add(allowed, z, q); },
     [&](int j, uint32_t allowed, int left) { float z[VEC], q[VEC]; take8<T>(z_row + j, left, z); if (REF) take8<T>(q_row + j, left, q); add(allowed, z, q); },
-    [](const Piece&, int) {});
+    [](const Piece&, int, int, int) {});
   return join_workgroup(a, REF, ENTROPY);
 }
 
@@ -428,13 +432,15 @@ static __global__ void __launch_bounds__(THREADS) ur5_policy_loss(Terms t) { add
 template <typename T, bool MASK, bool REF, typename Past> __device__ __forceinline__ void grad_piece(const Rows& R, int row, int piece, Slope S, float factor, int a, void* grad, Past past) {
   typename T::raw* out = (typename T::raw*)grad + (long long)row * R.actions;
   const float zero[VEC] = {};
-  const auto clear = [&](const Piece& P, int g) {          // 8 pixels of all maps of the piece
+  const auto clear = [&](const Piece& P, int g, int map, int step) {   // 8 pixels of maps of the piece
     const int p = P.first + g * VEC, left = R.pixels - p;
-    for (int m = 0; m < P.maps; m++) put8<T>(out + (P.map0 + m) * R.pixels + p, left, left >= VEC, zero, past);
+    for (int m = map; m < P.maps; m += step) put8<T>(out + (P.map0 + m) * R.pixels + p, left, left >= VEC, zero, past);
   };
   if (!S.on) {                                             // zeros; the logits are not read
     const Piece P = piece_of(R, piece);
-    for (int g = threadIdx.x; g * VEC < P.pixels; g += THREADS) clear(P, g);
+    const int groups = (P.pixels + VEC - 1) / VEC;
+    if (groups < THREADS) for (int i = threadIdx.x; i < groups * P.maps; i += THREADS) clear(P, i % groups, i / groups, P.maps);
+    else for (int g = threadIdx.x; g < groups; g += THREADS) clear(P, g, 0, 1);
     return;
   }
   S.rs *= factor; S.take *= factor;
@@ -453,7 +459,7 @@ template <typename T, bool MASK, bool REF, typename Past> __device__ __forceinli
 #pragma unroll
       for (int i = 0; i < VEC; i++) g[i] += a - j == i ? S.take : 0.f;
   };
-  for_piece<MASK>(R, row, piece, [&](int j) { return Both<T, REF>(z_row, q_row, j, yes{}); },
+  for_piece<MASK, true>(R, row, piece, [&](int j) { return Both<T, REF>(z_row, q_row, j, yes{}); },
     [&](int j, uint32_t allowed, const Both<T, REF>& b) { float z[VEC], q[VEC], g[VEC]; b.get(z, q); slope(j, allowed, z, q, g); store8(T{}, out + j, g, past); },
     [&](int j, uint32_t allowed, int left) {
       float z[VEC], q[VEC], g[VEC];
@@ -538,21 +544,33 @@ static_assert(FEW <= THREADS, "one part of the counts");
 // ---- preference loss. Episodes are runs of rows: episode k holds the rows offsets[k] .. offsets[k + 1]. S_k = sum over its counting rows of logp - ref_logp,
 // margin_i = beta (S_2i - S_2i+1), loss = mean over pairs of (1 - eps) softplus(-margin) + eps softplus(margin).
 struct Prefer { const int64_t* action; const float* ref_logp; const int64_t* offsets; int pairs; double beta, eps; };
-// a workgroup per pair, a wavefront per row of it
-template <typename T> __global__ void __launch_bounds__(THREADS) ur5_policy_prefer_pairs(Rows R, Prefer P, const Part* parts, Slope* slopes, double* term, float* margin) {
+// the end of a row, by a wavefront: what it adds to its episode, in every lane; its slope's m and rs
+template <typename T> __device__ __forceinline__ double prefer_row(const Rows& R, const Prefer& P, const Part* parts, Slope* slopes, int row) {
+  const Sums a = join_row(parts + (size_t)row * R.pieces, R.pieces, false);
+  const double ls = log(a.s), l = (double)logit<T>(R, row, P.action[row]) - a.m - ls - P.ref_logp[row];
+  if ((threadIdx.x & 63) == 0) { slopes[row].m = a.m; slopes[row].rs = (float)(1 / a.s); }
+  return l;
+}
+// long episodes: all rows in a launch of their own, a wavefront each; what a row adds stays in its first record (10 000 rows of 2400 actions in one pair, us a call: 1985 with its workgroup alone, 99 so)
+template <typename T> __global__ void __launch_bounds__(THREADS) ur5_policy_prefer_rows(Rows R, Prefer P, Part* parts, Slope* slopes) {
+  const int row = blockIdx.x * WAVES + (threadIdx.x >> 6);
+  if (row >= R.rows || !slopes[row].on) return;
+  const double l = prefer_row<T>(R, P, parts, slopes, row);
+  if ((threadIdx.x & 63) == 0) parts[(size_t)row * R.pieces].sums.s = l;
+}
+// a workgroup per pair; of rows that are not ended yet a wavefront each
+template <typename T, bool ENDED> __global__ void __launch_bounds__(THREADS) ur5_policy_prefer_pairs(Rows R, Prefer P, const Part* parts, Slope* slopes, double* term, float* margin) {
   const int i = blockIdx.x, wave = threadIdx.x >> 6;
   int end[3];
   for (int k = 0; k < 3; k++) end[k] = (int)min(max((long long)P.offsets[2 * i + k], 0ll), (long long)R.rows);   // offsets outside the rows are taken as their ends
   double d = 0;
   for (int half = 0; half < 2; half++)
-    for (int row = end[half] + wave; row < end[half + 1]; row += WAVES) {
+    for (int row = end[half] + (ENDED ? (int)threadIdx.x : wave); row < end[half + 1]; row += ENDED ? THREADS : WAVES) {
       if (!slopes[row].on) continue;
-      const Sums a = join_row(parts + (size_t)row * R.pieces, R.pieces, false);
-      const double ls = log(a.s), l = (double)logit<T>(R, row, P.action[row]) - a.m - ls - P.ref_logp[row];
+      const double l = ENDED ? parts[(size_t)row * R.pieces].sums.s : prefer_row<T>(R, P, parts, slopes, row);
       d += half ? -l : l;
-      if ((threadIdx.x & 63) == 0) { slopes[row].m = a.m; slopes[row].rs = (float)(1 / a.s); }
     }
-  const double mg = P.beta * workgroup_sum((threadIdx.x & 63) == 0 ? d : 0.0);
+  const double mg = P.beta * workgroup_sum(ENDED || (threadIdx.x & 63) == 0 ? d : 0.0);
   const double up = 1 / (1 + exp(mg));                                       // sigmoid(-margin)
   const double soft = fmax(mg, 0.0) + log1p(exp(-fabs(mg)));                 // softplus(margin)
   if (threadIdx.x == 0) {
@@ -686,8 +704,8 @@ template <typename T, bool MASK> __global__ void __launch_bounds__(THREADS) ur5_
     draw8<T>(z_row, key, j, a, allowed, z, e, first, found, best);
     first = false;
   };
-  for_piece<MASK>(R, row, piece, [&](int j) { return fetch8<T>(z_row + j); }, [&](int j, uint32_t allowed, const Eight<T>& w) { float z[VEC]; unpack8(w, z); draw(j, allowed, z); },
-    [&](int j, uint32_t allowed, int left) { float z[VEC]; take8<T>(z_row + j, left, z); draw(j, allowed, z); }, [](const Piece&, int) {});
+  for_piece<MASK, false>(R, row, piece, [&](int j) { return fetch8<T>(z_row + j); }, [&](int j, uint32_t allowed, const Eight<T>& w) { float z[VEC]; unpack8(w, z); draw(j, allowed, z); },
+    [&](int j, uint32_t allowed, int left) { float z[VEC]; take8<T>(z_row + j, left, z); draw(j, allowed, z); }, [](const Piece&, int, int, int) {});
   const Sums sums = join_workgroup(a, false, false);   // (its barrier stands between the list and its readers)
   const int listed = found.listed;
   if (listed > LISTED) {                               // the others' bests, too

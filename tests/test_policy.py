@@ -168,7 +168,9 @@ def _at(x, a):
 def _close(got, want, tol, what):
     got, want = got.double(), want.double()
     tol = torch.as_tensor(tol, dtype=torch.float64, device=want.device) + want.abs() * half_step(torch.float32)
-    off = (got - want).abs() - tol
+    # results are float32: what lies beyond its range (a sum over an episode of logits of the type's lowest value, -3.4e38 each) rounds to an infinity of its sign, and no other
+    beyond = want.abs() > torch.finfo(torch.float32).max
+    off = torch.where(beyond, torch.where(got == want.sign() * math.inf, 0.0, math.inf), (got - want).abs() - tol)
     assert not torch.isnan(got).any() and (off <= 0).all(), f"{what}: off by {float((got - want).abs().max()):.3g}, {float(off.max()):.3g} over what it may be"
 
 
@@ -403,6 +405,22 @@ def test_both_sides_of_the_rule_for_few_rows(shape, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(6, 3000, 1, 1), (5, 700, 1, 2), (4, 3001, 1, 9), (3, 90, 3, 11), (30, 500, 2, 8)])
+def test_small_masks_of_many_maps(shape, dtype):
+    """Fewer pixels than a workgroup has threads, shared by many maps: every place that is not allowed still gets its zero."""
+    z, mask, ok, a, counts, old, adv, ref = _clip_case(shape, dtype, "random", True, seed=shape[1])
+    numbers, scale = dict(clip=0.2, kl_coef=0.5, entropy_coef=0.01), 64.0 if dtype == torch.float16 else 1.0
+    for held in (mask, mask[1:2]):                                  # (the second: one mask for all rows)
+        here = ok if held is mask else (held[:, None].expand(shape) & torch.isfinite(z)).reshape(shape[0], -1)
+        counts = (a >= 0) & (a < here.shape[1]) & _at(here, a)
+        torch.full((shape[0] * here.shape[1],), math.nan, dtype=dtype, device="cuda")                        # what the gradient's memory held before
+        got, grad = policy.clipped_policy_grad(z, a, old, adv, held, ref, grad_scale=scale, **numbers)
+        _check_clip(got, grad, _plain_clip(z, here, a, counts, old, adv, ref, **numbers), dtype, numbers, scale)
+        assert (grad.reshape(here.shape)[~here | ~counts[:, None]] == 0).all()
+
+
+@pytest.mark.gpu
 def test_many_short_rows():
     """More rows than one workgroup counts, in parts that end inside it."""
     for n, shape, kind in ((257, (2, 1, 3), "random"), (70_001, (1, 1, 5), "none"), (20_000, (2, 2, 2), "random")):
@@ -434,7 +452,9 @@ def _plain_prefer(z, ok, a, counts, ref_logp, offsets, beta, eps):
 @pytest.mark.parametrize("eps", [0.0, 0.1])
 @pytest.mark.parametrize("kind", MASKS)
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("shape,offsets", [((1, 1, 1, 1), [0, 0, 1]), ((4, 2, 5, 9), [0, 4, 4]), ((5, 6, 40, 40), [1, 2, 4, 4, 4]), ((67, 3, 9, 9), [0, 30, 65, 65, 66, 66, 66]), ((3, 1, 33, 67), [0, 1, 3])])
+@pytest.mark.parametrize("shape,offsets", [((1, 1, 1, 1), [0, 0, 1]), ((4, 2, 5, 9), [0, 4, 4]), ((5, 6, 40, 40), [1, 2, 4, 4, 4]), ((67, 3, 9, 9), [0, 30, 65, 65, 66, 66, 66]), ((3, 1, 33, 67), [0, 1, 3]),
+                                           ((70, 1, 5, 9), [3, 40, 69]), ((150, 2, 40, 40), [0, 20, 110, 110, 150]), ((4200, 1, 1, 7), list(range(0, 4201, 15)))],
+                         ids=lambda v: "x".join(map(str, v)) if isinstance(v, tuple) else f"{len(v) // 2}pairs")
 def test_preference_loss_and_gradient(shape, offsets, dtype, kind, eps):
     z, mask, ok = _inputs(shape, dtype, kind, seed=6)
     a, counts = _actions(ok)
@@ -443,9 +463,14 @@ def test_preference_loss_and_gradient(shape, offsets, dtype, kind, eps):
     want = _plain_prefer(z, ok, a, counts, rl, off, 0.4, eps)
     scale = 64.0 if dtype == torch.float16 else 1.0
     got, grad = policy.preference_grad(z, a, rl, off, mask, beta=0.4, label_smoothing=eps, grad_scale=scale)
-    per = 0.4 * SUM * shape[0]                                   # every row's log-probability may be SUM off
+    # every row's log-probability may be SUM off; and 64 bits hold a sum of n terms, in whatever order, to n 2^-53 of the sum of their sizes, here and in the plain form: that is below
+    # 1e-12, but for actions of the type's lowest logit, 3.4e38, which cancel between episodes
+    sizes = torch.where(counts, (_at(Plain(z, ok).logp, a) - rl.double()).abs(), 0.0)
+    pair = ((torch.searchsorted(off, torch.arange(shape[0]).cuda(), right=True) - 1) // 2).clamp(0, len(offsets) // 2 - 1)
+    per = 0.4 * (SUM * shape[0] + shape[0] * 2.0 ** -52 * torch.zeros(len(offsets) // 2, dtype=torch.float64, device="cuda").index_add_(0, pair, sizes))
     _close(got.margin, want["margin"], per, "margin")
-    _close(got.loss, want["loss"], per, "loss")
+    _close(got.loss, want["loss"], per.mean(), "loss")
+    per = per[pair][:, None]
     # the weight (at most beta / pairs) follows the margin with a slope of at most beta / 4 pairs, the probability is 2 SUM off
     tol = (5 * SUM + per) * want["made_of"] * scale + want["grad"].abs() * scale * half_step(dtype) * (1 + 1e-3) + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
     assert ((grad.reshape(want["grad"].shape).double() - want["grad"] * scale).abs() <= tol).all()
