@@ -34,6 +34,12 @@ def _layout(shape):
     return planes, size, -(-size // GROUP)
 
 
+def _smaller(t):
+    """Whether a checkpoint of ``t`` takes less memory: a plane of a few values still takes a whole group, and an expanded tensor holds less than its shape says."""
+    planes, _, groups = _layout(t.shape)
+    return planes * groups * (GROUP + 4) < min(t.numel() * t.element_size(), t.untyped_storage().nbytes())
+
+
 class PackedActivation:
     """A checkpoint: ``codes`` int8 [planes, groups, 64], ``scales`` float32 [planes, groups], and the ``shape`` and ``dtype`` that ``unpack`` restores. Codes and, behind them, scales lie
     in one tensor of bytes, ``data``: on a small activation a call takes as long as its allocations."""
@@ -105,21 +111,23 @@ class _PointwiseConv(torch.autograd.Function):
         y = torch.matmul(w, x.flatten(2).contiguous())
         if bias is not None:
             y = y + bias.view(1, -1, 1)
-        ctx.save_for_backward(pack(x).data, weight)
+        ctx.packed = _smaller(x)                                                             # (else its backward pass packs it)
+        ctx.save_for_backward(pack(x).data if ctx.packed else x, weight)
         ctx.shape, ctx.dtype, ctx.has_bias = x.shape, x.dtype, bias is not None
         return y.view(n, w.shape[0], *x.shape[2:])
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        data, weight = ctx.saved_tensors
+        kept, weight = ctx.saved_tensors
         dx = dw = db = None
         cin, cout = ctx.shape[1], weight.shape[0]
         if ctx.needs_input_grad[0]:
             w = weight.reshape(cout, cin).t().contiguous().to(dy.dtype)                      # (under autocast the output, and so dy, has fewer bits than the input)
             dx = torch.matmul(w, dy.flatten(2).contiguous()).view(ctx.shape).to(ctx.dtype)
         if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
-            dw, db = PackedActivation(data, ctx.shape, ctx.dtype).weight_grad(dy, bias=ctx.has_bias)
+            kept = PackedActivation(kept, ctx.shape, ctx.dtype) if ctx.packed else pack(kept)
+            dw, db = kept.weight_grad(dy, bias=ctx.has_bias)
             dw = dw.view(weight.shape).to(weight.dtype)
             db = db.to(weight.dtype) if ctx.has_bias else None
         return dx, dw, db
@@ -182,7 +190,7 @@ def _is_parameter(t):
 
 class saved_activations:
     """Context manager for a forward pass: floating-point GPU tensors of three or more dimensions and at least ``min_values`` values that autograd saves inside it are kept as 8-bit
-    checkpoints and restored when their backward runs. Parameters (leaves that want a gradient, frozen nn.Parameters), views of them and
+    checkpoints, where those are smaller, and restored when their backward runs. Parameters (leaves that want a gradient, frozen nn.Parameters), views of them and
     autocast's copies of the former are left alone; a weight that is computed from parameters is an activation here. In it, ``qnet``'s pointwise convolutions keep theirs for ``weight_grad`` and its ReLUs which values are positive (``relu``)."""
 
     def __init__(self, min_values=4096):
@@ -191,7 +199,7 @@ class saved_activations:
     def _pack(self, t):
         if not (t.is_cuda and t.dtype in DTYPES and t.dim() >= 3 and t.numel() >= self.min_values):
             return t
-        return t if _is_parameter(t) else pack(t)
+        return pack(t) if _smaller(t) and not _is_parameter(t) else t
 
     @staticmethod
     def _unpack(t):

@@ -378,6 +378,38 @@ def test_frozen_and_cast_parameters_are_not_packed():
 
 
 @pytest.mark.gpu
+def test_planes_of_a_few_values_are_kept_as_they_are():
+    """A plane takes a group of 64 codes at least: pooled features would grow by it. The weight gradient is that of the checkpoint all the same."""
+    x = torch.randn(64, 96, 1, 1, device="cuda").requires_grad_()
+    w = torch.randn(32, 96, device="cuda").requires_grad_()
+    up = torch.randn(64, 32, 1, 1, device="cuda")
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    with checkpoint8.saved_activations():
+        h = x * 1.0
+        y = checkpoint8.pointwise_conv(torch.sigmoid(h), w)
+    held = torch.cuda.memory_allocated() - before
+    assert held <= 4 * 4 * x.numel() + 2 * 4 * y.numel()
+    dx, dw = torch.autograd.grad(y, (x, w), up)
+    seen = torch.sigmoid(x.detach())
+    assert torch.equal(dw, checkpoint8.pack(seen).weight_grad(up)[0])
+    want = (w.t().contiguous() @ up.flatten(1).t().contiguous()).t().reshape(x.shape) * seen * (1 - seen)     # sigmoid's own output is not rounded
+    assert torch.allclose(dx, want, rtol=1e-4, atol=1e-5)
+
+
+@pytest.mark.gpu
+def test_expanded_tensors_are_kept_as_they_are():
+    x, gain = torch.randn(8, 16, 40, 40, device="cuda").requires_grad_(), torch.rand(1, 16, 1, 1, device="cuda").sqrt().expand(8, 16, 40, 40)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    with checkpoint8.saved_activations():
+        y = (x * gain).sum()
+    assert torch.cuda.memory_allocated() - before < 4096
+    dx, = torch.autograd.grad(y, x)
+    assert torch.equal(dx, gain)
+
+
+@pytest.mark.gpu
 def test_pointwise_conv_of_an_empty_batch():
     x, w, b = torch.empty(0, 5, 3, 4).cuda().requires_grad_(), torch.randn(7, 5).cuda().requires_grad_(), torch.randn(7).cuda().requires_grad_()
     y = checkpoint8.pointwise_conv(x, w, b)
