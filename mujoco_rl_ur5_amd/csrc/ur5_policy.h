@@ -620,8 +620,8 @@ __device__ __forceinline__ float unordered(int o) { return __int_as_float(o ^ ((
 __device__ __forceinline__ float below(double score) { return (float)score - (1e-4f + 1e-6f * fabsf((float)score)); }
 
 struct Best { double score; int at; };
-__device__ __forceinline__ void join_best(Best& b, int width) {
-  for (int o = width >> 1; o; o >>= 1) {
+__device__ __forceinline__ void join_best(Best& b) {   // over a wavefront, in every lane
+  for (int o = 32; o; o >>= 1) {
     const double s = __shfl_xor(b.score, o);
     const int i = __shfl_xor(b.at, o);
     if (better(s, i, b.score, b.at)) { b.score = s; b.at = i; }
@@ -709,14 +709,14 @@ template <typename T, bool MASK> __global__ void __launch_bounds__(THREADS) ur5_
   const Sums sums = join_workgroup(a, false, false);   // (its barrier stands between the list and its readers)
   const int listed = found.listed;
   if (listed > LISTED) {                               // the others' bests, too
-    join_best(best, 64);
+    join_best(best);
     if ((threadIdx.x & 63) == 0) wave[threadIdx.x >> 6] = best;
     __syncthreads();
     best = wave[threadIdx.x & (WAVES - 1)];
   }
   if (threadIdx.x >= 64) return;
   if ((int)threadIdx.x < listed) score<T>(z_row, key, found.at[threadIdx.x], best);
-  join_best(best, 64);
+  join_best(best);
   if (threadIdx.x) return;
   if (R.pieces == 1) write_draw<T>(R, row, sums.m, sums.s, best, action, logp);
   else draws[blockIdx.x] = Draw{best.score, sums.s, sums.m, best.at};
@@ -734,7 +734,7 @@ template <typename T> __global__ void __launch_bounds__(THREADS) ur5_policy_samp
     if (better(d.score, d.best, best.score, best.at)) best = Best{d.score, d.best};
   }
   join_lanes<64>(a, false, false);
-  join_best(best, 64);
+  join_best(best);
   if (lane == 0) write_draw<T>(R, row, a.m, a.s, best, action, logp);
 }
 
