@@ -33,7 +33,8 @@ typedef struct ur5_rows {
   int64_t work_bytes;
 } ur5_rows;
 
-/* mask_len: 0 without a mask; pairs: of the preference loss, 0 for the others */
+/* mask_len: 0 without a mask; pairs: of the preference loss, 0 for the clipped loss, -1 for ur5_policy_sample and ur5_policy_logp, which need less, and nothing (NULL) for short rows.
+   0 also for sizes that a call refuses. */
 int64_t ur5_policy_work_bytes(int64_t rows, int64_t actions, int64_t mask_len, int64_t pairs);
 
 /* action[i] ~ softmax(row i) among the allowed actions and its log-probability. The draw is a pure function of (offset, gids[i]): the noise of action j is the j-th number of

@@ -66,6 +66,8 @@ int64_t lay_out(const Rows& R, int64_t terms, void* base, Work* w) {
   if (w) *w = Work{(Part*)p, (Slope*)(p + parts), (double*)(p + parts + slopes), counting, counting + 1};
   return parts + slopes + sums + (1 + (n + THREADS - 1) / THREADS) * 4;
 }
+constexpr int64_t ENDS = -1;                         // in the place of pairs: sampling and log-probabilities, which leave records of rows of several pieces and nothing else
+int64_t need(const Rows& R, int64_t pairs) { return pairs != ENDS ? lay_out(R, pairs, nullptr, nullptr) : R.pieces > 1 ? (int64_t)R.rows * R.pieces * (int64_t)sizeof(Part) : 0; }
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 constexpr int64_t MOST = 0x7fffffff;
 constexpr int64_t MOST_LAUNCHED = (1 << 24) - 1;     // workgroups of 256 threads: a launch holds less than 2^32 threads
@@ -89,9 +91,10 @@ const char* check_rows(const ur5_rows* r, int64_t pairs, const Aim& aim, Rows* R
   if (r->stride < r->actions && r->rows > 1) return "the row stride is smaller than a row";
   if (r->ref && r->ref_stride < r->actions && r->rows > 1) return "the reference's row stride is smaller than a row";
   if (r->rows && !r->logits) return "no logits";
-  if ((r->rows || pairs) && (!r->work || !aligned16(r->work) || r->work_bytes < lay_out(*R, pairs, nullptr, nullptr))) return "the workspace is missing, not 16-byte aligned, or smaller than ur5_policy_work_bytes";
+  const int64_t bytes = r->rows || pairs > 0 ? need(*R, pairs) : 0;
+  if (bytes && (!r->work || !aligned16(r->work) || r->work_bytes < bytes)) return "the workspace is missing, not 16-byte aligned, or smaller than ur5_policy_work_bytes";
   R->logits = r->logits; R->ref = r->ref; R->mask = r->mask; R->stride = r->stride; R->ref_stride = r->ref_stride; R->mask_stride = r->mask_stride;
-  lay_out(*R, pairs, r->work, w);
+  lay_out(*R, pairs, r->work, w);                    // (the records come first)
   return nullptr;
 }
 
@@ -161,13 +164,16 @@ void clip_gradient(Rows R, const ur5_rows* r, const ur5_clip* c, const Terms& t,
 extern "C" {
 
 int64_t ur5_policy_work_bytes(int64_t rows, int64_t actions, int64_t mask_len, int64_t pairs) {
-  Rows R;
-  return pairs < 0 || check_size(rows, actions, mask_len, pairs, LOSS, &R) ? 0 : lay_out(R, pairs, nullptr, nullptr);
+  Rows R, L;
+  if (pairs < ENDS || check_size(rows, actions, mask_len, pairs, pairs == ENDS ? SAMPLE : LOSS, &R)) return 0;
+  if (pairs != ENDS) return need(R, pairs);
+  cut(rows, actions, mask_len, LOGP, &L);
+  return need(R.pieces > L.pieces ? R : L, ENDS);
 }
 
 int ur5_policy_sample(const ur5_rows* r, uint64_t offset, const int64_t* gids, int64_t* action, float* logp) {
   Rows R; Work w;
-  CHECK(check_rows(r, 0, SAMPLE, &R, &w));
+  CHECK(check_rows(r, ENDS, SAMPLE, &R, &w));
   if (!R.rows) return 0;
   if (!gids || !action || !logp) return fail(UR5_ERR_ARG, __func__, "gids, action and logp are needed");
   ON(r->device);
@@ -182,7 +188,7 @@ int ur5_policy_sample(const ur5_rows* r, uint64_t offset, const int64_t* gids, i
 
 int ur5_policy_logp(const ur5_rows* r, const int64_t* action, float* logp, float* entropy) {
   Rows R; Work w;
-  CHECK(check_rows(r, 0, LOGP, &R, &w));
+  CHECK(check_rows(r, ENDS, LOGP, &R, &w));
   if (!R.rows) return 0;
   if (!action || !logp) return fail(UR5_ERR_ARG, __func__, "action and logp are needed");
   ON(r->device);

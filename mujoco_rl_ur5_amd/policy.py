@@ -127,7 +127,9 @@ def _reference(ref, z, shape):
 
 
 def _work(z, mask, pairs=0):
-    return torch.empty(_library().ur5_policy_work_bytes(z.n, z.width, 0 if mask is None else mask.width, pairs), dtype=torch.uint8, device=z.tensor.device)
+    """The workspace, None where none is needed. pairs = -1: of sampling and log-probabilities."""
+    size = _library().ur5_policy_work_bytes(z.n, z.width, 0 if mask is None else mask.width, pairs)
+    return torch.empty(size, dtype=torch.uint8, device=z.tensor.device) if size else None
 
 
 def _rows(z, mask, ref, work):
@@ -136,7 +138,7 @@ def _rows(z, mask, ref, work):
     index = t.get_device()
     return _ROWS.pack(t.data_ptr(), 0 if ref is None else ref.tensor.data_ptr(), 0 if mask is None else mask.tensor.data_ptr(), z.stride, 0 if ref is None else ref.stride,
                       0 if mask is None or mask.n == 1 else mask.stride, z.n, z.width, 0 if mask is None else mask.width, DTYPES[t.dtype], index, _raw_stream(index),
-                      work.data_ptr(), work.numel())
+                      0 if work is None else work.data_ptr(), 0 if work is None else work.numel())
 
 
 def sample_actions(logits, seed, gids, round_index, mask=None, stream=SAMPLE_STREAM):
@@ -148,7 +150,7 @@ def sample_actions(logits, seed, gids, round_index, mask=None, stream=SAMPLE_STR
     m, g = _mask(mask, z), _vector(gids, z.n, torch.int64, t.get_device(), "gids")
     action = torch.empty(z.n, dtype=torch.int64, device=t.device)
     logp = torch.empty(z.n, dtype=torch.float32, device=t.device)
-    work = _work(z, m)
+    work = _work(z, m, -1)
     _check(_library().ur5_policy_sample(_rows(z, m, None, work), sharding.scene_key_offset(seed, round_index, stream), g.data_ptr(), action.data_ptr(), logp.data_ptr()),
            "ur5_policy_sample")
     return action, logp
@@ -162,7 +164,7 @@ def action_log_probs(logits, action, mask=None):
     m, a = _mask(mask, z), _vector(action, z.n, torch.int64, t.get_device(), "action")
     logp = torch.empty(z.n, dtype=torch.float32, device=t.device)
     entropy = torch.empty(z.n, dtype=torch.float32, device=t.device)
-    work = _work(z, m)
+    work = _work(z, m, -1)
     _check(_library().ur5_policy_logp(_rows(z, m, None, work), a.data_ptr(), logp.data_ptr(), entropy.data_ptr()), "ur5_policy_logp")
     return logp, entropy
 

@@ -38,13 +38,13 @@ def _good_rows(**kw):
     lib = native.load()
     n, a = kw.pop("rows", 4), kw.pop("actions", 90)
     d = dict(logits=4096, ref=None, mask=None, stride=a, ref_stride=0, mask_stride=0, rows=n, actions=a, mask_len=0, dtype=0, device=0, stream=None, work=4096,
-             work_bytes=max(16, lib.ur5_policy_work_bytes(n, a, 0, 1)))
+             work_bytes=max(16, lib.ur5_policy_work_bytes(n, a, 0, 1)))   # (most of all)
     d.update(kw)
     return native.Rows(*[d[f] for f, _ in native.Rows._fields_])
 
 
 @pytest.mark.parametrize("change", [dict(dtype=3), dict(dtype=-1), dict(rows=-1), dict(actions=0), dict(actions=1 << 31), dict(rows=1 << 26), dict(stride=89), dict(logits=None),
-                                    dict(work=None), dict(work=4100), dict(work_bytes=16), dict(mask=4096, mask_len=0), dict(mask=4096, mask_len=7),
+                                    dict(actions=90000, work=None), dict(actions=90000, work=4100), dict(actions=90000, work_bytes=16), dict(mask=4096, mask_len=0), dict(mask=4096, mask_len=7),
                                     dict(mask=4096, mask_len=45, mask_stride=-1), dict(ref=4096, ref_stride=1)])
 def test_entry_points_refuse_bad_rows(change):
     """Every check runs before the device is asked for anything: no pointer below is ever used."""
@@ -75,7 +75,8 @@ def test_entry_points_refuse_bad_numbers_and_missing_outputs():
     assert lib.ur5_policy_clip_loss(C.byref(r), clip(), None, 4096, 4096, 4096) == -1 and lib.ur5_policy_clip_grad(C.byref(r), clip(), None) == -1
     assert lib.ur5_policy_prefer_loss(C.byref(r), pref(), 4096, None) == -1 and lib.ur5_policy_prefer_grad(C.byref(r), pref(), None) == -1
     assert lib.ur5_policy_sample(C.byref(r), 0, None, 4096, 4096) == -1 and lib.ur5_policy_logp(C.byref(r), 4096, None, None) == -1 and lib.ur5_policy_sample(None, 0, 4096, 4096, 4096) == -1
-    assert all(lib.ur5_policy_work_bytes(*bad) == 0 for bad in ((-1, 5, 0, 0), (5, 0, 0, 0), (5, 6, 4, 0), (5, 6, -1, 0), (5, 6, 0, -1)))
+    assert all(lib.ur5_policy_work_bytes(*bad) == 0 for bad in ((-1, 5, 0, 0), (5, 0, 0, 0), (5, 6, 4, 0), (5, 6, -1, 0), (5, 6, 0, -2)))
+    assert lib.ur5_policy_work_bytes(5, 6, 0, -1) == 0 < lib.ur5_policy_work_bytes(5, 60000, 0, -1) < lib.ur5_policy_work_bytes(5, 60000, 0, 0)   # short rows: sampling and log-probabilities need none
 
 
 def test_sizes_past_one_launch_are_refused():
