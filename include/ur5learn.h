@@ -70,6 +70,7 @@ typedef struct ur5_prefer {
    Rows that do not count, or belong to no episode, add nothing. */
 int ur5_policy_prefer_loss(const ur5_rows* r, const ur5_prefer* p, float* loss, float* margin);
 int ur5_policy_prefer_grad(const ur5_rows* r, const ur5_prefer* p, void* grad);
+/* both at once, in two (few rows and pairs), three or four (long episodes) launches. */
 int ur5_policy_prefer_loss_grad(const ur5_rows* r, const ur5_prefer* p, float* loss, float* margin, void* grad);
 
 /* 8-bit activation checkpoints: planes [planes][size] of dtype become codes int8 [planes][groups][64] and scales float [planes][groups], groups = ceil(size / 64): scale = the group's

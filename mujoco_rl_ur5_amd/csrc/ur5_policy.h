@@ -544,47 +544,111 @@ static_assert(FEW <= THREADS, "one part of the counts");
 // ---- preference loss. Episodes are runs of rows: episode k holds the rows offsets[k] .. offsets[k + 1]. S_k = sum over its counting rows of logp - ref_logp,
 // margin_i = beta (S_2i - S_2i+1), loss = mean over pairs of (1 - eps) softplus(-margin) + eps softplus(margin).
 struct Prefer { const int64_t* action; const float* ref_logp; const int64_t* offsets; int pairs; double beta, eps; };
-// the end of a row, by a wavefront: what it adds to its episode, in every lane; its slope's m and rs
-template <typename T> __device__ __forceinline__ double prefer_row(const Rows& R, const Prefer& P, const Part* parts, Slope* slopes, int row) {
-  const Sums a = join_row(parts + (size_t)row * R.pieces, R.pieces, false);
-  const double ls = log(a.s), l = (double)logit<T>(R, row, P.action[row]) - a.m - ls - P.ref_logp[row];
-  if ((threadIdx.x & 63) == 0) { slopes[row].m = a.m; slopes[row].rs = (float)(1 / a.s); }
-  return l;
+// the end of a row that counts, by a wavefront, in every lane: what it adds to its episode, and its slope's m and rs
+struct PreferRow { double l; float m, rs; };
+template <typename T> __device__ __forceinline__ PreferRow prefer_row(const Rows& R, const Prefer& P, const Part* parts, int pieces, int row) {
+  const Sums a = join_row(parts + (size_t)row * pieces, pieces, false);
+  return PreferRow{(double)logit<T>(R, row, P.action[row]) - a.m - log(a.s) - P.ref_logp[row], a.m, (float)(1 / a.s)};
 }
-// long episodes: all rows in a launch of their own, a wavefront each; what a row adds stays in its first record (10 000 rows of 2400 actions in one pair, us a call: 1985 with its workgroup alone, 99 so)
+struct Ends { int at[3]; };            // a pair's rows: at[0] .. of the preferred episode, at[1] .. at[2] of the other; offsets outside the rows are taken as their ends
+__device__ __forceinline__ Ends ends_of(const Rows& R, const Prefer& P, int pair) {
+  Ends e;
+  for (int k = 0; k < 3; k++) e.at[k] = (int)min(max((long long)P.offsets[2 * pair + k], 0ll), (long long)R.rows);
+  return e;
+}
+// from the sum over a pair: its margin, its term of the loss, and d loss / d logp of the preferred episode's rows
+struct PairEnd { float margin, w; double term; };
+__device__ __forceinline__ PairEnd pair_end(const Prefer& P, double d) {
+  const double mg = P.beta * d, up = 1 / (1 + exp(mg));                      // sigmoid(-margin)
+  const double rest = log1p(exp(-fabs(mg)));                                 // softplus(x) = max(x, 0) + this, of margin and -margin
+  return PairEnd{(float)mg, (float)(-P.beta * ((1 - P.eps) * up - P.eps * (1 - up)) / P.pairs), (1 - P.eps) * (fmax(-mg, 0.0) + rest) + P.eps * (fmax(mg, 0.0) + rest)};
+}
+// long episodes: all rows in a launch of their own, a wavefront each; what a row adds stays in its first record (10 000 rows of 2400 actions in one pair, us a call: 1985 with its
+// workgroup alone, 99 so)
 template <typename T> __global__ void __launch_bounds__(THREADS) ur5_policy_prefer_rows(Rows R, Prefer P, Part* parts, Slope* slopes) {
   const int row = blockIdx.x * WAVES + (threadIdx.x >> 6);
   if (row >= R.rows || !slopes[row].on) return;
-  const double l = prefer_row<T>(R, P, parts, slopes, row);
-  if ((threadIdx.x & 63) == 0) parts[(size_t)row * R.pieces].sums.s = l;
+  const PreferRow end = prefer_row<T>(R, P, parts, R.pieces, row);
+  if (threadIdx.x & 63) return;
+  slopes[row].m = end.m; slopes[row].rs = end.rs;
+  parts[(size_t)row * R.pieces].sums.s = end.l;
 }
 // a workgroup per pair; of rows that are not ended yet a wavefront each
 template <typename T, bool ENDED> __global__ void __launch_bounds__(THREADS) ur5_policy_prefer_pairs(Rows R, Prefer P, const Part* parts, Slope* slopes, double* term, float* margin) {
-  const int i = blockIdx.x, wave = threadIdx.x >> 6;
-  int end[3];
-  for (int k = 0; k < 3; k++) end[k] = (int)min(max((long long)P.offsets[2 * i + k], 0ll), (long long)R.rows);   // offsets outside the rows are taken as their ends
+  const Ends e = ends_of(R, P, blockIdx.x);
   double d = 0;
   for (int half = 0; half < 2; half++)
-    for (int row = end[half] + (ENDED ? (int)threadIdx.x : wave); row < end[half + 1]; row += ENDED ? THREADS : WAVES) {
+    for (int row = e.at[half] + (ENDED ? threadIdx.x : threadIdx.x >> 6); row < e.at[half + 1]; row += ENDED ? THREADS : WAVES) {
       if (!slopes[row].on) continue;
-      const double l = ENDED ? parts[(size_t)row * R.pieces].sums.s : prefer_row<T>(R, P, parts, slopes, row);
+      double l;
+      if (ENDED) l = parts[(size_t)row * R.pieces].sums.s;
+      else {
+        const PreferRow end = prefer_row<T>(R, P, parts, R.pieces, row);
+        if ((threadIdx.x & 63) == 0) { slopes[row].m = end.m; slopes[row].rs = end.rs; }
+        l = end.l;
+      }
       d += half ? -l : l;
     }
-  const double mg = P.beta * workgroup_sum(ENDED || (threadIdx.x & 63) == 0 ? d : 0.0);
-  const double up = 1 / (1 + exp(mg));                                       // sigmoid(-margin)
-  const double soft = fmax(mg, 0.0) + log1p(exp(-fabs(mg)));                 // softplus(margin)
-  if (threadIdx.x == 0) {
-    margin[i] = (float)mg;
-    term[i] = (1 - P.eps) * (soft - mg) + P.eps * soft;
-  }
-  const float w = (float)(-P.beta * ((1 - P.eps) * up - P.eps * (1 - up)) / P.pairs);   // d loss / d logp of the preferred episode's rows
+  const PairEnd pair = pair_end(P, workgroup_sum(ENDED || (threadIdx.x & 63) == 0 ? d : 0.0));
+  if (threadIdx.x == 0) { margin[blockIdx.x] = pair.margin; term[blockIdx.x] = pair.term; }
   for (int half = 0; half < 2; half++)
-    for (int row = end[half] + threadIdx.x; row < end[half + 1]; row += THREADS) {
+    for (int row = e.at[half] + threadIdx.x; row < e.at[half + 1]; row += THREADS) {
       Slope& S = slopes[row];
-      S.take = half ? -w : w;
+      S.take = half ? -pair.w : pair.w;
       S.rs *= S.take;
       S.c0 = -1.f;
     }
+}
+// Few rows and pairs: the gradient ends them by itself, every workgroup its row's pair, the first one all of them for the loss. The sums run as in ur5_policy_prefer_pairs, wavefront
+// by wavefront: the same bits. 17 f16 rows of 131 x 93, us a call: 20.2 in three launches, 18.4 in two; 8 fp32 rows of 9600 in one pair 18.8, 16.2.
+template <typename T, bool MASK> __global__ void __launch_bounds__(THREADS) ur5_policy_prefer_few(Rows R, int pieces, Prefer P, const Part* parts, const Slope* slopes, float* loss, float* margin, float scale, const float* upstream, void* grad) {
+  const int block = (int)blockIdx.x - FIRST, wave = threadIdx.x >> 6;
+  if (block < 0) {
+    if (blockIdx.x) return;
+    __shared__ double l[FEW], term[FEW];
+    for (int row = wave; row < R.rows; row += WAVES) {
+      const double v = slopes[row].on ? prefer_row<T>(R, P, parts, pieces, row).l : 0.0;
+      if ((threadIdx.x & 63) == 0) l[row] = v;
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < P.pairs) {
+      const Ends e = ends_of(R, P, threadIdx.x);
+      double d[WAVES] = {};
+      for (int w = 0; w < WAVES; w++)
+        for (int half = 0; half < 2; half++)
+          for (int row = e.at[half] + w; row < e.at[half + 1]; row += WAVES) if (slopes[row].on) d[w] += half ? -l[row] : l[row];
+      const PairEnd pair = pair_end(P, ((d[0] + d[1]) + d[2]) + d[3]);
+      margin[threadIdx.x] = pair.margin;
+      term[threadIdx.x] = pair.term;
+    }
+    __syncthreads();
+    add_terms(Terms{term, P.pairs, nullptr, loss});
+    return;
+  }
+  const int mine = R.rows - 1 - block / R.pieces, piece = block % R.pieces;
+  int pair = 0;
+  Ends e{};
+  for (; pair < P.pairs; pair++) {
+    e = ends_of(R, P, pair);
+    if (mine >= e.at[0] && mine < e.at[2]) break;
+  }
+  __shared__ Slope S;
+  if (threadIdx.x == 0) S = Slope{};
+  __syncthreads();
+  if (pair < P.pairs && slopes[mine].on) {
+    double d = 0;
+    for (int half = 0; half < 2; half++)
+      for (int row = e.at[half] + wave; row < e.at[half + 1]; row += WAVES) {
+        if (!slopes[row].on) continue;
+        const PreferRow end = prefer_row<T>(R, P, parts, pieces, row);
+        d += half ? -end.l : end.l;
+        if (row == mine && (threadIdx.x & 63) == 0) { S.m = end.m; S.rs = end.rs; S.take = half ? -1.f : 1.f; S.c0 = -1.f; S.on = 1; }
+      }
+    const float w = pair_end(P, workgroup_sum((threadIdx.x & 63) == 0 ? d : 0.0)).w;
+    if (threadIdx.x == 0) { S.take *= w; S.rs *= S.take; }
+    __syncthreads();
+  }
+  grad_piece<T, MASK, false>(R, mine, piece, S, grad_factor(scale, upstream, nullptr), (int)P.action[mine], grad, no{});
 }
 
 // ---- log-probability of an action and entropy per row. logp 0 where the action lies outside the row (no action), -inf where it may not be taken; entropy 0 where

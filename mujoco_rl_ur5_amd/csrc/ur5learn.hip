@@ -142,6 +142,8 @@ void prefer_pairs(const Rows& R, int dtype, hipStream_t s, const Prefer& P, cons
     by_flag(ended, [&](auto e) { ur5_policy_prefer_pairs<decltype(t), decltype(e)::value><<<P.pairs, THREADS, 0, s>>>(R, P, w.parts, w.slopes, w.term, margin); });
   });
 }
+// rows that the gradient's workgroups end by themselves: FEW, or as many fewer as a lane has records of one
+bool few(const Rows& R) { return R.rows * (((int64_t)R.pieces + 63) / 64) <= FEW; }
 // a call over more memory than the caches hold
 bool past_caches(const Rows& R, int dtype) { return (int64_t)R.rows * R.actions * (dtype == UR5_F32 ? 4 : 2) * (R.ref ? 3 : 2) > CACHE_BYTES; }
 void gradient(Rows R, int dtype, hipStream_t s, const Terms& t, const int64_t* action, const Work& w, float scale, const float* upstream, void* grad) {
@@ -229,7 +231,7 @@ int ur5_policy_clip_loss_grad(const ur5_rows* r, const ur5_clip* c, float* loss,
   ON(r->device);
   const hipStream_t s = (hipStream_t)r->stream;
   const ClipOut out{logp, kl, entropy};
-  if (R.rows && R.rows * (((int64_t)R.pieces + 63) / 64) <= FEW && (!R.ref || c->kl_coef > 0) && !past_caches(R, r->dtype)) {
+  if (R.rows && few(R) && (!R.ref || c->kl_coef > 0) && !past_caches(R, r->dtype)) {
     const Clip C = clip_of(c);
     const int pieces = R.pieces;
     stats(R, r->dtype, s, Span{}, C.action, w);
@@ -275,6 +277,16 @@ int ur5_policy_prefer_loss_grad(const ur5_rows* r, const ur5_prefer* p, float* l
   R.ref = nullptr;
   ON(r->device);
   const hipStream_t s = (hipStream_t)r->stream;
+  if (R.rows && few(R) && p->pairs <= FEW && !past_caches(R, r->dtype)) {
+    const Prefer P = prefer_of(p);
+    const int pieces = R.pieces;
+    stats(R, r->dtype, s, Span{P.offsets, 2 * P.pairs}, P.action, w);
+    cut(R.rows, R.actions, R.mask ? R.pixels : 0, GRADIENT, &R);
+    by_type(r->dtype, [&](auto t) { by_flag(R.mask, [&](auto m) {
+      ur5_policy_prefer_few<decltype(t), decltype(m)::value><<<FIRST + R.rows * R.pieces, THREADS, 0, s>>>(R, pieces, P, w.parts, w.slopes, loss, margin, p->grad_scale, p->upstream, grad);
+    }); });
+    return launched(__func__);
+  }
   prefer_pairs(R, r->dtype, s, prefer_of(p), w, margin);
   gradient(R, r->dtype, s, Terms{w.term, (int)p->pairs, nullptr, loss}, p->action, w, p->grad_scale, p->upstream, grad);
   return launched(__func__);
