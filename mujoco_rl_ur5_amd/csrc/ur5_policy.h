@@ -617,6 +617,7 @@ template <typename T, bool MASK> __global__ void __launch_bounds__(THREADS) ur5_
       for (int w = 0; w < WAVES; w++)
         for (int half = 0; half < 2; half++)
           for (int row = e.at[half] + w; row < e.at[half + 1]; row += WAVES) if (slopes[row].on) d[w] += half ? -l[row] : l[row];
+      static_assert(WAVES == 4, "the order of workgroup_sum");
       const PairEnd pair = pair_end(P, ((d[0] + d[1]) + d[2]) + d[3]);
       margin[threadIdx.x] = pair.margin;
       term[threadIdx.x] = pair.term;
