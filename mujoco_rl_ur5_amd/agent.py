@@ -112,7 +112,7 @@ def color_jitter(rgb, generator=None, brightness=0.5, contrast=0.5, saturation=0
 
 
 def _saving(activations):
-    """The context of a forward pass whose backward pass follows: activations = None keeps them as they are, "int8" as 8-bit checkpoints (checkpoint8.saved_activations)."""
+    """The context of a forward pass whose backward pass follows: activations = None keeps them as they are, "int8" keeps the layers' inputs as 8-bit checkpoints (checkpoint8.saved_activations)."""
     if activations not in (None, "int8"):
         raise ValueError(f"activations must be None or 'int8', not {activations!r}")
     return contextlib.nullcontext() if activations is None else checkpoint8.saved_activations()

@@ -2,16 +2,19 @@
 instead of 4), as HIP kernels (include/ur5learn.h, csrc/ur5_act8.h).
 
 ``pack`` / ``PackedActivation.unpack`` are the checkpoint itself; ``PackedActivation.weight_grad`` is a pointwise convolution's weight gradient that reads the codes as they are;
-``pointwise_conv`` is such a layer; ``saved_activations`` keeps every activation that a network saves for its backward pass this way (``agent.Learner(activations="int8")``). The
-forward pass is unchanged; gradients see activations that are off by at most half a step, 1/254 of the largest of their 64 neighbours.
+``pointwise_conv`` is such a layer; ``saved_activations`` keeps the inputs of a network's layers this way between forward and backward pass (``agent.Learner(activations="int8")``). The
+forward pass is unchanged; the layers' gradients see inputs that are off by at most half a step, 1/254 of the largest of their 64 neighbours.
 
 Tensors are float32 / float16 / bfloat16 on the GPU; work is queued on the current stream of their device; there is no CPU fallback.
 """
 from __future__ import annotations
 
+import contextlib
 import threading
 
 import torch
+import torch.nn.functional as F
+from torch.overrides import TorchFunctionMode
 
 from .policy import DTYPES, _check, _gpu, _library, _raw_stream
 
@@ -188,16 +191,45 @@ def _is_parameter(t):
     return made is not None and made.name() == "ToCopyBackward0" and made.next_functions[0][0].name() == "torch::autograd::AccumulateGrad"
 
 
+# The layers whose inputs are packed: products and convolutions are linear in what their backward pass reads, normalisations read their input against its own mean and spread, pooling
+# asks for its shape alone. What other functions save stays as it is: autograd keeps a sigmoid's OUTPUT and multiplies by q (1 - q), an exp's or a softmax's likewise, and a log divides by
+# its input. Half a step is an unbounded share of those (0.0005 next to a 0.2 has code 0: no gradient at all). Of a layer, its input alone: not a normalisation's reciprocal spreads.
+_PRODUCTS = frozenset([torch.matmul, torch.mm, torch.bmm, torch.addmm, torch.baddbmm, torch.einsum] + [getattr(torch.Tensor, name) for name in "matmul __matmul__ __rmatmul__ mm bmm addmm baddbmm".split()])
+_LAYERS = frozenset(getattr(module, name) for module, names in (
+    (F, "conv1d conv2d conv3d conv_transpose1d conv_transpose2d conv_transpose3d linear batch_norm instance_norm group_norm layer_norm max_pool1d max_pool2d max_pool3d avg_pool1d avg_pool2d "
+        "avg_pool3d adaptive_avg_pool1d adaptive_avg_pool2d adaptive_avg_pool3d adaptive_max_pool1d adaptive_max_pool2d adaptive_max_pool3d"),
+    (torch, "batch_norm instance_norm group_norm layer_norm max_pool1d max_pool2d max_pool3d")) for name in names.split())
+
+
+class _Functions(TorchFunctionMode):
+    """Notes for the hooks below how many values the inputs of the layer or product that is running have. (A composite function, such as an attention module's, is seen as one: what runs
+    inside it is not.) The number, not the tensor: autocast and a layer's own reshaping hand autograd another one."""
+
+    def __torch_function__(self, func, types, args=(), kwargs=None):
+        kwargs = kwargs or {}
+        inputs = (args[0] if args else kwargs.get("input"),) if func in _LAYERS else (*args, *kwargs.values()) if func in _PRODUCTS else ()
+        before, _active.inputs = getattr(_active, "inputs", ()), [t.numel() for t in inputs if isinstance(t, torch.Tensor)]
+        try:
+            return func(*args, **kwargs)
+        finally:
+            _active.inputs = before
+
+
 class saved_activations:
-    """Context manager for a forward pass: floating-point GPU tensors of three or more dimensions and at least ``min_values`` values that autograd saves inside it are kept as 8-bit
-    checkpoints, where those are smaller, and restored when their backward runs. Parameters (leaves that want a gradient, frozen nn.Parameters), views of them and
-    autocast's copies of the former are left alone; a weight that is computed from parameters is an activation here. In it, ``qnet``'s pointwise convolutions keep theirs for ``weight_grad`` and its ReLUs which values are positive (``relu``)."""
+    """Context manager for a forward pass: the inputs of convolutions, matrix products, normalisations and poolings that autograd saves inside it -- floating-point GPU tensors of three or more
+    dimensions and at least ``min_values`` values -- are kept as 8-bit checkpoints, where those are smaller, and restored when their backward runs. What other functions save (a sigmoid's or
+    softmax's output, a logarithm's argument) is kept as it is, and so are a layer's weights and parameters (leaves that want a gradient, frozen nn.Parameters), views of them and
+    autocast's copies of the former; a factor of a product that is computed from parameters is an activation here. In it, ``qnet``'s pointwise convolutions keep theirs for ``weight_grad`` and its ReLUs which values are positive (``relu``).
+
+    A normalisation sees its input half a step off: where a group's values lie close together and far from 0, that is more of their spread than of themselves. What is kept must not be
+    changed in place before the backward pass; unlike without the context, that is not noticed."""
 
     def __init__(self, min_values=4096):
         self.min_values = int(min_values)
+        self._entered = []
 
     def _pack(self, t):
-        if not (t.is_cuda and t.dtype in DTYPES and t.dim() >= 3 and t.numel() >= self.min_values):
+        if not (t.is_cuda and t.dtype in DTYPES and t.dim() >= 3 and t.numel() >= self.min_values and t.numel() in getattr(_active, "inputs", ())):
             return t
         return pack(t) if _smaller(t) and not _is_parameter(t) else t
 
@@ -206,11 +238,13 @@ class saved_activations:
         return t.unpack() if isinstance(t, PackedActivation) else t
 
     def __enter__(self):
-        self._hooks = torch.autograd.graph.saved_tensors_hooks(self._pack, self._unpack)
-        self._hooks.__enter__()
+        inside = contextlib.ExitStack()
+        inside.enter_context(torch.autograd.graph.saved_tensors_hooks(self._pack, self._unpack))
+        inside.enter_context(_Functions())
+        self._entered.append(inside)
         _active.depth = getattr(_active, "depth", 0) + 1
         return self
 
     def __exit__(self, *exc):
         _active.depth -= 1
-        return self._hooks.__exit__(*exc)
+        return self._entered.pop().__exit__(*exc)
