@@ -116,7 +116,7 @@ class _PointwiseConv(torch.autograd.Function):
             y = y + bias.view(1, -1, 1)
         ctx.packed = _smaller(x)                                                             # (else its backward pass packs it)
         ctx.save_for_backward(pack(x).data if ctx.packed else x, weight)
-        ctx.shape, ctx.dtype, ctx.has_bias = x.shape, x.dtype, bias is not None
+        ctx.shape, ctx.dtype, ctx.bias_dtype = x.shape, x.dtype, None if bias is None else bias.dtype
         return y.view(n, w.shape[0], *x.shape[2:])
 
     @staticmethod
@@ -130,17 +130,17 @@ class _PointwiseConv(torch.autograd.Function):
             dx = torch.matmul(w, dy.flatten(2).contiguous()).view(ctx.shape).to(ctx.dtype)
         if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
             kept = PackedActivation(kept, ctx.shape, ctx.dtype) if ctx.packed else pack(kept)
-            dw, db = kept.weight_grad(dy, bias=ctx.has_bias)
+            dw, db = kept.weight_grad(dy, bias=ctx.bias_dtype is not None)
             dw = dw.view(weight.shape).to(weight.dtype)
-            db = db.to(weight.dtype) if ctx.has_bias else None
+            db = None if db is None else db.to(ctx.bias_dtype)
         return dx, dw, db
 
 
 def pointwise_conv(x, weight, bias=None):
     """1 x 1 convolution [N, C, ...] -> [N, O, ...] (weight [O, C] or [O, C, 1, 1]) whose input is kept in 8 bits for the weight gradient. Same result and input gradient as the
-    plain layer."""
+    plain layer. Under autocast, which decides the product's type, input and weight may differ in theirs; gradients come in the types of what they belong to."""
     _float_gpu(x, "x")
-    if x.dim() < 3 or weight.numel() != weight.shape[0] * x.shape[1] or weight.dtype != x.dtype or weight.device != x.device:
+    if x.dim() < 3 or weight.numel() != weight.shape[0] * x.shape[1] or weight.device != x.device or weight.dtype not in DTYPES or (weight.dtype != x.dtype and not torch.is_autocast_enabled("cuda")):
         raise ValueError(f"weight {tuple(weight.shape)} {weight.dtype} does not fit x {tuple(x.shape)} {x.dtype}")
     return _PointwiseConv.apply(x, weight, bias)
 

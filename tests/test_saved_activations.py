@@ -139,3 +139,53 @@ def test_the_context_knows_which_function_saves():
             torch.exp(x)
         torch.exp(x)
     assert len(seen) == 2 and not any(seen) and not checkpoint8.active()
+
+
+# ------------------------------------------------------------------ types
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("per_image", [False, True])
+def test_the_policy_network_under_autocast(dtype, per_image):
+    """Inside the network a 16-bit activation meets fp32 weights. Same output as without checkpoints, and gradients near those."""
+    import contextlib
+    torch.manual_seed(1)
+    net = qnet.MULTIDISCRETE_POLICY_RESNET(6).cuda().train()
+    x = torch.rand(3, 4, 40, 40, device="cuda")
+    up = torch.randn(3, 6, 40, 40, device="cuda")
+    out = []
+    for context in (contextlib.nullcontext(), checkpoint8.saved_activations()):
+        net.zero_grad(set_to_none=True)
+        with context, torch.autocast("cuda", dtype=dtype), (qnet.per_sample_statistics() if per_image else contextlib.nullcontext()):
+            y = net(x)
+        (y.float() * up).sum().backward()
+        out.append((y.detach().float(), y.dtype, {n: p.grad.clone() for n, p in net.named_parameters()}))
+    (y, t, grads), (y8, t8, grads8) = out
+    # both runs round every layer to the same 16-bit type; where the library adds in another order a rounding may fall the other way, a step of the type per layer
+    assert t == t8 and float((y - y8).norm() / y.norm()) < 8 * torch.finfo(dtype).eps
+    most = max(float(v.norm()) for v in grads.values())
+    for name, a in grads.items():
+        assert grads8[name].dtype == a.dtype == torch.float32
+        if float(a.norm()) > 1e-2 * most:
+            assert float((a - grads8[name]).norm() / a.norm()) < 0.2, name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("types", ["xh", "wh", "xw", "none"])
+def test_pointwise_conv_of_mixed_types_under_autocast(dtype, types):
+    g = torch.Generator().manual_seed(5)
+    x, w, b = torch.randn(3, 20, 9, 14, generator=g).cuda(), torch.randn(11, 20, generator=g).cuda(), torch.randn(11, generator=g).cuda()
+    x = (x.to(dtype) if "x" in types else x).requires_grad_()
+    w = (w.to(dtype) if "w" in types else w).requires_grad_()
+    b = b.requires_grad_()
+    up = torch.randn(3, 11, 9, 14, generator=g).cuda()
+    with torch.autocast("cuda", dtype=dtype):
+        y = checkpoint8.pointwise_conv(x, w, b)
+    grads = torch.autograd.grad(y, (x, w, b), up.to(y.dtype))
+    assert [t.dtype for t in grads] == [x.dtype, w.dtype, b.dtype]
+    want = torch.autograd.grad(F.conv2d(x.double(), w.double()[..., None, None], b.double()), (x, w, b), up.double())
+    for a, e in zip(grads, want):                               # inputs half a checkpoint's step off, products rounded to the type: a few per cent of the largest entry is far over both
+        assert float((a.double() - e.double()).abs().max()) < 0.03 * float(e.abs().max())
+    if x.dtype != w.dtype:
+        with pytest.raises(ValueError, match="does not fit"):   # without autocast nothing decides the product's type: refused, as the plain layer refuses it
+            checkpoint8.pointwise_conv(x, w, b)
