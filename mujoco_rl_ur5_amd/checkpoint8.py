@@ -182,6 +182,11 @@ def active():
     return getattr(_active, "depth", 0) > 0
 
 
+def active_for(x):
+    """Whether this thread is inside ``saved_activations`` and x is of the tensors that it is for."""
+    return active() and x.is_cuda and x.dtype in DTYPES
+
+
 def _is_parameter(t):
     """A parameter, a view of one, or its copy in another type (what autocast hands to a layer)."""
     source = t if t._base is None else t._base

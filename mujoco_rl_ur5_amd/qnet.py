@@ -57,7 +57,7 @@ def _conv1x1_as_gemm(conv, x):
     assert conv.kernel_size == (1, 1) and conv.stride == (1, 1) and conv.padding == (0, 0) and conv.dilation == (1, 1) and conv.groups == 1, conv
     if not (x.is_cuda or _FORCE_GEMM_1X1):   # on the host the reference's own operator (the CPU tests compare a 13-step Adam sequence with the reference to 2e-4)
         return conv(x)
-    if x.is_cuda and checkpoint8.active() and torch.is_grad_enabled():   # training from 8-bit activation checkpoints
+    if checkpoint8.active_for(x) and torch.is_grad_enabled():   # training from 8-bit activation checkpoints
         return checkpoint8.pointwise_conv(x, conv.weight, conv.bias)
     n, c, h, w = x.shape
     y = torch.matmul(conv.weight.view(conv.out_channels, c), x.reshape(n, c, h * w))
@@ -76,7 +76,7 @@ def _conv3x3_as_gemm(conv, x):
         return conv(x)
     n, c, h, w = x.shape
     cols = nn.functional.unfold(x, kernel_size=3, padding=1)                          # [N, 9 C, H W], rows ordered (channel, ky, kx) like weight.view(O, -1)
-    if x.is_cuda and checkpoint8.active() and torch.is_grad_enabled():
+    if checkpoint8.active_for(x) and torch.is_grad_enabled():
         return checkpoint8.pointwise_conv(cols, conv.weight.view(conv.out_channels, 9 * c)).view(n, conv.out_channels, h, w)
     return torch.matmul(conv.weight.view(conv.out_channels, 9 * c), cols).view(n, conv.out_channels, h, w)
 
@@ -102,7 +102,7 @@ class BasicBlock(nn.Module):
         self.conv3 = nn.Conv2d(inplanes, planes, kernel_size=1, stride=1) if inplanes != planes else None
 
     def forward(self, x):
-        relu = checkpoint8.relu if x.is_cuda and checkpoint8.active() else self.relu
+        relu = checkpoint8.relu if checkpoint8.active_for(x) else self.relu
         out = self.bn2(self.conv2(relu(self.bn1(self.conv1(x)))))
         skip = x if self.conv3 is None else _conv1x1_as_gemm(self.conv3, x)
         return relu(out + skip)

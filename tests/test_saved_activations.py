@@ -189,3 +189,16 @@ def test_pointwise_conv_of_mixed_types_under_autocast(dtype, types):
     if x.dtype != w.dtype:
         with pytest.raises(ValueError, match="does not fit"):   # without autocast nothing decides the product's type: refused, as the plain layer refuses it
             checkpoint8.pointwise_conv(x, w, b)
+
+
+@pytest.mark.gpu
+def test_a_network_of_another_type_is_left_alone():
+    torch.manual_seed(2)
+    block = qnet.BasicBlock(4, 6).cuda().double().train()
+    x = torch.randn(2, 4, 30, 30, device="cuda", dtype=torch.double).requires_grad_()
+    want = torch.autograd.grad(block(x).sum(), [x, *block.parameters()])
+    with checkpoint8.saved_activations():
+        y = block(x)
+    got = torch.autograd.grad(y.sum(), [x, *block.parameters()])
+    for a, b in zip(got, want):
+        assert torch.allclose(a, b, rtol=1e-9, atol=1e-9)
