@@ -142,6 +142,8 @@ def pointwise_conv(x, weight, bias=None):
     _float_gpu(x, "x")
     if x.dim() < 3 or weight.numel() != weight.shape[0] * x.shape[1] or weight.device != x.device or weight.dtype not in DTYPES or (weight.dtype != x.dtype and not torch.is_autocast_enabled("cuda")):
         raise ValueError(f"weight {tuple(weight.shape)} {weight.dtype} does not fit x {tuple(x.shape)} {x.dtype}")
+    if bias is not None and (not isinstance(bias, torch.Tensor) or bias.shape != weight.shape[:1] or bias.device != x.device or bias.dtype not in DTYPES):
+        raise ValueError(f"bias must be a [{weight.shape[0]}] tensor of float32, float16 or bfloat16 on {x.device}")
     return _PointwiseConv.apply(x, weight, bias)
 
 

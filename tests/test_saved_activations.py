@@ -202,3 +202,11 @@ def test_a_network_of_another_type_is_left_alone():
     got = torch.autograd.grad(y.sum(), [x, *block.parameters()])
     for a, b in zip(got, want):
         assert torch.allclose(a, b, rtol=1e-9, atol=1e-9)
+
+
+@pytest.mark.gpu
+def test_pointwise_conv_refuses_a_bias_that_does_not_fit():
+    x, w = torch.randn(2, 5, 3, 4).cuda(), torch.randn(7, 5).cuda()
+    for bias in (torch.zeros(1).cuda(), torch.zeros(5).cuda(), torch.zeros(7), torch.zeros(7, 1).cuda(), torch.zeros(7, dtype=torch.double).cuda(), torch.zeros(7, dtype=torch.long).cuda(), 0.5):
+        with pytest.raises(ValueError, match="bias"):
+            checkpoint8.pointwise_conv(x, w, bias)
