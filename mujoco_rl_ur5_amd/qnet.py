@@ -85,6 +85,13 @@ def _conv3x3(cin, cout):
     return nn.Conv2d(cin, cout, kernel_size=3, stride=1, padding=1, bias=False)
 
 
+class _ReLU(nn.ReLU):
+    """``nn.ReLU`` (the same module to hooks and checkpoints) that keeps a bit per value for its backward pass inside ``checkpoint8.saved_activations``."""
+
+    def forward(self, x):
+        return checkpoint8.relu(x) if checkpoint8.active_for(x) else super().forward(x)
+
+
 class BasicBlock(nn.Module):
     """Modules.py:92-142 -- two 3x3 convolutions with batch norm; a 1x1 convolution (with bias) on the skip path when the channel
     count changes. No stride, no down-sampling in this network."""
@@ -94,7 +101,7 @@ class BasicBlock(nn.Module):
         super().__init__()
         self.conv1 = _conv3x3(inplanes, planes)
         self.bn1 = _BatchNorm2d(planes)
-        self.relu = nn.ReLU(inplace=True)
+        self.relu = _ReLU(inplace=True)
         self.conv2 = _conv3x3(planes, planes)
         self.bn2 = _BatchNorm2d(planes)
         self.downsample = None
@@ -102,10 +109,9 @@ class BasicBlock(nn.Module):
         self.conv3 = nn.Conv2d(inplanes, planes, kernel_size=1, stride=1) if inplanes != planes else None
 
     def forward(self, x):
-        relu = checkpoint8.relu if checkpoint8.active_for(x) else self.relu
-        out = self.bn2(self.conv2(relu(self.bn1(self.conv1(x)))))
+        out = self.bn2(self.conv2(self.relu(self.bn1(self.conv1(x)))))
         skip = x if self.conv3 is None else _conv1x1_as_gemm(self.conv3, x)
-        return relu(out + skip)
+        return self.relu(out + skip)
 
 
 class Perception_Module(nn.Module):

@@ -210,3 +210,18 @@ def test_pointwise_conv_refuses_a_bias_that_does_not_fit():
     for bias in (torch.zeros(1).cuda(), torch.zeros(5).cuda(), torch.zeros(7), torch.zeros(7, 1).cuda(), torch.zeros(7, dtype=torch.double).cuda(), torch.zeros(7, dtype=torch.long).cuda(), 0.5):
         with pytest.raises(ValueError, match="bias"):
             checkpoint8.pointwise_conv(x, w, bias)
+
+
+# ------------------------------------------------------------------ modules
+@pytest.mark.gpu
+def test_module_hooks_run_inside_the_context():
+    torch.manual_seed(3)
+    block = qnet.BasicBlock(8, 8).cuda().train()
+    x = torch.randn(2, 8, 30, 30, device="cuda")
+    calls = []
+    block.relu.register_forward_hook(lambda m, i, o: calls.append(tuple(o.shape)))
+    block(x)
+    plain = list(calls)
+    with checkpoint8.saved_activations():
+        block(x)
+    assert len(plain) == 2 and calls[2:] == plain
