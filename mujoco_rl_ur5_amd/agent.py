@@ -26,6 +26,7 @@ output states the ratio it ran at (``update_to_data``).
 """
 from __future__ import annotations
 
+import collections
 import contextlib
 import copy
 import math
@@ -40,6 +41,7 @@ from .qnet import MULTIDISCRETE_POLICY_RESNET, MULTIDISCRETE_RESNET, ReplayBuffe
 
 MEMORY_SIZE = 2000            # Grasping_Agent_multidiscrete.py:26-38
 BATCH_SIZE = 12
+BASELINE_GRASPS = 256         # of objective="policy": earlier grasps that a reward is compared with
 LEARNING_RATE = 0.001
 EPS_START, EPS_END, EPS_DECAY = 1.0, 0.2, 8000
 
@@ -286,7 +288,7 @@ class BatchedGraspAgent:
                  eps_end=EPS_END, eps_decay=EPS_DECAY, seed=20, load_path=None, first_scene_id=0, n_total=None, transitions_per_update=1,
                  max_updates_per_round=64, pipeline_groups=1, objective="q", activations=None, policy_options=None, **env_kwargs):
         # objective: "q" is the reference's (epsilon-greedy on a Q map, binary cross entropy from a replay buffer); "policy" samples the actions of a stochastic policy over the table's
-        # pixels and trains it on its own rounds (PolicyLearner, policy_options: its keyword arguments; advantage = reward minus the round's mean). activations="int8": 8-bit checkpoints.
+        # pixels and trains it on its own rounds (PolicyLearner, policy_options: its keyword arguments; advantages: _advantage). activations="int8": 8-bit checkpoints.
         if objective not in ("q", "policy"):
             raise ValueError(f"objective must be 'q' or 'policy', not {objective!r}")
         if objective == "policy" and (pipeline_groups > 1 or sharding.collectives_active()):
@@ -347,6 +349,7 @@ class BatchedGraspAgent:
                                    max_updates_per_round, activations)                 # :140-156
             self.memory = self.learner.memory
         self.optimizer = self.learner.optimizer
+        self._rewards = collections.deque()                                              # of the policy's last rounds: (sum, grasps) each (_advantage)
         self.eps_start, self.eps_end, self.eps_decay = eps_start, eps_end, eps_decay
         self.steps_done, self.eps_threshold = 0, eps_start
         # :165-180 / :215-217 / :448-465: how often the greedy policy chose each rotation, and the successes per rotation of greedy and of random actions. Kept as device
@@ -459,6 +462,18 @@ class BatchedGraspAgent:
         self.last_loss = self.learner.learn()
         return self.last_loss
 
+    def _advantage(self, reward):
+        """A scene's reward minus the mean of the rewards that the round's other scenes and the last rounds (BASELINE_GRASPS grasps or the last round alone) brought; the reward itself where there
+        is nothing to compare it with. A scene's own reward has no part in the mean, so the expected gradient does not depend on it; earlier rounds make one for a single scene. Rewards that
+        are all the same give 0 exactly: whole numbers are compared before they are divided (a rest of 1e-8 would be a gradient that Adam stretches to its learning rate)."""
+        r = reward.double()
+        earlier, others, total = self._rewards, sum(n for _, n in self._rewards) + r.numel() - 1, r.sum()
+        advantage = (r * others - (sum(s for s, _ in earlier) + total - r)) / others if others else r
+        earlier.append((total, r.numel()))
+        while sum(n for _, n in earlier) - earlier[0][1] >= BASELINE_GRASPS:
+            earlier.popleft()
+        return advantage.float()
+
     # ------------------------------------------------------------------ the same round with the scene groups pipelined (pipeline_groups > 1)
     def _round_pipelined(self, learn, return_observation):
         import contextlib
@@ -539,7 +554,7 @@ class BatchedGraspAgent:
         rec = torch.stack([self.gids.int(), env_action[:, 0].int(), env_action[:, 1].int(), reward.int()], dim=1)
         outcomes = sharding.gather_outcomes(rec)                                                         # the round's only collective on the rollout side: 16 B per scene
         if self.objective == "policy":
-            advantage = reward.float() - reward.float().mean()
+            advantage = self._advantage(reward)
             losses = self.learner.update(state, action, logp, advantage, mask) if learn else []
             utd = len(losses) / self.N
         else:

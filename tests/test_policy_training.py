@@ -1,9 +1,12 @@
 """Training the grasp policy over rounds (agent.PolicyLearner, BatchedGraspAgent(objective="policy")): what rounds without a signal do, what one scene learns, empty batches, resuming."""
+import collections
+import types
+
 import pytest
 import torch
 
 from mujoco_rl_ur5_amd import qnet
-from mujoco_rl_ur5_amd.agent import BatchedGraspAgent, PolicyLearner
+from mujoco_rl_ur5_amd.agent import BASELINE_GRASPS, BatchedGraspAgent, PolicyLearner
 from mujoco_rl_ur5_amd.envs import GraspEnv
 
 
@@ -35,6 +38,49 @@ def test_rounds_of_one_reward_leave_the_weights(model_it1, n, reward):
         agent.round()
     after = _weights(agent)
     assert float((after - before).norm() / before.norm()) < 1e-5
+
+
+@pytest.mark.gpu
+def test_one_scene_learns_from_a_lone_reward(model_it1):
+    agent = _agent(model_it1, 1, [[0], [0], [1]], learning_rate=1e-5)
+    seen = {}
+    update = agent.learner.update
+    agent.learner.update = lambda state, action, logp, advantage, mask: seen.update(state=state, action=action, logp=logp, advantage=advantage, mask=mask) or update(state, action, logp, advantage, mask)
+    for _ in range(3):
+        agent.round()
+    assert float(seen["advantage"]) > 0.5
+    assert float(agent.learner.log_probs(seen["state"], seen["action"], seen["mask"])) > float(seen["logp"])
+
+
+@pytest.mark.gpu
+def test_advantages_compare_with_the_other_scenes_and_earlier_rounds(model_it1):
+    """Every scene against the mean of the round's other rewards and of what earlier rounds brought, weighted by how many these are: its own reward does not enter, so the gradient has the
+    expected direction whatever the baseline is."""
+    rewards = [[1, 0, 0, 1], [0, 0, 1, 0], [1, 1, 1, 0]]
+    agent = _agent(model_it1, 4, rewards)
+    seen = []
+    agent.learner.update = lambda state, action, logp, advantage, mask: seen.append(advantage.tolist()) or []
+    for _ in rewards:
+        agent.round()
+    before = []
+    for round_rewards, got in zip(rewards, seen):
+        for i, r in enumerate(round_rewards):
+            others = before + round_rewards[:i] + round_rewards[i + 1:]
+            assert abs(got[i] - (r - sum(others) / len(others))) < 1e-6
+        before = before + round_rewards
+
+
+def test_a_baseline_forgets_old_rounds():
+    """Whole rounds are dropped once the later ones hold as many grasps as wanted; the last one always counts."""
+    agent = types.SimpleNamespace(_rewards=collections.deque())
+    advantage = lambda *r: BatchedGraspAgent._advantage(agent, torch.tensor(r, dtype=torch.int32)).tolist()  # noqa: E731
+    assert advantage(1) == [1.0] and advantage(1) == [0.0] and advantage(0) == [-1.0]
+    many = [1] * BASELINE_GRASPS
+    assert advantage(*many)[0] == pytest.approx(1 - (2 + BASELINE_GRASPS - 1) / (3 + BASELINE_GRASPS - 1)) and len(agent._rewards) == 1
+    assert advantage(0) == [-1.0] and len(agent._rewards) == 2
+    for _ in range(BASELINE_GRASPS - 2):
+        advantage(0)
+    assert advantage(0)[0] < 0 and advantage(0) == [0.0] and len(agent._rewards) == BASELINE_GRASPS
 
 
 # ------------------------------------------------------------------ the learner alone
