@@ -234,18 +234,19 @@ class PolicyLearner:
 
     def act(self, state, seed, gids, round_index, mask=None, chunk=256):
         """(action [N], log-probability [N]) drawn for the scenes with global ids ``gids`` (``policy.sample_actions``); ``mask`` [N, H, W] or [N, H * W]: the pixels that may be chosen."""
-        parts = []
         with torch.no_grad():
-            for i in range(0, state.shape[0], chunk):
-                part = slice(i, i + chunk)
-                parts.append(policy.sample_actions(self.logits(state[part]), seed, gids[part], round_index, mask=None if mask is None else mask[part]))
+            parts = [policy.sample_actions(self.logits(state[i:i + chunk]), seed, gids[i:i + chunk], round_index, mask=None if mask is None else mask[i:i + chunk])
+                     for i in range(0, state.shape[0], chunk)]
+        if not parts:
+            return state.new_empty(0, dtype=torch.int64), state.new_empty(0, dtype=torch.float32)
         return torch.cat([a for a, _ in parts]), torch.cat([lp for _, lp in parts])
 
     def log_probs(self, state, action, mask=None, net=None, chunk=256):
         """Log-probabilities [N] of given actions, without a gradient (of another network with ``net``)."""
         with torch.no_grad():
-            return torch.cat([policy.action_log_probs(self.logits(state[i:i + chunk], net), action[i:i + chunk], mask=None if mask is None else mask[i:i + chunk])[0]
-                              for i in range(0, state.shape[0], chunk)])
+            parts = [policy.action_log_probs(self.logits(state[i:i + chunk], net), action[i:i + chunk], mask=None if mask is None else mask[i:i + chunk])[0]
+                     for i in range(0, state.shape[0], chunk)]
+        return torch.cat(parts) if parts else state.new_empty(0, dtype=torch.float32)
 
     def _step(self, logits, grad):
         logits.backward(grad)

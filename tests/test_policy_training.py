@@ -90,6 +90,17 @@ def _learner(**kw):
 
 
 @pytest.mark.gpu
+def test_empty_batches():
+    learner = _learner()
+    state, none = torch.empty(0, 4, 24, 20, device="cuda"), torch.empty(0, dtype=torch.long, device="cuda")
+    for mask in (None, torch.empty(0, 24, 20, dtype=torch.bool, device="cuda")):
+        action, logp = learner.act(state, 9, none, 0, mask)
+        assert action.shape == logp.shape == (0,) and action.dtype == torch.int64 and logp.dtype == torch.float32 and action.is_cuda
+        logp = learner.log_probs(state, none, mask)
+        assert logp.shape == (0,) and logp.dtype == torch.float32 and logp.is_cuda
+
+
+@pytest.mark.gpu
 def test_batches_in_which_no_row_counts_leave_the_weights():
     learner = _learner(batch_size=2)
     state, action, zero = torch.rand(4, 4, 24, 20, device="cuda"), torch.full((4,), -1, device="cuda"), torch.zeros(4, device="cuda")
