@@ -364,6 +364,10 @@ class BatchedGraspAgent:
                 for rot, cnt in dict(checkpoint.get(key, {})).items():
                     if 0 <= int(rot) < self.n_actions_2:
                         self._rot_counts[row, int(rot)] = int(cnt)
+        if checkpoint is not None and objective == "policy":                            # a resumed policy is held to the network that its run started from, and compares rewards with the last rounds'
+            if self.learner.reference is not None and "policy_reference" in checkpoint:
+                self.learner.reference.load_state_dict(checkpoint["policy_reference"])
+            self._rewards.extend((torch.tensor(s, dtype=torch.float64, device=self.device), int(n)) for s, n in checkpoint.get("policy_rewards", ()))
         self.first_scene_id = self.env.first_scene_id                                   # one source of truth: the env's scene range
         self.n_total = self.env.n_total
 
@@ -576,10 +580,16 @@ class BatchedGraspAgent:
     random_rotations_successes = property(lambda self: self._rotation_dict(2))       # :465
 
     def save(self, path):
-        """The reference trainer's checkpoint (Grasping_Agent_multidiscrete.py:560-575), key for key: what ``load_path`` of this class and of the reference's ``Grasp_Agent`` read."""
+        """The reference trainer's checkpoint (Grasping_Agent_multidiscrete.py:560-575), key for key: what ``load_path`` of this class and of the reference's ``Grasp_Agent`` read.
+        objective="policy" adds what its training needs beside the network: the frozen copy of a kl_coef, and the last rounds' rewards."""
+        policy_state = {}
+        if self.objective == "policy":
+            policy_state["policy_rewards"] = [(float(s), n) for s, n in self._rewards]
+            if self.learner.reference is not None:
+                policy_state["policy_reference"] = self.learner.reference.state_dict()
         torch.save({"step": self.steps_done, "model_state_dict": self.policy_net.state_dict(), "optimizer_state_dict": self.optimizer.state_dict(),
                     "epsilon": self.eps_threshold, "greedy_rotations": dict(self.greedy_rotations), "greedy_rotations_successes": dict(self.greedy_rotations_successes),
-                    "random_rotations_successes": dict(self.random_rotations_successes)}, path)
+                    "random_rotations_successes": dict(self.random_rotations_successes), **policy_state}, path)
 
     def _end_round(self, learn, losses, utd, raw, action, reward, skipped, greedy, outcomes):
         self.last_loss = losses[-1] if losses else None

@@ -109,3 +109,34 @@ def test_batches_in_which_no_row_counts_leave_the_weights():
         learner.update(state, action, zero, zero + 1)
     after = torch.cat([p.detach().flatten() for p in learner.policy_net.parameters()])
     assert float((after - before).norm() / before.norm()) < 1e-5
+
+
+# ------------------------------------------------------------------ saving and resuming
+@pytest.mark.gpu
+def test_a_resumed_run_is_held_to_the_policy_it_started_from(model_it1, tmp_path):
+    path = str(tmp_path / "policy.pt")
+    options = dict(policy_options=dict(kl_coef=0.1, batch_size=2))
+    agent = _agent(model_it1, 2, [[1, 0], [0, 0], [0, 1]], **options)
+    start = {k: v.clone() for k, v in agent.learner.reference.state_dict().items()}
+    for _ in range(3):
+        agent.round()
+    agent.save(path)
+    resumed = _agent(model_it1, 2, [[0, 0], [0, 1]], seed=21, load_path=path, **options)
+    kept = resumed.learner.reference.state_dict()
+    assert all(torch.equal(v, kept[k]) for k, v in start.items())
+    assert any(not torch.equal(v, kept[k]) for k, v in resumed.policy_net.state_dict().items())
+    assert not any(p.requires_grad for p in resumed.learner.reference.parameters()) and resumed.optimizer.param_groups[0]["decoupled_weight_decay"]
+    # and the same advantages follow
+    seen = []
+    for a in (agent, resumed):
+        a.env.step_device = lambda action, depth, device=None, sync=True: (torch.tensor([0, 1], dtype=torch.int32, device="cuda"), torch.zeros(2, dtype=torch.bool, device="cuda"))
+        a.learner.update = lambda state, action, logp, advantage, mask: seen.append(advantage.clone()) or []
+        a.round()
+    assert torch.equal(seen[0], seen[1])
+    # a file without them (of a Q run, or of a run without an anchor): the reference is the network that is loaded
+    plain = torch.load(path, map_location="cuda")
+    for key in [k for k in plain if k.startswith("policy")]:
+        del plain[key]
+    torch.save(plain, path)
+    other = _agent(model_it1, 2, [[0, 0]], load_path=path, **options)
+    assert all(torch.equal(v, other.learner.reference.state_dict()[k]) for k, v in other.policy_net.state_dict().items())
