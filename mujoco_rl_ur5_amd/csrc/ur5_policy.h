@@ -561,7 +561,8 @@ struct PairEnd { float margin, w; double term; };
 __device__ __forceinline__ PairEnd pair_end(const Prefer& P, double d) {
   const double mg = P.beta * d, up = 1 / (1 + exp(mg));                      // sigmoid(-margin)
   const double rest = log1p(exp(-fabs(mg)));                                 // softplus(x) = max(x, 0) + this, of margin and -margin
-  return PairEnd{(float)mg, (float)(-P.beta * ((1 - P.eps) * up - P.eps * (1 - up)) / P.pairs), (1 - P.eps) * (fmax(-mg, 0.0) + rest) + P.eps * (fmax(mg, 0.0) + rest)};
+  const double other = P.eps > 0 ? P.eps * (fmax(mg, 0.0) + rest) : 0.0;     // (an infinite margin that has no weight adds nothing)
+  return PairEnd{(float)mg, (float)(-P.beta * ((1 - P.eps) * up - P.eps * (1 - up)) / P.pairs), (1 - P.eps) * (fmax(-mg, 0.0) + rest) + other};
 }
 // long episodes: all rows in a launch of their own, a wavefront each; what a row adds stays in its first record (10 000 rows of 2400 actions in one pair, us a call: 1985 with its
 // workgroup alone, 99 so)

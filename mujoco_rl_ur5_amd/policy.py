@@ -307,7 +307,8 @@ def preference_loss(logits, action, ref_logp, offsets, mask=None, beta=0.1, labe
 
         margin_i = beta (sum over episode 2 i of (logp - ref_logp) - the same over episode 2 i + 1),    loss = mean_i (1 - eps) softplus(-margin_i) + eps softplus(margin_i)
 
-    with eps = ``label_smoothing``. Rows of no episode get a zero gradient."""
+    with eps = ``label_smoothing``. Rows of no episode get a zero gradient. A ref_logp of -inf (an action that the reference rules out) makes its pair's margin infinite; loss and
+    gradient are their limits."""
     return PreferenceLoss(*_PreferenceLoss.apply(logits, _Prefer(logits, action, ref_logp, offsets, mask, beta, label_smoothing)))
 
 
