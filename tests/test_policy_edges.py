@@ -1,4 +1,4 @@
-"""The policy operators at the ends of their ranges: infinite log-probabilities of a reference."""
+"""The policy operators at the ends of their ranges: infinite log-probabilities of a reference, and the longest sums that one thread adds up."""
 import math
 
 import pytest
@@ -41,3 +41,50 @@ def test_a_preference_over_an_action_that_the_reference_rules_out(side, eps, row
     terms = policy.preference_loss(leaf, a, ruled, off, beta=beta, label_smoothing=eps)
     terms.loss.backward()
     assert torch.equal(terms.loss.detach(), got.loss) and torch.equal(terms.margin, got.margin) and torch.equal(leaf.grad, grad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(16, 16384, 1, 8), (8, 40000, 1, 9), (64, 4096, 2, 8)])
+def test_the_longest_sums_of_a_thread(shape, dtype):
+    """Up to 64 turns of 8 values, and one more where the mask's length is no multiple of 8: 520 terms in 32 bits, 520 x 2^-24 of their sum at the worst, and 1.4e-6 of each term by the
+    hardware's 2^x within 20 of the maximum; everything after that is 64 bits wide."""
+    n, maps, h, w = shape
+    LONG = 520 * 2.0 ** -24 + 1.4e-6
+    g = torch.Generator().manual_seed(n)
+    z = (2 * torch.randn(shape, generator=g)).to(dtype).cuda()
+    mask = torch.rand((n, h, w), generator=g) < 0.9
+    mask[:, 0, 0] = True
+    mask = mask.cuda()
+    action = (torch.randint(0, maps, (n,), generator=g) * h * w).cuda()
+    ok = mask[:, None].expand(shape).reshape(n, -1)
+    x = torch.where(ok, z.reshape(n, -1).double(), -math.inf)
+    lp = torch.log_softmax(x, 1)
+    p, inside = lp.exp(), torch.where(ok, lp, 0.0)
+    h64 = -(p * inside).sum(1)
+    logp, entropy = policy.action_log_probs(z, action, mask)
+    want = lp.gather(1, action[:, None])[:, 0]
+    assert ((logp.double() - want).abs() <= LONG + want.abs() * 2.0 ** -24).all()
+    assert ((entropy.double() - h64).abs() <= LONG * (1 + h64) + h64 * 2.0 ** -24).all()
+    drawn, drawn_logp = policy.sample_actions(z, 3, torch.arange(n).cuda(), 0, mask)
+    want = lp.gather(1, drawn[:, None])[:, 0]
+    assert ok.gather(1, drawn[:, None]).all() and ((drawn_logp.double() - want).abs() <= LONG + want.abs() * 2.0 ** -24).all()
+    old, adv = logp - 0.1, torch.ones(n).cuda()
+    ref = (z.float() + 0.5 * torch.randn(shape, generator=g).cuda()).to(dtype)
+    y = torch.where(ok, ref.reshape(n, -1).double(), -math.inf)
+    apart = torch.where(ok, lp - torch.log_softmax(y, 1), 0.0)
+    kl = (p * apart).sum(1)
+    scale = 4096.0
+    terms, grad = policy.clipped_policy_grad(z, action, old, adv, mask, ref, kl_coef=0.5, entropy_coef=0.01, grad_scale=scale)
+    # |z - q| stays below 4; a KL is a sum of terms of that size
+    assert ((terms.kl.double() - kl).abs() <= 4 * LONG + kl * 2.0 ** -24).all()
+    ratio = torch.exp(lp.gather(1, action[:, None])[:, 0] - old.double())
+    take = torch.where(ratio <= 1.2, -ratio, 0.0)
+    one = torch.zeros_like(p).scatter_(1, action[:, None], take[:, None])
+    parts = [(-take)[:, None].expand_as(p), 0.5 * (apart - kl[:, None]), 0.01 * (inside + h64[:, None])]
+    exact = (p * sum(parts) + one) * scale / n
+    made_of = (p * (sum(t.abs() for t in parts) + 0.5 * 4 + 0.01 * 20) + one.abs()) * scale / n
+    half = torch.finfo(dtype).eps / 2
+    # a probability is 2 LONG off, the sum it is multiplied with one more, and the rounding to the type is half a step, or half of the smallest
+    tol = 5 * LONG * made_of + exact.abs() * half * (1 + 1e-3) + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    assert ((grad.reshape(n, -1).double() - exact).abs() <= tol).all()
