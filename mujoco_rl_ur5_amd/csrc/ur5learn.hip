@@ -144,6 +144,10 @@ void prefer_pairs(const Rows& R, int dtype, hipStream_t s, const Prefer& P, cons
 }
 // rows that the gradient's workgroups end by themselves: FEW, or as many fewer as a lane has records of one
 bool few(const Rows& R) { return R.rows * (((int64_t)R.pieces + 63) / 64) <= FEW; }
+// The preference loss: a workgroup ends every row of its pair, its wavefronts a quarter each. Rows of up to 64 records gain to the edge of the rule (24 rows of 6 x 40 x 40 in one pair, two
+// launches and three: 18.7 and 21.5 us a call, 14.7 and 15.4 in a graph; 24 f16 rows of 131 x 93 18.8, 21.6, 15.3, 17.2). Rows of more than that only in short pairs: 8 fp32 rows of
+// 6 x 200 x 200 (120 records) in one pair 18.2 and 21.0 (16.1 and 14.6 in a graph), 12 rows in three 18.4 and 20.8 (18.0, 17.6), but 12 in one 25.1 and 21.1 (25.3, 19.5).
+bool few_pairs(const Rows& R, int64_t pairs) { return few(R) && pairs <= FEW && (R.pieces <= 64 || R.rows <= 8 || R.rows <= 4 * pairs); }
 // a call over more memory than the caches hold
 bool past_caches(const Rows& R, int dtype) { return (int64_t)R.rows * R.actions * (dtype == UR5_F32 ? 4 : 2) * (R.ref ? 3 : 2) > CACHE_BYTES; }
 void gradient(Rows R, int dtype, hipStream_t s, const Terms& t, const int64_t* action, const Work& w, float scale, const float* upstream, void* grad) {
@@ -277,7 +281,7 @@ int ur5_policy_prefer_loss_grad(const ur5_rows* r, const ur5_prefer* p, float* l
   R.ref = nullptr;
   ON(r->device);
   const hipStream_t s = (hipStream_t)r->stream;
-  if (R.rows && few(R) && p->pairs <= FEW && !past_caches(R, r->dtype)) {
+  if (R.rows && few_pairs(R, p->pairs) && !past_caches(R, r->dtype)) {
     const Prefer P = prefer_of(p);
     const int pieces = R.pieces;
     stats(R, r->dtype, s, Span{P.offsets, 2 * P.pairs}, P.action, w);

@@ -88,3 +88,20 @@ def test_the_longest_sums_of_a_thread(shape, dtype):
     # a probability is 2 LONG off, the sum it is multiplied with one more, and the rounding to the type is half a step, or half of the smallest
     tol = 5 * LONG * made_of + exact.abs() * half * (1 + 1e-3) + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
     assert ((grad.reshape(n, -1).double() - exact).abs() <= tol).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,ends", [(8, [0, 5, 8]), (9, [0, 2, 9]), (12, [0, 1, 4, 6, 7, 9, 12]), (12, [0, 3, 6, 9, 12]), (12, [0, 12, 12])])
+def test_preferences_of_long_rows_on_both_sides_of_the_rule_for_few(rows, ends):
+    """Rows of more than 64 records, in pairs that the gradient ends by itself and in longer ones: the bits of the form that takes the gradient later, which always ends them first."""
+    g = torch.Generator().manual_seed(rows)
+    z = (2 * torch.randn(rows, 6, 200, 200, generator=g)).cuda()
+    mask = (torch.rand(rows, 200, 200, generator=g) < 0.5).cuda()
+    mask[:, 0, 0] = True
+    action = torch.zeros(rows, dtype=torch.long).cuda()
+    rl, off = policy.action_log_probs(z, action, mask)[0] + 0.5 * torch.randn(rows, generator=g).cuda(), torch.tensor(ends).cuda()
+    got, grad = policy.preference_grad(z, action, rl, off, mask, beta=0.4, label_smoothing=0.1)
+    leaf = z.clone().requires_grad_()
+    terms = policy.preference_loss(leaf, action, rl, off, mask, beta=0.4, label_smoothing=0.1)
+    terms.loss.backward()
+    assert torch.equal(terms.loss.detach(), got.loss) and torch.equal(terms.margin, got.margin) and torch.equal(leaf.grad, grad)
