@@ -204,7 +204,8 @@ def _is_parameter(t):
 _PRODUCTS = frozenset([torch.matmul, torch.mm, torch.bmm, torch.addmm, torch.baddbmm, torch.einsum] + [getattr(torch.Tensor, name) for name in "matmul __matmul__ __rmatmul__ mm bmm addmm baddbmm".split()])
 _LAYERS = frozenset(getattr(module, name) for module, names in (
     (F, "conv1d conv2d conv3d conv_transpose1d conv_transpose2d conv_transpose3d linear batch_norm instance_norm group_norm layer_norm max_pool1d max_pool2d max_pool3d avg_pool1d avg_pool2d "
-        "avg_pool3d adaptive_avg_pool1d adaptive_avg_pool2d adaptive_avg_pool3d adaptive_max_pool1d adaptive_max_pool2d adaptive_max_pool3d"),
+        "avg_pool3d adaptive_avg_pool1d adaptive_avg_pool2d adaptive_avg_pool3d adaptive_max_pool1d adaptive_max_pool2d adaptive_max_pool3d max_pool1d_with_indices max_pool2d_with_indices "
+        "max_pool3d_with_indices adaptive_max_pool1d_with_indices adaptive_max_pool2d_with_indices adaptive_max_pool3d_with_indices"),
     (torch, "batch_norm instance_norm group_norm layer_norm max_pool1d max_pool2d max_pool3d")) for name in names.split())
 
 

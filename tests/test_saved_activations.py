@@ -71,7 +71,7 @@ def test_a_network_whose_maps_lie_near_their_ends(shift):
 
 LAYERS = {"conv2d": lambda x: F.conv2d(x, torch.ones(3, 16, 3, 3, device=x.device, requires_grad=True)), "matmul": lambda x: x.flatten(0, 1) @ torch.ones(64, 20, 5, device=x.device, requires_grad=True),
           "batch_norm": lambda x: nn.BatchNorm2d(16).to(x.device)(x),
-          "group_norm": lambda x: nn.GroupNorm(4, 16).to(x.device)(x), "layer_norm": lambda x: F.layer_norm(x, (20,)), "max_pool2d": lambda x: nn.MaxPool2d(2)(x),
+          "group_norm": lambda x: nn.GroupNorm(4, 16).to(x.device)(x), "layer_norm": lambda x: F.layer_norm(x, (20,)), "max_pool2d": lambda x: nn.MaxPool2d(2)(x), "max_pool2d_indices": lambda x: nn.MaxPool2d(2, return_indices=True)(x)[0],
           "conv_transpose2d": lambda x: nn.ConvTranspose2d(16, 3, 2).to(x.device)(x)}
 
 
