@@ -225,8 +225,8 @@ class _Functions(TorchFunctionMode):
 
 class saved_activations:
     """Context manager for a forward pass: the inputs of convolutions, matrix products, normalisations and poolings that autograd saves inside it -- floating-point GPU tensors of three or more
-    dimensions and at least ``min_values`` values -- are kept as 8-bit checkpoints, where those are smaller, and restored when their backward runs. What other functions save (a sigmoid's or
-    softmax's output, a logarithm's argument) is kept as it is, and so are a layer's weights and parameters (leaves that want a gradient, frozen nn.Parameters), views of them and
+    dimensions and at least ``min_values`` values -- are kept as 8-bit checkpoints, where those are smaller, and restored when their backward runs. What other functions save (a sigmoid's,
+    softmax's or plain ReLU's output, a logarithm's argument) is kept as it is, and so are a layer's weights and parameters (leaves that want a gradient, frozen nn.Parameters), views of them and
     autocast's copies of the former; a factor of a product that is computed from parameters is an activation here. In it, ``qnet``'s pointwise convolutions keep theirs for ``weight_grad`` and its ReLUs which values are positive (``relu``).
 
     A normalisation sees its input half a step off: where a group's values lie close together and far from 0, that is more of their spread than of themselves. What is kept must not be

@@ -130,7 +130,7 @@ template <typename T, typename Past> __global__ void __launch_bounds__(THREADS) 
 }
 
 // ---- ReLU whose backward pass needs a bit per value: 64 neighbouring lanes hold 64 PER values, word i of theirs has a bit per lane, for value i of each. Bound by memory: 2 x 4 (2)
-// + 1/8 bytes per value in both directions (41 M fp32 values, one MI355X: 53 us each way, 6.3 TB/s).
+// + 1/8 bytes per value in both directions (41 M fp32 values, one MI355X: 54 us each way, 6.2 TB/s; bf16 30 and 33 us).
 template <typename T> struct Run { long long at; int left; long long word; };   // this thread's values: the first, how many exist, and the first word of its wavefront
 template <typename T> __device__ __forceinline__ Run<T> run_of(int k, long long count) {
   const long long wave = ((long long)blockIdx.x * 2 + k) * (THREADS / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -198,8 +198,11 @@ template <typename T, typename Past> __global__ void __launch_bounds__(THREADS) 
 // them: lane l holds channel l % 32 and pixels 32 (l / 32) .. + 31 of the group (the order of the pixels is free as long as both operands agree). Two buffers in LDS: while
 // the matrix instructions run over group g, group g + 1 is cut into the other buffer and group g + 2 is on its way; one barrier per group.
 // Ranges are `splits` in number, and ur5_act8_wgrad_sum adds their parts in order: no atomics, the same result every time.
-// 12 images of 64 -> 128 channels and 100 x 100 fp32 pixels: 22 us, 4 TB/s, bound by memory. 64 images of 256 -> 512 and 50 x 50: 145 us (868 TFLOP/s of the three bf16
-// products; 183 us, 690, once the card holds its power by its clock): bound by the matrix instructions and the vector instructions that cut, convert and scale between them.
+// 12 images of 64 -> 128 channels and 100 x 100 fp32 pixels: 21 us (bf16 16). 61 MB of gradients and 8 MB of codes are 3.3 TB/s; 75 MB are fetched and 8 MB of parts written, 3.9. A
+// workgroup's 99 KB of LDS leave one per CU, it has seven or eight groups in all, and one of them on its way: latency, not the memory's rate.
+// 64 images of 256 -> 512 and 50 x 50: 148 us at 2.1 GHz, 176 in a loop, where the card holds its power by its clock (2.1 -> 1.75 GHz); the cycles are the same 310 k. The three bf16 products
+// are 123 k of them per SIMD, the vector instructions that cut, convert and scale another 118 k, LDS reads about 60 k, and they add up instead of overlapping: the matrix pipes are busy for 44 %
+// of a CU's busy cycles. (bf16 gradients, a third of the products and two thirds of the vector instructions: 108 and 115 us.)
 typedef float F16 __attribute__((ext_vector_type(16)));
 typedef __bf16 B8 __attribute__((ext_vector_type(8)));
 typedef _Float16 H8 __attribute__((ext_vector_type(8)));

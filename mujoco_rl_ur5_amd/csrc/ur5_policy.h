@@ -367,7 +367,7 @@ template <typename T, bool MASK, bool REF, bool ENTROPY> __device__ __forceinlin
 // ---- what both losses have in common. Per row, dL/dz_j = p_j (c0 + kl (z_j - q_j - gap) + entropy (z_j - m - level)) + [j = action] take; p_j = exp(z_j - m) rs.
 // Three launches: statistics of the pieces -- a Slope per row and a term per row or pair of the loss -- the gradient, of which the first workgroup adds the terms up.
 // (Joining a row's records in every workgroup of the gradient saves a launch and costs each of them 3 us of double arithmetic before its first load: ur5_policy_clip_few.)
-// Bound by memory where rows are many -- 513 masked bf16 rows of 6 x 200 x 200 with their reference: 71 + 5 + 91 us; the mask's runs end inside 128-byte lines, 281 MB are
+// Bound by memory where rows are many -- 513 masked bf16 rows of 6 x 200 x 200 with their reference: 71 + 5 + 89 us; the mask's runs end inside 128-byte lines, 281 MB are
 // fetched for 199 MB of allowed logits --, by the latency of the launches where they are few (12 fp32 rows: 9 + 14 us).
 struct Slope { float m, rs, c0, kl, gap, entropy, level, take; int on; };   // on: the row counts; anything else is unset where it does not
 struct Span { const int64_t* ends; int last; };   // the preference loss: rows outside [ends[0], ends[last]) belong to no episode and do not count; ends == null: all rows
