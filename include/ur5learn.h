@@ -67,7 +67,7 @@ typedef struct ur5_prefer {
   const float* upstream;
 } ur5_prefer;
 /* loss[1] = mean over pairs of (1 - eps) softplus(-margin) + eps softplus(margin), margin = beta ((preferred episode's sum of logp - ref_logp) - (the other's)); margin [pairs].
-   Rows that do not count, or belong to no episode, add nothing. */
+   Rows that do not count, or belong to no episode, add nothing. A ref_logp of -inf makes its pair's margin infinite; loss and gradient are then their limits. */
 int ur5_policy_prefer_loss(const ur5_rows* r, const ur5_prefer* p, float* loss, float* margin);
 int ur5_policy_prefer_grad(const ur5_rows* r, const ur5_prefer* p, void* grad);
 /* both at once, in two (few rows and pairs), three or four (long episodes) launches. */
